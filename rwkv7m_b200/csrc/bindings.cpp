@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <climits>
 #include <cstdio>
 #include <cstdlib>
 #include <map>
@@ -235,6 +236,124 @@ std::vector<Tensor> gemm_ce_stats(const Tensor& A, const Tensor& B, const Tensor
   rk::ce_combine(stats.data_ptr<float>(), (int)tiles, lse.data_ptr<float>(), maxv.data_ptr<float>(), argmax.data_ptr<int>(),
                  nll.data_ptr<float>(), (int)M, stream());
   return {lse, maxv, argmax, nll};
+}
+
+// ---- distribution over the vocabulary -------------------------------------------------
+
+void check_logits(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.size(1) >= 1 && (t.stride(1) == 1 || t.size(1) == 1) &&
+                  (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat),
+              name, " must be a bf16 or fp32 CUDA matrix with contiguous rows");
+  TORCH_CHECK(t.size(0) <= INT_MAX && t.size(1) <= (1 << 30), name, ": too many rows or columns");
+}
+const Tensor& check_rows(const Tensor& t, const Tensor& like, at::ScalarType type, std::vector<int64_t> sizes, const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.is_contiguous() && t.scalar_type() == type && t.sizes() == at::IntArrayRef(sizes),
+              name, ": wrong device, dtype, shape or layout");
+  return t;
+}
+const float* rows_ptr(const c10::optional<Tensor>& t, const Tensor& like, int64_t rows, const char* name) {
+  if (!t.has_value() || !t->defined()) return nullptr;
+  return check_rows(*t, like, at::kFloat, {rows}, name).data_ptr<float>();
+}
+
+// logits [R, V], ids int32 [R] -> stats [R, 2], logprob [R], entropy [R], and with top_k > 0 top_ids, top_logprobs [R, k]
+std::vector<Tensor> token_logprobs_fwd(const Tensor& logits, const Tensor& ids, int64_t top_k, double tau) {
+  check_logits(logits, "logits");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t R = logits.size(0), V = logits.size(1);
+  check_rows(ids, logits, at::kInt, {R}, "ids");
+  TORCH_CHECK(top_k >= 0 && top_k <= 64 && top_k <= V, "top_k must be between 0 and 64 and at most the vocabulary");
+  auto f32 = logits.options().dtype(at::kFloat);
+  Tensor stats = torch::empty({R, 2}, f32), logprob = torch::empty({R}, f32), entropy = torch::empty({R}, f32);
+  std::vector<Tensor> out = {stats, logprob, entropy};
+  rk::RowStatsArgs a{};
+  a.logits = logits.data_ptr(); a.is_bf16 = logits.scalar_type() == at::kBFloat16; a.ld = logits.stride(0);
+  a.rows = (int)R; a.V = (int)V; a.tau = (float)tau; a.inv_tau = (float)(1.0 / tau);
+  a.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  a.entropy = entropy.data_ptr<float>(); a.ids = ids.data_ptr<int>(); a.logprob = logprob.data_ptr<float>();
+  a.top_k = (int)top_k;
+  if (top_k > 0) {
+    out.push_back(torch::empty({R, top_k}, f32.dtype(at::kInt)));
+    out.push_back(torch::empty({R, top_k}, f32));
+    a.top_ids = out[3].data_ptr<int>(); a.top_logprobs = out[4].data_ptr<float>();
+  }
+  TORCH_CHECK(rk::row_stats(a, stream()) == 0, "token_logprobs launch failed");
+  return out;
+}
+
+// Gradient with respect to the logits of sum_j w[r, j] ln q[ids[r, j]] + g_entropy H; see kernels.h for the scaling of w.
+Tensor logits_grad(const Tensor& logits, const Tensor& stats, const Tensor& ids, const Tensor& w, double tau, double weight_mul,
+                   const c10::optional<Tensor>& entropy, const c10::optional<Tensor>& g_entropy,
+                   const c10::optional<Tensor>& g_scale, const c10::optional<Tensor>& mask) {
+  check_logits(logits, "logits");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t R = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(ids.dim() == 2, "ids must be [rows, K]");
+  const int64_t K = ids.size(1);
+  check_rows(stats, logits, at::kFloat, {R, 2}, "stats");
+  check_rows(ids, logits, at::kInt, {R, K}, "ids");
+  check_rows(w, logits, at::kFloat, {R, K}, "weights");
+  rk::RowGradArgs a{};
+  a.logits = logits.data_ptr(); a.is_bf16 = logits.scalar_type() == at::kBFloat16; a.ld = logits.stride(0);
+  a.rows = (int)R; a.V = (int)V; a.inv_tau = (float)(1.0 / tau); a.weight_mul = (float)weight_mul;
+  a.stats = reinterpret_cast<const float2*>(stats.data_ptr<float>());
+  a.g_entropy = rows_ptr(g_entropy, logits, R, "g_entropy");
+  a.entropy = rows_ptr(entropy, logits, R, "entropy");
+  TORCH_CHECK(a.g_entropy == nullptr || a.entropy != nullptr, "logits_grad: an entropy gradient needs the entropy");
+  a.g_scale = rows_ptr(g_scale, logits, 1, "g_scale");
+  a.mask = rows_ptr(mask, logits, R, "mask");
+  a.K = (int)K; a.ids = ids.data_ptr<int>(); a.w = w.data_ptr<float>();
+  Tensor d = torch::empty({R, V}, logits.options());
+  a.dlogits = d.data_ptr(); a.ldd = V;
+  TORCH_CHECK(rk::row_grad(a, stream()) == 0, "logits_grad launch failed");
+  return d;
+}
+
+// ids int32 [R, K], logits bf16/fp32 [R, K] -> ids and probabilities sorted by id, {sum p ln p, any} per row
+std::vector<Tensor> teacher_prepare(const Tensor& ids, const Tensor& logits, int64_t V, double tau) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous() &&
+                  (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
+              "teacher logits must be a contiguous bf16 or fp32 CUDA matrix");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t R = logits.size(0), K = logits.size(1);
+  TORCH_CHECK(K >= 1 && K <= 256, "a teacher gives between 1 and 256 alternatives");
+  check_rows(ids, logits, at::kInt, {R, K}, "teacher ids");
+  auto f32 = logits.options().dtype(at::kFloat);
+  Tensor oid = torch::empty({R, K}, f32.dtype(at::kInt)), p = torch::empty({R, K}, f32), row = torch::empty({R, 2}, f32);
+  TORCH_CHECK(rk::teacher_prepare(ids.data_ptr<int>(), logits.data_ptr(), logits.scalar_type() == at::kBFloat16, (int)R, (int)K,
+                                  (int)V, (float)(1.0 / tau), oid.data_ptr<int>(), p.data_ptr<float>(),
+                                  reinterpret_cast<float2*>(row.data_ptr<float>()), stream()) == 0,
+              "teacher_prepare launch failed");
+  return {oid, p, row};
+}
+
+// -> stats [R, 2] and the scalars sum of mask tau^2 KL, sum of mask
+std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& t_ids, const Tensor& t_prob, const Tensor& t_row,
+                                const c10::optional<Tensor>& mask, double tau) {
+  check_logits(logits, "logits");
+  c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t R = logits.size(0), V = logits.size(1), K = t_ids.size(1);
+  check_rows(t_ids, logits, at::kInt, {R, K}, "teacher ids");
+  check_rows(t_prob, logits, at::kFloat, {R, K}, "teacher probabilities");
+  check_rows(t_row, logits, at::kFloat, {R, 2}, "teacher rows");
+  auto f32 = logits.options().dtype(at::kFloat);
+  Tensor stats = torch::empty({R, 2}, f32), loss = torch::empty({R}, f32);
+  Tensor total = torch::empty({}, f32), count = torch::empty({}, f32);
+  rk::RowStatsArgs a{};
+  a.logits = logits.data_ptr(); a.is_bf16 = logits.scalar_type() == at::kBFloat16; a.ld = logits.stride(0);
+  a.rows = (int)R; a.V = (int)V; a.tau = (float)tau; a.inv_tau = (float)(1.0 / tau);
+  a.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  a.mask = rows_ptr(mask, logits, R, "mask");
+  a.K = (int)K; a.t_ids = t_ids.data_ptr<int>(); a.t_prob = t_prob.data_ptr<float>();
+  a.t_row = reinterpret_cast<const float2*>(t_row.data_ptr<float>());
+  a.row_loss = loss.data_ptr<float>();
+  TORCH_CHECK(rk::row_stats(a, stream()) == 0, "distill launch failed");
+  rk::RowTotalsArgs t{};
+  t.count = 2; t.rows = (int)R;
+  t.in[0] = a.row_loss; t.in[1] = a.mask;
+  t.out[0] = total.data_ptr<float>(); t.out[1] = count.data_ptr<float>();
+  TORCH_CHECK(rk::row_totals(t, stream()) == 0, "distill totals launch failed");
+  return {stats, total, count};
 }
 
 // Up to four y_i = act_i(A_i B_i^T) with the same number of rows in one launch (bf16 in, bf16 out).  Returns false, having
@@ -917,6 +1036,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_bwd", &embedding_bwd);
   m.def("ce_fwd", &ce_fwd);
   m.def("gemm_ce_stats", &gemm_ce_stats);
+  m.def("token_logprobs_fwd", &token_logprobs_fwd);
+  m.def("logits_grad", &logits_grad);
+  m.def("teacher_prepare", &teacher_prepare);
+  m.def("distill_fwd", &distill_fwd);
   m.def("ce_bwd", &ce_bwd);
   m.def("dp_step", &dp_step);
   m.def("dp_step_timings", &dp_step_timings);

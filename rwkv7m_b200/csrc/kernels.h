@@ -108,6 +108,44 @@ void ce_combine(const float* stats, int tiles, float* lse, float* maxv, int* arg
 void ce_bwd(void* logits, const int* targets, const float* mask, const float* lse, const float* maxv,
             const int* argmax, const float* g_ce, const float* g_l2, int rows, int V, cudaStream_t st);
 
+// ---- distribution over the vocabulary -------------------------------------------------
+// Statistics of softmax(z / tau) for every row of logits, and whatever of the outputs is asked for (null = not wanted).
+struct RowStatsArgs {
+  const void* logits; bool is_bf16;      // [rows, V], row pitch ld elements, any alignment of the element type
+  int64_t ld;
+  int rows, V;
+  float tau, inv_tau;
+  float2* stats;                         // [rows]: maximum, log2 of the sum of exponentials relative to it
+  float* entropy;                        // [rows]
+  const int* ids; float* logprob;        // [rows]: log-probability of one column each, 0 for an id outside [0, V)
+  int top_k; int* top_ids; float* top_logprobs;   // [rows, top_k], largest first, equal logits by index
+  const float* mask;                     // [rows] or null: rows at zero are not read
+  int K; const int* t_ids; const float* t_prob; const float2* t_row; float* row_loss;   // teacher_prepare's output; distillation loss
+};
+int row_stats(const RowStatsArgs& a, cudaStream_t st);
+// dz_i = 1/tau [ sum_j w_j (i = ids_j) - q_i (sum_j w_j + g_H (H + ln q_i)) ] with w_j = weight_mul g_scale mask w[row, j]
+struct RowGradArgs {
+  const void* logits; void* dlogits; bool is_bf16;
+  int64_t ld, ldd;
+  int rows, V;
+  float inv_tau, weight_mul;
+  const float2* stats;
+  const float* entropy; const float* g_entropy;   // both or neither
+  const float* g_scale;                  // device scalar or null
+  const float* mask;                     // [rows] or null
+  int K; const int* ids; const float* w; // [rows, K] sparse part; ids outside [0, V) are skipped
+};
+int row_grad(const RowGradArgs& a, cudaStream_t st);
+// Teacher's alternatives -> probabilities sorted by id (absent ones last, id INT_MAX), {sum p ln p, any} per row.
+int teacher_prepare(const int* ids, const void* logits, bool logits_bf16, int rows, int K, int V, float inv_tau, int* out_ids,
+                    float* out_p, float2* out_row, cudaStream_t st);
+// *out[i] = sum of in[i] over the rows (the row count where in[i] is null)
+struct RowTotalsArgs {
+  const float* in[4]; float* out[4];
+  int count, rows;
+};
+int row_totals(const RowTotalsArgs& a, cudaStream_t st);
+
 // ---- data-parallel optimizer step over symmetric memory -------------------------------
 constexpr int kMaxRanks = 8;
 struct DpPeers {

@@ -11,6 +11,8 @@ PyTorch bodies on any device and exists for the numerics tests.
 from __future__ import annotations
 
 import contextlib
+import math
+from typing import NamedTuple
 
 import torch
 
@@ -249,6 +251,108 @@ def head_loss(hidden, ln_w, ln_b, head_w, targets, mask, chunk=None, eps=1e-5):
     return totals
 
 
+class TokenLogprobs(NamedTuple):
+    """Scores of the distribution over the vocabulary, one entry per position: log-probability of the given token, entropy
+    in nats, and (with ``top_k > 0``) the most likely ids with their log-probabilities, [..., top_k]."""
+
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor | None = None
+    top_logprobs: torch.Tensor | None = None
+
+
+TOP_K_MAX = 64            # alternatives of token_logprobs
+TEACHER_K_MAX = 256       # alternatives a teacher may give per position
+
+
+def _check_temperature(temperature):
+    t = float(temperature)
+    if not (t > 0.0 and math.isfinite(t)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    return t
+
+
+def _check_vocab_input(name, x, what):
+    if not torch.is_tensor(x) or not x.is_floating_point():
+        raise TypeError(f"{name}: {what} must be a floating-point tensor")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name}: {what} need a last dimension of at least one, got {tuple(x.shape)}")
+    if use_cuda(x) and x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{name}: {what} on a GPU are bfloat16 or float32, got {x.dtype}")
+
+
+def _check_ids(name, ids, shape, device, what="ids"):
+    if not torch.is_tensor(ids) or ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name}: {what} must be an int32 or int64 tensor")
+    if tuple(ids.shape) != tuple(shape):
+        raise ValueError(f"{name}: {what} have shape {tuple(ids.shape)}, expected {tuple(shape)}")
+    if ids.device != device:
+        raise ValueError(f"{name}: {what} are on {ids.device}, expected {device}")
+
+
+def _check_teacher(name, rows_shape, device, teacher_ids, teacher_logits):
+    if not torch.is_tensor(teacher_logits) or not teacher_logits.is_floating_point():
+        raise TypeError(f"{name}: teacher_logits must be a floating-point tensor")
+    if teacher_logits.dim() != len(rows_shape) + 1 or tuple(teacher_logits.shape[:-1]) != tuple(rows_shape):
+        raise ValueError(f"{name}: teacher_logits have shape {tuple(teacher_logits.shape)}, expected {tuple(rows_shape)} "
+                         "and a dimension of alternatives")
+    if not 1 <= teacher_logits.shape[-1] <= TEACHER_K_MAX:
+        raise ValueError(f"{name}: a teacher gives between 1 and {TEACHER_K_MAX} alternatives, got {teacher_logits.shape[-1]}")
+    if teacher_logits.device != device:
+        raise ValueError(f"{name}: teacher_logits are on {teacher_logits.device}, expected {device}")
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: the teacher is not differentiated, detach teacher_logits")
+    _check_ids(name, teacher_ids, teacher_logits.shape, device, "teacher_ids")
+
+
+def _check_mask(name, mask, shape, device):
+    if mask is None:
+        return
+    if not torch.is_tensor(mask) or tuple(mask.shape) != tuple(shape):
+        raise ValueError(f"{name}: mask must be a tensor of shape {tuple(shape)}")
+    if mask.device != device:
+        raise ValueError(f"{name}: mask is on {mask.device}, expected {device}")
+    if mask.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: the mask is not differentiated, detach it")
+
+
+def token_logprobs(logits, ids, *, top_k=0, temperature=1.0) -> TokenLogprobs:
+    """Log-probability of ``ids`` [...] under softmax(``logits`` [..., V] / temperature), its entropy, and the ``top_k`` (at
+    most 64) most likely ids with their log-probabilities, equal logits in the order of their index.
+
+    fp32 results from bf16 or fp32 logits of any row stride.  An id outside the vocabulary (-1 for padding) is no token:
+    log-probability 0, no gradient.  Columns at -inf have probability 0; a row with a NaN or without a finite logit has NaN
+    for every result (ids of alternatives are then unspecified, -1 where there is none).  Differentiable in ``logits``
+    through ``logprob``, ``entropy`` and ``top_logprobs``; on a GPU a row that no gradient reaches gets zeros whatever it
+    holds."""
+    _check_vocab_input("token_logprobs", logits, "logits")
+    _check_ids("token_logprobs", ids, logits.shape[:-1], logits.device)
+    temperature = _check_temperature(temperature)
+    if not isinstance(top_k, int) or not 0 <= top_k <= min(TOP_K_MAX, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: top_k must be an integer between 0 and {min(TOP_K_MAX, logits.shape[-1])}, got {top_k}")
+    if use_cuda(logits):
+        return TokenLogprobs(*_cuda().token_logprobs(logits, ids, top_k, temperature))
+    return TokenLogprobs(*reference.token_logprobs(logits, ids, top_k, temperature))
+
+
+def distill_loss(logits, teacher_ids, teacher_logits, mask=None, *, temperature=1.0):
+    """Distillation from a teacher's top logits: ``(kd_total, kd_count)``, the sum over positions of
+    mask temperature^2 KL(p || softmax(``logits`` [..., V] / temperature)) and the sum of the mask, fp32 scalars.
+
+    p is the softmax of ``teacher_logits`` [..., K] / temperature over the alternatives ``teacher_ids`` [..., K] (1 <= K <=
+    256; log-probabilities serve as well as logits, p does not change with a constant).  An id outside the vocabulary or a
+    logit of -inf marks an absent alternative; an id that occurs twice counts with both.  A position whose mask is 0 or
+    whose teacher is empty adds nothing to ``kd_total`` and gets a zero gradient, whatever its logits hold.  Differentiable
+    in ``logits``."""
+    _check_vocab_input("distill_loss", logits, "logits")
+    _check_teacher("distill_loss", logits.shape[:-1], logits.device, teacher_ids, teacher_logits)
+    _check_mask("distill_loss", mask, logits.shape[:-1], logits.device)
+    temperature = _check_temperature(temperature)
+    if use_cuda(logits):
+        return _cuda().distill_loss(logits, teacher_ids, teacher_logits, mask, temperature)
+    return reference.distill_loss(logits, teacher_ids, teacher_logits, mask, temperature)
+
+
 def screening_scan(mod, q_r, q_w, gate, delta_xh, delta_slot, h_base, state, **scalars):
     """Slot-dependent part of the screening memory, sequential over time."""
     if use_cuda(h_base):
@@ -280,4 +384,7 @@ __all__ = [
     "wkv7",
     "gn_bonus_gate",
     "head_loss",
+    "token_logprobs",
+    "distill_loss",
+    "TokenLogprobs",
 ]

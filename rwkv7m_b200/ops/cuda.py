@@ -12,6 +12,7 @@ from __future__ import annotations
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import reference as R
 from .build import load_extension
@@ -1069,6 +1070,112 @@ def head_loss(hidden, ln_w, ln_b, head_w, targets, mask, chunk=None, eps=1e-5):
         )
         totals = part if totals is None else tuple(a + b for a, b in zip(totals, part))
     return totals
+
+
+# ---------------------------------------------------------------------------
+# The distribution over the vocabulary
+# ---------------------------------------------------------------------------
+
+
+def _vocab_rows(x):
+    """[..., V] as a matrix whose rows are contiguous; a view wherever the strides allow one."""
+    x2 = x.reshape(-1, x.shape[-1])
+    return x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous()
+
+
+def _id_rows(ids, *shape):
+    return ids.reshape(shape).to(torch.int32).contiguous()
+
+
+def _mask_rows(mask):
+    return None if mask is None else mask.detach().reshape(-1).float().contiguous()
+
+
+def _scalar_grad(g):
+    return g.float().reshape(1).contiguous()
+
+
+class TokenLogprobsFn(torch.autograd.Function):
+    """Statistics, log-probability, entropy and alternatives in one pass over the logits; backward one pass more."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, top_k, tau):
+        ctx.set_materialize_grads(False)
+        z = _vocab_rows(logits)
+        idr = _id_rows(ids, -1)
+        out = _C.token_logprobs_fwd(z, idr, top_k, tau)
+        _count()
+        stats, lp, ent = out[:3]
+        top_ids, top_lp = out[3:] if top_k else (None, None)
+        ctx.tau, ctx.shape = tau, logits.shape
+        ctx.save_for_backward(z, idr, stats, ent, top_ids)
+        lead = logits.shape[:-1]
+        res = (lp.view(lead), ent.view(lead))
+        if not top_k:
+            return res + (None, None)
+        top_ids = top_ids.view(*lead, top_k)
+        ctx.mark_non_differentiable(top_ids)
+        return res + (top_ids, top_lp.view(*lead, top_k))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, _g_ids, g_top):
+        z, ids, stats, ent, top_ids = ctx.saved_tensors
+        if g_lp is None and g_ent is None and g_top is None:
+            return None, None, None, None
+        ids = ids.view(-1, 1)
+        w = torch.zeros(ids.shape, device=z.device) if g_lp is None else g_lp.float().reshape(-1, 1).contiguous()
+        if g_top is not None:
+            k = top_ids.shape[-1]
+            ids = torch.cat((ids, top_ids.view(-1, k)), dim=1)
+            w = torch.cat((w, g_top.float().reshape(-1, k)), dim=1)
+        g_ent = None if g_ent is None else g_ent.float().reshape(-1).contiguous()
+        dz = _C.logits_grad(z, stats, ids, w, ctx.tau, 1.0, ent, g_ent, None, None)
+        _count()
+        return dz.view(ctx.shape), None, None, None
+
+
+def token_logprobs(logits, ids, top_k, tau):
+    return TokenLogprobsFn.apply(logits, ids, top_k, tau)
+
+
+def _teacher_rows(teacher_ids, teacher_logits, V, tau):
+    """(ids, p, {sum p ln p, any}) of the teacher's alternatives, sorted by id within each row."""
+    K = teacher_logits.shape[-1]
+    t = teacher_logits.detach().reshape(-1, K)
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        t = t.float()
+    out = _C.teacher_prepare(_id_rows(teacher_ids, -1, K), t.contiguous(), V, tau)
+    _count()
+    return out
+
+
+class DistillLossFn(torch.autograd.Function):
+    """Distillation from logits: the teacher's rows, one pass over the logits, the totals; backward one pass more."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logits, mask, tau):
+        z = _vocab_rows(logits)
+        ids, p, trow = _teacher_rows(teacher_ids, teacher_logits, z.shape[1], tau)
+        msk = _mask_rows(mask)
+        stats, total, count = _C.distill_fwd(z, ids, p, trow, msk, tau)
+        _count(2)
+        ctx.tau, ctx.shape = tau, logits.shape
+        ctx.save_for_backward(z, ids, p, stats, msk)
+        ctx.mark_non_differentiable(count)
+        return total, count
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_kd, _g_count):
+        z, ids, p, stats, msk = ctx.saved_tensors
+        dz = _C.logits_grad(z, stats, ids, p, ctx.tau, -ctx.tau * ctx.tau, None, None, _scalar_grad(g_kd), msk)
+        _count()
+        return dz.view(ctx.shape), None, None, None, None
+
+
+def distill_loss(logits, teacher_ids, teacher_logits, mask, tau):
+    return DistillLossFn.apply(logits, teacher_ids, teacher_logits, mask, tau)
 
 
 def _screen_write_targets(delta_xh, delta_slot, slot_embed, W, dk, dv, tensor_core=False):

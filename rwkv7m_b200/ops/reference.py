@@ -8,6 +8,8 @@ src/rwkv7m/model/nnx_model.py:592-798) and losses (src/rwkv7m/model/losses.py:21
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -224,6 +226,54 @@ def l2wrap_components(logits, factor=L2WRAP_FACTOR):
 def l2wrap_loss(logits, factor=L2WRAP_FACTOR):
     total, count = l2wrap_components(logits, factor=factor)
     return total / count
+
+
+# ---- the distribution over the vocabulary ---------------------------------------------
+
+
+def _wide(x):
+    return x if x.dtype == torch.float64 else x.float()
+
+
+def token_logprobs(logits, ids, top_k=0, temperature=1.0):
+    """(logprob, entropy, top_ids, top_logprobs) of softmax(logits / temperature): the log-probability of ``ids`` (0 where the
+    id lies outside the vocabulary), the entropy in nats and the ``top_k`` most likely columns, equal logits by index."""
+    z = _wide(logits)
+    V = z.shape[-1]
+    logq = torch.log_softmax(z / temperature, dim=-1)
+    idx = ids.long().unsqueeze(-1)
+    inside = (idx >= 0) & (idx < V)
+    lp = torch.where(inside, logq.gather(-1, idx.clamp(0, V - 1)), torch.zeros_like(logq[..., :1])).squeeze(-1)
+    q = logq.exp()
+    entropy = -(q * logq.masked_fill(q == 0, 0.0)).sum(-1)
+    if top_k == 0:
+        return lp, entropy, None, None
+    order = torch.sort(z.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    return lp, entropy, order.to(torch.int32), logq.gather(-1, order)
+
+
+def teacher_distribution(teacher_ids, teacher_logits, vocab_size, temperature=1.0):
+    """(ids, p): softmax of the teacher's top logits over the alternatives that are there.  An id outside the vocabulary or
+    a logit of -inf marks an absent one (p = 0, id 0); a row without any has p = 0 throughout."""
+    t = _wide(teacher_logits) / temperature
+    there = (teacher_ids >= 0) & (teacher_ids < vocab_size) & (t > -math.inf)
+    any_there = there.any(-1, keepdim=True)
+    p = torch.softmax(t.masked_fill(~there, -math.inf).masked_fill(~any_there, 0.0), dim=-1)
+    return torch.where(there, teacher_ids, torch.zeros_like(teacher_ids)).long(), p.masked_fill(~there, 0.0)
+
+
+def distill_loss(logits, teacher_ids, teacher_logits, mask=None, temperature=1.0):
+    """(kd_total, kd_count): the masked sum over rows of temperature^2 KL(teacher's alternatives || softmax(logits /
+    temperature)) and the sum of the mask.  A row whose mask is zero or whose teacher is empty contributes nothing, whatever
+    its logits hold."""
+    z = _wide(logits)
+    ids, p = teacher_distribution(teacher_ids, teacher_logits, z.shape[-1], temperature)
+    weight = torch.ones_like(z[..., 0]) if mask is None else mask.to(z.dtype)
+    used = ((weight != 0) & (p.sum(-1) > 0)).unsqueeze(-1)
+    logq = torch.log_softmax(z.masked_fill(~used, 0.0) / temperature, dim=-1)
+    terms = p * (p.clamp(min=1e-38).log() - logq.gather(-1, ids))
+    rows = torch.where(used & (p > 0), terms, torch.zeros_like(terms)).sum(-1) * (temperature * temperature)
+    return (rows * weight).sum(), weight.sum()
 
 
 def compute_age_mask(ages, cfg):
