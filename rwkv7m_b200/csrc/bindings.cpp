@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <climits>
 #include <cstdio>
 #include <cstdlib>
@@ -354,6 +355,169 @@ std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& t_ids, const
   t.out[0] = total.data_ptr<float>(); t.out[1] = count.data_ptr<float>();
   TORCH_CHECK(rk::row_totals(t, stream()) == 0, "distill totals launch failed");
   return {stats, total, count};
+}
+
+// Through the head: z = H W^T with H bf16 [M, C] and W bf16 [V, C]; z is never written.
+constexpr int64_t kHeadStatsRows = 32768;   // rows whose tile statistics are held at a time: 16 bytes per row and 256 columns
+
+rk::GemmArgs head_gemm(const Tensor& H, const Tensor& W, int64_t r0, int64_t rows, int epilogue, int64_t pair, double tau) {
+  rk::GemmArgs p{};
+  p.A = static_cast<const char*>(H.data_ptr()) + r0 * H.stride(0) * 2;
+  p.B = W.data_ptr();
+  p.lda = (int)H.stride(0); p.ldb = (int)W.stride(0);
+  p.M = (int)rows; p.N = (int)W.size(0); p.K = (int)H.size(1);
+  p.layout = rk::kGemmTN; p.epilogue = epilogue; p.pair = (int)pair;
+  p.error_flag = gemm_error_flag(H.device()).data_ptr<int>();
+  p.vocab.tau = (float)tau; p.vocab.inv_tau = (float)(1.0 / tau); p.vocab.c = (float)(1.4426950408889634 / tau);
+  return p;
+}
+void check_head(const Tensor& H, const Tensor& W, const char* name) {
+  TORCH_CHECK(H.is_cuda() && H.device() == W.device() && H.scalar_type() == at::kBFloat16 && W.scalar_type() == at::kBFloat16 &&
+                  H.dim() == 2 && W.dim() == 2 && H.stride(1) == 1 && W.stride(1) == 1 && H.size(1) == W.size(1) &&
+                  H.size(0) >= 1 && W.size(0) >= 1 && H.size(0) <= INT_MAX && W.size(0) <= (1 << 30),
+              name, ": bf16 row-major hidden states [M, C] and weight [V, C]");
+}
+
+// -> logprob, entropy [M], and for the backward pass stat [M, 4] and the targets' z [M]
+std::vector<Tensor> head_prob_stats(const Tensor& H, const Tensor& W, const Tensor& ids, double tau, int64_t pair) {
+  check_head(H, W, "head_token_logprobs");
+  c10::cuda::CUDAGuard guard(H.device());
+  const int64_t M = H.size(0), V = W.size(0), tiles = (V + 255) / 256;
+  check_rows(ids, H, at::kInt, {M}, "ids");
+  auto f32 = H.options().dtype(at::kFloat);
+  Tensor lp = torch::empty({M}, f32), ent = torch::empty({M}, f32), stat = torch::empty({M, 4}, f32), tz = torch::empty({M}, f32);
+  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32);
+  for (int64_t r = 0; r < M; r += kHeadStatsRows) {
+    const int64_t n = std::min(kHeadStatsRows, M - r);
+    rk::GemmArgs p = head_gemm(H, W, r, n, rk::kEpiProbStats, pair, tau);
+    p.D = buf.data_ptr(); p.ldd = (int)(tiles * 4);
+    p.vocab.target = ids.data_ptr<int>() + r;
+    p.vocab.target_z = tz.data_ptr<float>() + r;
+    const int rc = rk::gemm_bf16(p, stream());
+    TORCH_CHECK(rc == 0, "head_token_logprobs: product launch failed with code ", rc);
+    TORCH_CHECK(rk::head_prob_combine(reinterpret_cast<const float4*>(buf.data_ptr<float>()), (int)tiles, p.vocab.target,
+                                      p.vocab.target_z, (int)n, (int)V, (float)tau, lp.data_ptr<float>() + r,
+                                      ent.data_ptr<float>() + r, reinterpret_cast<float4*>(stat.data_ptr<float>()) + r,
+                                      stream()) == 0,
+                "head_token_logprobs: combine launch failed");
+  }
+  return {lp, ent, stat, tz};
+}
+
+void check_dz(const Tensor& dz, const Tensor& H, const Tensor& W) {
+  TORCH_CHECK(dz.is_cuda() && dz.device() == H.device() && dz.scalar_type() == at::kBFloat16 && dz.dim() == 2 &&
+                  dz.size(0) == H.size(0) && dz.size(1) == W.size(0) && dz.stride(1) == 1 && dz.stride(0) % 8 == 0 &&
+                  dz.stride(0) >= dz.size(1),
+              "gradient buffer: bf16 [rows, V] with a row pitch that is a multiple of 8");
+}
+
+// Gradient of the rows' log-probabilities and entropies with respect to z, into dz (bf16 [M, V], padded row pitch).
+void head_prob_grad(const Tensor& H, const Tensor& W, const Tensor& ids, const Tensor& stat, const Tensor& tz,
+                    const c10::optional<Tensor>& g_lp, const c10::optional<Tensor>& g_ent, double tau, Tensor dz, int64_t pair) {
+  check_head(H, W, "head_token_logprobs");
+  c10::cuda::CUDAGuard guard(H.device());
+  check_dz(dz, H, W);
+  const int64_t M = H.size(0), V = W.size(0);
+  check_rows(ids, H, at::kInt, {M}, "ids");
+  check_rows(stat, H, at::kFloat, {M, 4}, "stat");
+  check_rows(tz, H, at::kFloat, {M}, "target logits");
+  rk::GemmArgs p = head_gemm(H, W, 0, M, rk::kEpiProbGrad, pair, tau);
+  p.D = dz.data_ptr(); p.ldd = (int)dz.stride(0);
+  p.vocab.target = ids.data_ptr<int>();
+  p.vocab.stat = reinterpret_cast<const float4*>(stat.data_ptr<float>());
+  p.vocab.g0 = rows_ptr(g_lp, H, M, "g_logprob");
+  p.vocab.g1 = rows_ptr(g_ent, H, M, "g_entropy");
+  const int rc = rk::gemm_bf16(p, stream());
+  TORCH_CHECK(rc == 0, "head_token_logprobs backward: product launch failed with code ", rc);
+  rk::HeadFix f{};
+  f.dz = p.D; f.ld = dz.stride(0); f.rows = (int)M; f.V = (int)V; f.tau = (float)tau;
+  f.target = p.vocab.target; f.target_z = tz.data_ptr<float>(); f.stat = p.vocab.stat; f.g0 = p.vocab.g0; f.g1 = p.vocab.g1;
+  TORCH_CHECK(rk::head_prob_fix(f, stream()) == 0, "head_token_logprobs backward: launch failed");
+}
+
+// -> scalars ce_total, ce_count, l2_total, l2_count, kd_total, kd_count, then stat [M, 4], weight [M, 2], argmax, target z [M],
+// z of the teacher's alternatives [M, K]
+std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const Tensor& targets, const c10::optional<Tensor>& mask,
+                                       const Tensor& t_ids, const Tensor& t_prob, const Tensor& t_row, double tau, int64_t pair) {
+  check_head(H, W, "head_distill_loss");
+  c10::cuda::CUDAGuard guard(H.device());
+  const int64_t M = H.size(0), V = W.size(0), K = t_ids.size(1), tiles = (V + 255) / 256;
+  check_rows(targets, H, at::kInt, {M}, "targets");
+  check_rows(t_ids, H, at::kInt, {M, K}, "teacher ids");
+  check_rows(t_prob, H, at::kFloat, {M, K}, "teacher probabilities");
+  check_rows(t_row, H, at::kFloat, {M, 2}, "teacher rows");
+  const float* msk = rows_ptr(mask, H, M, "mask");
+  auto f32 = H.options().dtype(at::kFloat);
+  Tensor stat = torch::empty({M, 4}, f32), weight = torch::empty({M, 2}, f32), am = torch::empty({M}, f32.dtype(at::kInt));
+  Tensor tz = torch::empty({M}, f32), cz = torch::empty({M, K}, f32), rows = torch::empty({4, M}, f32);
+  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32);
+  float* rp = rows.data_ptr<float>();
+  for (int64_t r = 0; r < M; r += kHeadStatsRows) {
+    const int64_t n = std::min(kHeadStatsRows, M - r);
+    rk::GemmArgs p = head_gemm(H, W, r, n, rk::kEpiDistillStats, pair, tau);
+    p.D = buf.data_ptr(); p.ldd = (int)(tiles * 4);
+    p.vocab.target = targets.data_ptr<int>() + r;
+    p.vocab.target_z = tz.data_ptr<float>() + r;
+    p.vocab.listed = (int)K;
+    p.vocab.cols = t_ids.data_ptr<int>() + r * K;
+    p.vocab.cols_z = cz.data_ptr<float>() + r * K;
+    const int rc = rk::gemm_bf16(p, stream());
+    TORCH_CHECK(rc == 0, "head_distill_loss: product launch failed with code ", rc);
+    rk::HeadDistillRows a{};
+    a.rows = (int)n; a.V = (int)V; a.K = (int)K; a.tau = (float)tau;
+    a.target = p.vocab.target; a.mask = msk == nullptr ? nullptr : msk + r;
+    a.target_z = p.vocab.target_z; a.cols_z = p.vocab.cols_z; a.t_ids = p.vocab.cols;
+    a.t_prob = t_prob.data_ptr<float>() + r * K;
+    a.t_row = reinterpret_cast<const float2*>(t_row.data_ptr<float>()) + r;
+    a.stat = reinterpret_cast<float4*>(stat.data_ptr<float>()) + r;
+    a.weight = reinterpret_cast<float2*>(weight.data_ptr<float>()) + r;
+    a.argmax = am.data_ptr<int>() + r;
+    a.ce = rp + r; a.l2 = rp + M + r; a.kd = rp + 2 * M + r; a.ce_count = rp + 3 * M + r;
+    TORCH_CHECK(rk::head_distill_combine(reinterpret_cast<const float4*>(buf.data_ptr<float>()), (int)tiles, a, stream()) == 0,
+                "head_distill_loss: combine launch failed");
+  }
+  std::vector<Tensor> out;
+  rk::RowTotalsArgs t{};
+  const float* in[6] = {rp, rp + 3 * M, rp + M, nullptr, rp + 2 * M, msk};
+  t.count = 6; t.rows = (int)M;
+  for (int i = 0; i < 6; ++i) {
+    out.push_back(torch::empty({}, f32));
+    t.in[i] = in[i]; t.out[i] = out[i].data_ptr<float>();
+  }
+  TORCH_CHECK(rk::row_totals(t, stream()) == 0, "head_distill_loss: totals launch failed");
+  for (const Tensor& x : {stat, weight, am, tz, cz}) out.push_back(x);
+  return out;
+}
+
+// Gradient of g_ce ce_total + g_l2 l2_total + g_kd kd_total with respect to z, into dz (bf16 [M, V], padded row pitch).
+void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, const std::vector<Tensor>& saved, const Tensor& t_ids,
+                       const Tensor& t_prob, const c10::optional<Tensor>& g_ce, const c10::optional<Tensor>& g_l2,
+                       const c10::optional<Tensor>& g_kd, double tau, Tensor dz, int64_t pair) {
+  check_head(H, W, "head_distill_loss");
+  c10::cuda::CUDAGuard guard(H.device());
+  check_dz(dz, H, W);
+  TORCH_CHECK(saved.size() == 5, "head_distill_grad: stat, weight, argmax, target logits, listed logits");
+  const int64_t M = H.size(0), V = W.size(0), K = t_ids.size(1);
+  check_rows(targets, H, at::kInt, {M}, "targets");
+  check_rows(t_ids, H, at::kInt, {M, K}, "teacher ids");
+  check_rows(t_prob, H, at::kFloat, {M, K}, "teacher probabilities");
+  rk::GemmArgs p = head_gemm(H, W, 0, M, rk::kEpiDistillGrad, pair, tau);
+  p.D = dz.data_ptr(); p.ldd = (int)dz.stride(0);
+  p.vocab.stat = reinterpret_cast<const float4*>(check_rows(saved[0], H, at::kFloat, {M, 4}, "stat").data_ptr<float>());
+  p.vocab.weight = reinterpret_cast<const float2*>(check_rows(saved[1], H, at::kFloat, {M, 2}, "weight").data_ptr<float>());
+  p.vocab.g0 = rows_ptr(g_ce, H, 1, "g_ce");
+  p.vocab.g1 = rows_ptr(g_kd, H, 1, "g_kd");
+  const int rc = rk::gemm_bf16(p, stream());
+  TORCH_CHECK(rc == 0, "head_distill_loss backward: product launch failed with code ", rc);
+  rk::HeadFix f{};
+  f.dz = p.D; f.ld = dz.stride(0); f.rows = (int)M; f.V = (int)V; f.K = (int)K; f.tau = (float)tau;
+  f.target = targets.data_ptr<int>(); f.stat = p.vocab.stat; f.weight = p.vocab.weight; f.g0 = p.vocab.g0; f.g1 = p.vocab.g1;
+  f.argmax = check_rows(saved[2], H, at::kInt, {M}, "argmax").data_ptr<int>();
+  f.target_z = check_rows(saved[3], H, at::kFloat, {M}, "target logits").data_ptr<float>();
+  f.cols_z = check_rows(saved[4], H, at::kFloat, {M, K}, "listed logits").data_ptr<float>();
+  f.g_l2 = rows_ptr(g_l2, H, 1, "g_l2");
+  f.t_ids = t_ids.data_ptr<int>(); f.t_prob = t_prob.data_ptr<float>();
+  TORCH_CHECK(rk::head_distill_fix(f, stream()) == 0, "head_distill_loss backward: launch failed");
 }
 
 // Up to four y_i = act_i(A_i B_i^T) with the same number of rows in one launch (bf16 in, bf16 out).  Returns false, having
@@ -1040,6 +1204,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("logits_grad", &logits_grad);
   m.def("teacher_prepare", &teacher_prepare);
   m.def("distill_fwd", &distill_fwd);
+  m.def("head_prob_stats", &head_prob_stats);
+  m.def("head_prob_grad", &head_prob_grad);
+  m.def("head_distill_stats", &head_distill_stats);
+  m.def("head_distill_grad", &head_distill_grad);
   m.def("ce_bwd", &ce_bwd);
   m.def("dp_step", &dp_step);
   m.def("dp_step_timings", &dp_step_timings);

@@ -230,6 +230,150 @@ __device__ __forceinline__ void ce_row_update(CeRow& st, const uint32_t (&v)[32]
   for (int j = 0; j < 32; ++j) st.s += __expf(x[j] - st.m);
 }
 
+// ---- vocabulary epilogues: the distribution softmax(z / tau) straight from the fp32 accumulator -------------------------
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// v[off] with a run-time offset: a chain of selects keeps v in registers
+__device__ __forceinline__ float pick32(const uint32_t (&v)[32], int off) {
+  uint32_t x = v[0];
+#pragma unroll
+  for (int j = 1; j < 32; ++j) x = j == off ? v[j] : x;
+  return __uint_as_float(x);
+}
+
+// Running statistics of one row over a tile.  s1 = sum 2^(z c - m c); s2 = sum 2^t t (kEpiProbStats), or the sum at
+// temperature 1 next to s1 at tau (kEpiDistillStats).
+struct VocabRow {
+  float m, s1, s2;
+  int am, k, next, tgt;
+};
+
+template <int EPI>
+__device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, uint32_t (&v)[32], int col0, int N, size_t row, const GemmVocab& g) {
+  if (col0 >= N) return;
+  const bool ragged = col0 + 32 > N;
+  if (ragged) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) if (col0 + j >= N) v[j] = 0xff800000u;
+  }
+  if (st.tgt >= col0 && st.tgt < col0 + 32) g.target_z[row] = pick32(v, st.tgt - col0);
+  if (EPI == kEpiDistillStats) {
+    while (st.next < col0 + 32) {          // the teacher's alternatives come in the order of the columns
+      g.cols_z[row * g.listed + st.k] = pick32(v, st.next - col0);
+      ++st.k;
+      st.next = st.k < g.listed ? g.cols[row * g.listed + st.k] : 0x7fffffff;
+    }
+  }
+  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(v[j]));
+  const float cm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+  if (cm > st.m) {
+    if (st.m != -INFINITY) {
+      const float d = (st.m - cm) * g.c, f = ex2(d);
+      if (EPI == kEpiProbStats) st.s2 = f * (st.s2 + d * st.s1);
+      else st.s2 *= ex2((st.m - cm) * 1.4426950408889634f);
+      st.s1 *= f;
+    }
+    st.m = cm;
+    if (EPI == kEpiDistillStats) {
+      int ci = 31;
+#pragma unroll
+      for (int j = 30; j >= 0; --j) ci = __uint_as_float(v[j]) == cm ? j : ci;   // the lowest column among equal values
+      st.am = col0 + ci;
+    }
+  }
+  const float mc = st.m * g.c, m1 = st.m * 1.4426950408889634f;
+  float a[2] = {0.f, 0.f}, b[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float z = __uint_as_float(v[j]);
+    float t = fmaf(z, g.c, -mc);
+    if (EPI == kEpiProbStats && ragged) t = fmaxf(t, -16384.f);       // 0 * t stays finite past the last column
+    const float e = ex2(t);
+    a[j & 1] += e;
+    if (EPI == kEpiProbStats) b[j & 1] = fmaf(e, t, b[j & 1]);
+    else b[j & 1] += ex2(fmaf(z, 1.4426950408889634f, -m1));
+  }
+  st.s1 += a[0] + a[1];
+  st.s2 += b[0] + b[1];
+}
+
+// Statistics of this thread's row over the 256 columns of a tile, from the accumulator at taddr.
+template <int EPI>
+__device__ __forceinline__ void vocab_stats_tile(uint32_t taddr, int n0, int N, int row, int M, float4* __restrict__ out,
+                                                 const GemmVocab& g) {
+  const bool live = row < M;
+  VocabRow st{-INFINITY, 0.f, 0.f, 0, 0, 0x7fffffff, -1};
+  if (live) {
+    st.tgt = g.target[row];
+    if (EPI == kEpiDistillStats) {
+      const int* cols = g.cols + (size_t)row * g.listed;
+      int lo = 0, hi = g.listed;             // first listed column at or right of this tile
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cols[mid] < n0) lo = mid + 1; else hi = mid;
+      }
+      st.k = lo;
+      if (lo < g.listed) st.next = cols[lo];
+    }
+  }
+#pragma unroll 1
+  for (int c = 0; c < 8; c += 2) {
+    uint32_t v0[32], v1[32];
+    tmem_ld_32x32(taddr + c * 32, v0);
+    tmem_ld_32x32(taddr + c * 32 + 32, v1);
+    tmem_ld_wait();
+    vocab_stats_chunk<EPI>(st, v0, n0 + c * 32, N, (size_t)row, g);
+    vocab_stats_chunk<EPI>(st, v1, n0 + c * 32 + 32, N, (size_t)row, g);
+  }
+  if (live)
+    *out = EPI == kEpiProbStats ? make_float4(st.m, st.s1, st.s2, 0.f) : make_float4(st.m, st.s2, st.s1, __int_as_float(st.am));
+}
+
+// A row's factors of the gradient epilogues: dz = q (A + B log2 q) with log2 q = z c + b, or a1 2^(z log2e + b1) + a 2^(z c + b).
+// A row that nothing flows into has live = false and gets zeros, whatever its z.
+struct VocabCoef { float b, A, B, b1; bool live; };
+
+template <int EPI>
+__device__ __forceinline__ VocabCoef vocab_coef(int row, int M, int N, const GemmVocab& g) {
+  VocabCoef k{0.f, 0.f, 0.f, 0.f, false};
+  if (row >= M) return k;
+  const float4 s = g.stat[row];
+  k.b = -fmaf(s.x, g.c, s.z);
+  if (EPI == kEpiProbGrad) {
+    const int id = g.target[row];
+    const float gl = g.g0 != nullptr && id >= 0 && id < N ? g.g0[row] : 0.f, gh = g.g1 != nullptr ? g.g1[row] : 0.f;
+    k.A = g.inv_tau * (-gl - (gh != 0.f ? gh * s.w : 0.f));
+    k.B = -gh * g.inv_tau * 0.6931471805599453f;
+    k.live = gl != 0.f || gh != 0.f;
+  } else {
+    const float2 w = g.weight[row];
+    k.b1 = -fmaf(s.x, 1.4426950408889634f, s.y);
+    k.B = g.g0 != nullptr ? g.g0[0] * w.x : 0.f;              // cross-entropy
+    k.A = g.g1 != nullptr ? g.g1[0] * w.y * g.tau : 0.f;      // distillation: tau^2 / tau
+    k.live = k.A != 0.f || k.B != 0.f;
+  }
+  return k;
+}
+
+template <int EPI>
+__device__ __forceinline__ void vocab_grad_chunk(uint32_t (&v)[32], const VocabCoef& k, float c) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float z = __uint_as_float(v[j]), l = fmaf(z, c, k.b);
+    float d;
+    if (EPI == kEpiProbGrad) d = ex2(l) * fmaf(k.B, l, k.A);
+    else d = fmaf(k.A, ex2(l), k.B * ex2(fmaf(z, 1.4426950408889634f, k.b1)));
+    v[j] = k.live ? __float_as_uint(d) : 0u;
+  }
+}
+
 // bf16 output through shared memory: the four epilogue warps write their 128 rows x 64 columns (two accumulator chunks
 // per thread = 128 bytes = one row of the box) into a 16 KB staging buffer in the 128-byte-swizzled layout, and one
 // thread hands the box to the copy engine (cp.async.bulk.tensor store), which writes full lines and clips at the matrix
@@ -307,7 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmD, int tma_out,
                  void* __restrict__ Dptr, int M, int N, int K, int ldd, int raster_m, int splits,
-                 const void* __restrict__ aux, int ldaux, int act, int* __restrict__ err) {
+                 const void* __restrict__ aux, int ldaux, int act, const __grid_constant__ GemmVocab vocab,
+                 int* __restrict__ err) {
   using TL = Tile<BN>;
   constexpr int kStages = TL::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -420,7 +565,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     bool ok = true;
     const bool atomic = splits > 1;
     constexpr bool kTwoInput = EPI == kEpiMulSqrt2Bf16 || EPI == kEpiAddBf16;
-    constexpr bool kCanStage = (EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput) && BN >= 64;
+    constexpr bool kVocabGrad = EPI == kEpiProbGrad || EPI == kEpiDistillGrad;     // always staged: the host insists on it
+    constexpr bool kCanStage = (EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput || kVocabGrad) && BN >= 64;
     const bool staged = kCanStage && tma_out != 0;
     const bool issuer = warp == 2 && lane == 0;   // the one thread whose bulk groups track the output stores
     int obuf = 0;
@@ -446,7 +592,11 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
         if (row < M)
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
+      } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
+        vocab_stats_tile<EPI>(t0, n0, N, row, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab);
       } else if constexpr (BN >= 64) {
+        VocabCoef coef;
+        if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
         // two 32-column chunks per round: the second load is in flight while the first chunk is converted and stored
 #pragma unroll 1
         for (int c = 0; c < BN / 32; c += 2) {
@@ -454,6 +604,10 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           tmem_ld_32x32(t0 + c * 32, v0);
           tmem_ld_32x32(t0 + c * 32 + 32, v1);
           tmem_ld_wait();
+          if constexpr (kVocabGrad) {
+            vocab_grad_chunk<EPI>(v0, coef, vocab.c);
+            vocab_grad_chunk<EPI>(v1, coef, vocab.c);
+          }
           if (kCanStage && staged) {
             if (n0 + c * 32 < N) {   // same for all 128 threads
               uint8_t* buf = out_stage + obuf * kOutStageBytes;
@@ -465,7 +619,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               if (issuer) { tma_store_2d(&tmD, buf, n0 + c * 32, m0); tma_store_commit(); }
               obuf ^= 1;
             }
-          } else {
+          } else if constexpr (!kVocabGrad) {
             store_chunk<EPI>(v0, Dptr, row, n0 + c * 32, M, N, ldd, atomic, aux, ldaux, act);
             store_chunk<EPI>(v1, Dptr, row, n0 + c * 32 + 32, M, N, ldd, atomic, aux, ldaux, act);
           }
@@ -702,7 +856,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmD, int tma_out,
                       void* __restrict__ Dptr, int M, int N, int K, int ldd, int raster_m, int splits,
-                      const void* __restrict__ aux, int ldaux, int act, int* __restrict__ err) {
+                      const void* __restrict__ aux, int ldaux, int act, const __grid_constant__ GemmVocab vocab,
+                      int* __restrict__ err) {
   using TL = PairTile;
   constexpr int kStages = TL::kStages;
   constexpr int BN2 = 256;  // tile width of the pair
@@ -824,7 +979,8 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     int acc = 0; uint32_t acc_phase = 0;
     bool ok = true;
     constexpr bool kTwoInput = EPI == kEpiMulSqrt2Bf16 || EPI == kEpiAddBf16;
-    constexpr bool kCanStage = EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput;
+    constexpr bool kVocabGrad = EPI == kEpiProbGrad || EPI == kEpiDistillGrad;
+    constexpr bool kCanStage = EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput || kVocabGrad;
     const bool staged = kCanStage && tma_out != 0;
     const bool issuer = warp == 2 && lane == 0;
     int obuf = 0;
@@ -851,13 +1007,21 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         }
         if (row < M)
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
-      } else
+      } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
+        vocab_stats_tile<EPI>(t0, n0, N, row, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab);
+      } else {
+      VocabCoef coef;
+      if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
 #pragma unroll 1
       for (int c = 0; c < BN2 / 32; c += 2) {   // two chunks per round: the second load overlaps the first chunk's stores
         uint32_t v0[32], v1[32];
         tmem_ld_32x32(t0 + c * 32, v0);
         tmem_ld_32x32(t0 + c * 32 + 32, v1);
         tmem_ld_wait();
+        if constexpr (kVocabGrad) {
+          vocab_grad_chunk<EPI>(v0, coef, vocab.c);
+          vocab_grad_chunk<EPI>(v1, coef, vocab.c);
+        }
         if (kCanStage && staged) {
           if (n0 + c * 32 < N && m0 < M) {   // same for all 128 threads
             uint8_t* buf = out_stage + obuf * kOutStageBytes;
@@ -869,10 +1033,11 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             if (issuer) { tma_store_2d(&tmD, buf, n0 + c * 32, m0); tma_store_commit(); }
             obuf ^= 1;
           }
-        } else {
+        } else if constexpr (!kVocabGrad) {
           store_chunk<EPI>(v0, Dptr, row, n0 + c * 32, M, N, ldd, atomic, aux, ldaux, act);
           store_chunk<EPI>(v1, Dptr, row, n0 + c * 32 + 32, M, N, ldd, atomic, aux, ldaux, act);
         }
+      }
       }
       tc_fence_before();
       __syncwarp();
@@ -1029,10 +1194,12 @@ int launch(const GemmArgs& p, cudaStream_t st) {
   alignas(64) CUtensorMap td = ta;
   int tma_out = 0;
   constexpr bool kTwoInput = EPI == kEpiMulSqrt2Bf16 || EPI == kEpiAddBf16;
-  if ((EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput) && BN >= 64 && tma_store_enabled() &&
+  constexpr bool kVocabGrad = EPI == kEpiProbGrad || EPI == kEpiDistillGrad;
+  if ((EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput || kVocabGrad) && BN >= 64 && (tma_store_enabled() || kVocabGrad) &&
       (reinterpret_cast<uintptr_t>(p.D) & 15) == 0 && p.ldd % 8 == 0 &&
       (!kTwoInput || (p.N % 64 == 0 && (reinterpret_cast<uintptr_t>(p.aux) & 15) == 0 && p.ldaux % 8 == 0)))
     tma_out = make_map(&td, p.D, p.M, p.N, p.ldd, BM) ? 1 : 0;
+  if (kVocabGrad && tma_out == 0) return 2;
   RK_TRACE("maps ok\n");
   auto kern = gemm_bf16_kernel<BN, A_MN, B_MN, EPI>;
   static bool attr_set = false;
@@ -1056,7 +1223,7 @@ int launch(const GemmArgs& p, cudaStream_t st) {
   const int grid = work < sm_count() ? work : sm_count();
   RK_TRACE("attr ok grid=%d smem=%d splits=%d\n", grid, TL::kSmemBytes, splits);
   kern<<<grid, kThreads, TL::kSmemBytes, st>>>(ta, tb, td, tma_out, p.D, p.M, p.N, p.K, p.ldd, raster_rows(p), splits, p.aux,
-                                               p.ldaux, p.act, p.error_flag);
+                                               p.ldaux, p.act, p.vocab, p.error_flag);
   RK_TRACE("launched\n");
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
@@ -1134,10 +1301,12 @@ int launch_pair(const GemmArgs& p, cudaStream_t st) {
   alignas(64) CUtensorMap td = ta;
   int tma_out = 0;
   constexpr bool kTwoInput = EPI == kEpiMulSqrt2Bf16 || EPI == kEpiAddBf16;
-  if ((EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput) && tma_store_enabled() &&
+  constexpr bool kVocabGrad = EPI == kEpiProbGrad || EPI == kEpiDistillGrad;
+  if ((EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput || kVocabGrad) && (tma_store_enabled() || kVocabGrad) &&
       (reinterpret_cast<uintptr_t>(p.D) & 15) == 0 && p.ldd % 8 == 0 &&
       (!kTwoInput || (p.N % 64 == 0 && (reinterpret_cast<uintptr_t>(p.aux) & 15) == 0 && p.ldaux % 8 == 0)))
     tma_out = make_map(&td, p.D, p.M, p.N, p.ldd, BM) ? 1 : 0;
+  if (kVocabGrad && tma_out == 0) return 2;
   auto kern = gemm_bf16_pair_kernel<A_MN, B_MN, EPI>;
   static bool attr_set = false;
   if (!attr_set) {
@@ -1163,7 +1332,7 @@ int launch_pair(const GemmArgs& p, cudaStream_t st) {
   const int work = tiles * splits;
   const int pairs = work < max_pairs ? work : max_pairs;
   kern<<<2 * pairs, kThreads, TL::kSmemBytes, st>>>(ta, tb, td, tma_out, p.D, p.M, p.N, p.K, p.ldd, raster_rows(p), splits,
-                                                    p.aux, p.ldaux, p.act, p.error_flag);
+                                                    p.aux, p.ldaux, p.act, p.vocab, p.error_flag);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
@@ -1176,6 +1345,18 @@ int launch_pair_epi(const GemmArgs& p, cudaStream_t st) {
     case kEpiAccumF32: return launch_pair<A_MN, B_MN, kEpiAccumF32>(p, st);
     case kEpiMulSqrt2Bf16: return launch_pair<A_MN, B_MN, kEpiMulSqrt2Bf16>(p, st);
     case kEpiAddBf16: return launch_pair<A_MN, B_MN, kEpiAddBf16>(p, st);
+  }
+  return 5;
+}
+
+// The vocabulary epilogues: 256-column tiles of either kernel (the pair where a full 256-row tile exists).
+int launch_vocab(const GemmArgs& p, cudaStream_t st) {
+  const bool pair = p.pair != 0 && p.M >= 256 && p.N >= 256 && p.K >= 512;
+  switch (p.epilogue) {
+    case kEpiProbStats: return pair ? launch_pair<0, 0, kEpiProbStats>(p, st) : launch<256, 0, 0, kEpiProbStats>(p, st);
+    case kEpiDistillStats: return pair ? launch_pair<0, 0, kEpiDistillStats>(p, st) : launch<256, 0, 0, kEpiDistillStats>(p, st);
+    case kEpiProbGrad: return pair ? launch_pair<0, 0, kEpiProbGrad>(p, st) : launch<256, 0, 0, kEpiProbGrad>(p, st);
+    case kEpiDistillGrad: return pair ? launch_pair<0, 0, kEpiDistillGrad>(p, st) : launch<256, 0, 0, kEpiDistillGrad>(p, st);
   }
   return 5;
 }
@@ -1432,6 +1613,12 @@ int gemm_bf16(const GemmArgs& p, cudaStream_t st) {
     if (p.error_flag == nullptr) return 7;
     if (p.pair != 0 && p.M >= 256 && p.N >= 256 && p.K >= 512) return launch_pair<0, 0, kEpiCeStats>(p, st);
     return launch<256, 0, 0, kEpiCeStats>(p, st);
+  }
+  if (p.epilogue == kEpiProbStats || p.epilogue == kEpiDistillStats || p.epilogue == kEpiProbGrad || p.epilogue == kEpiDistillGrad) {
+    const bool stats = p.epilogue == kEpiProbStats || p.epilogue == kEpiDistillStats;
+    if (p.layout != kGemmTN || (stats ? (p.ldd & 3) || p.ldd < 4 * ((p.N + 255) / 256) : (p.ldd & 7) || p.ldd < p.N)) return 6;
+    if (p.error_flag == nullptr) return 7;
+    return launch_vocab(p, st);
   }
   const bool two_input = p.epilogue == kEpiMulSqrt2Bf16 || p.epilogue == kEpiAddBf16;
   if (two_input && (p.aux == nullptr || (reinterpret_cast<uintptr_t>(p.aux) & 15) || (p.ldaux & 7))) return 6;

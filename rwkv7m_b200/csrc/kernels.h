@@ -140,11 +140,41 @@ int row_grad(const RowGradArgs& a, cudaStream_t st);
 int teacher_prepare(const int* ids, const void* logits, bool logits_bf16, int rows, int K, int V, float inv_tau, int* out_ids,
                     float* out_p, float2* out_row, cudaStream_t st);
 // *out[i] = sum of in[i] over the rows (the row count where in[i] is null)
+constexpr int kMaxTotals = 6;
 struct RowTotalsArgs {
-  const float* in[4]; float* out[4];
+  const float* in[kMaxTotals]; float* out[kMaxTotals];
   int count, rows;
 };
 int row_totals(const RowTotalsArgs& a, cudaStream_t st);
+// Folds the tiles of kEpiProbStats: log-probability of the target (0 outside the vocabulary), entropy, and the row's
+// {max, -, log2 S, entropy} for the gradient epilogue.
+int head_prob_combine(const float4* tiles, int ntiles, const int* target, const float* target_z, int rows, int V, float tau,
+                      float* logprob, float* entropy, float4* stat, cudaStream_t st);
+// Folds the tiles of kEpiDistillStats into the row's losses (mask included) and what the backward pass needs.
+struct HeadDistillRows {
+  int rows, V, K;
+  float tau;
+  const int* target; const float* mask;                 // mask null = ones
+  const float* target_z; const float* cols_z;           // written by the epilogue
+  const float* t_prob; const float2* t_row; const int* t_ids;   // teacher_prepare's output
+  float4* stat; float2* weight; int* argmax;
+  float *ce, *l2, *kd, *ce_count;                       // [rows]
+};
+int head_distill_combine(const float4* tiles, int ntiles, const HeadDistillRows& a, cudaStream_t st);
+// The listed columns of every row of dz written again with their whole value: dense part plus one-hot terms.
+struct HeadFix {
+  void* dz; int64_t ld;                                 // bf16 [rows, V]
+  int rows, V, K;
+  float tau;
+  const int* target; const float* target_z;
+  const float4* stat;
+  const float *g0, *g1;                                 // as in GemmVocab
+  // distillation only
+  const float2* weight; const int* argmax; const float* g_l2;
+  const int* t_ids; const float* t_prob; const float* cols_z;
+};
+int head_prob_fix(const HeadFix& a, cudaStream_t st);
+int head_distill_fix(const HeadFix& a, cudaStream_t st);
 
 // ---- data-parallel optimizer step over symmetric memory -------------------------------
 constexpr int kMaxRanks = 8;
@@ -253,9 +283,28 @@ enum GemmEpilogue {
   kEpiStoreBf16 = 0, kEpiReluSqBf16 = 1, kEpiStoreF32 = 2, kEpiAccumF32 = 3, kEpiScatterAddBf16 = 4,
   kEpiMulSqrt2Bf16 = 5,   // D = bf16(acc * 2 sqrt(aux)): backward of h = relu(.)^2 fused into the GEMM that produces dh
   kEpiAddBf16 = 6,        // D = bf16(acc + aux): residual add fused into the projection
-  kEpiCeStats = 7         // no matrix output: per (row, 256-column tile) the cross-entropy statistics of the bf16-rounded
+  kEpiCeStats = 7,        // no matrix output: per (row, 256-column tile) the cross-entropy statistics of the bf16-rounded
                           // result (maximum, sum of exp(x - maximum), arg-max column, logit of the row's target if it
                           // lies in the tile) as float4 into D [M, ceil(N / 256), 4]; aux = int32 targets [M].  Layout TN.
+  // The distribution softmax(z / tau) of the fp32 result z, see GemmVocab.  Layout TN.
+  kEpiProbStats = 8,      // no matrix output: per (row, 256-column tile) {max, sum 2^t, sum 2^t t, -} into D as above
+  kEpiDistillStats = 9,   // the same with {max, sum at temperature 1, sum at tau, arg-max column}
+  kEpiProbGrad = 10,      // D = bf16(q (A + B ln q)), the dense part of the gradient with respect to z
+  kEpiDistillGrad = 11    // D = bf16(a1 q_1 + a q_tau)
+};
+// What the vocabulary epilogues read and write besides D, one entry per row of the product.
+struct GemmVocab {
+  float c;                 // log2(e) / tau: t = (z - max) c
+  float inv_tau, tau;
+  int listed;              // columns per row in `cols` (kEpiDistillStats)
+  const int* target;       // [M]: the column whose z goes to target_z (statistics)
+  float* target_z;
+  const int* cols;         // [M, listed] in rising order, INT_MAX where there is none: their z goes to cols_z
+  float* cols_z;
+  const float4* stat;      // [M] gradients: {max, log2 S at temperature 1, log2 S at tau, entropy}
+  const float2* weight;    // [M] kEpiDistillGrad: weights of the cross-entropy and of the distillation term
+  const float* g0;         // upstream gradients: [M] of the log-probability, or the scalar of the cross-entropy; null = 0
+  const float* g1;         //                     [M] of the entropy, or the scalar of the distillation loss; null = 0
 };
 // Target of the kEpiScatterAddBf16 epilogue (GEMM -> reduce-scatter over time in one kernel): rows are [B, T] tokens,
 // rank r owns tokens [r*Tl, (r+1)*Tl) of every batch row and receives them in out[r] laid out [B, Tl, N].
@@ -279,6 +328,7 @@ struct GemmArgs {
   int pair;            // non-zero: use the CTA-pair (cta_group::2) kernel when the shape allows
   int* error_flag;     // device int, set non-zero if a bounded wait ran out
   int decode_kernel;   // non-zero: shapes with M <= 64 (layout kGemmTN) take the swap-AB cluster split-K kernel
+  GemmVocab vocab;     // the vocabulary epilogues only
 };
 int gemm_bf16(const GemmArgs& p, cudaStream_t st);
 // Up to four problems of layout kGemmTN with the bf16 store epilogue (each with its own activation) and the same M in one

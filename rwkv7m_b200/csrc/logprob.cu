@@ -451,26 +451,142 @@ __global__ void __launch_bounds__(256) teacher_prepare_kernel(const int* __restr
   if (lane == 0) out_row[row] = s > 0.f ? make_float2(kLn2 * (s2 * inv - log2_row(s)), 1.f) : make_float2(0.f, 0.f);
 }
 
-// Totals of up to four row vectors in one CTA: a fixed order, sums in 64 bits.
+// Totals of row vectors, one CTA each: a fixed order, sums in 64 bits.
 __global__ void __launch_bounds__(1024) row_totals_kernel(RowTotalsArgs a) {
   __shared__ double sm[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = 0; i < a.count; ++i) {
-    double s = 0.0;
-    if (a.in[i] == nullptr) s = threadIdx.x == 0 ? (double)a.rows : 0.0;
-    else for (int r = threadIdx.x; r < a.rows; r += 1024) s += (double)a.in[i][r];
+  const float* in = a.in[blockIdx.x];
+  double s = 0.0;
+  if (in == nullptr) s = threadIdx.x == 0 ? (double)a.rows : 0.0;
+  else for (int r = threadIdx.x; r < a.rows; r += 1024) s += (double)in[r];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) sm[warp] = s;
+  __syncthreads();
+  if (warp == 0) {
+    s = sm[lane];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) sm[warp] = s;
-    __syncthreads();
-    if (warp == 0) {
-      s = sm[lane];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) *a.out[i] = (float)s;
-    }
-    __syncthreads();
+    if (lane == 0) *a.out[blockIdx.x] = (float)s;
   }
+}
+
+// ---- through the head: folding the tiles of the product's epilogue (one warp per row) -------------------------------------
+
+__global__ void __launch_bounds__(256) head_prob_combine_kernel(const float4* __restrict__ tiles, int ntiles,
+                                                                const int* __restrict__ target, const float* __restrict__ target_z,
+                                                                int rows, int V, float inv_tau, float* __restrict__ logprob,
+                                                                float* __restrict__ entropy, float4* __restrict__ stat) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const float c = kLog2e * inv_tau;
+  Stat st{-INFINITY, 0.f, 0.f};
+  for (int t = lane; t < ntiles; t += 32) {
+    const float4 v = tiles[(size_t)row * ntiles + t];
+    st = merge(st, Stat{v.x, v.y, v.z}, c);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) st = merge(st, shfl_xor(st, o), c);
+  if (lane == 0) {
+    const float l2s = log2_row(st.s1), ln_s = st.s1 > 0.f ? l2s * kLn2 : __int_as_float(0x7fffffff);
+    const float h = ln_s - kLn2 * (st.s2 / st.s1);
+    const int id = target[row];
+    logprob[row] = id >= 0 && id < V ? (target_z[row] - st.m) * inv_tau - ln_s : 0.f;
+    entropy[row] = h;
+    stat[row] = make_float4(st.m, 0.f, l2s, h);
+  }
+}
+
+__global__ void __launch_bounds__(256) head_distill_combine_kernel(const float4* __restrict__ tiles, int ntiles, HeadDistillRows a) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  const float inv_tau = 1.f / a.tau, c = kLog2e * inv_tau;
+  float m = -INFINITY, s = 0.f, st = 0.f;             // sums at temperature 1 and at tau
+  int am = INT_MAX;
+  auto fold = [&](float m2, float s2, float st2, int am2) {
+    const float mm = fmaxf(m, m2);
+    const float d1 = m == -INFINITY ? 0.f : m - mm, d2 = m2 == -INFINITY ? 0.f : m2 - mm;
+    s = s * exp2_fast(d1 * kLog2e) + s2 * exp2_fast(d2 * kLog2e);
+    st = st * exp2_fast(d1 * c) + st2 * exp2_fast(d2 * c);
+    am = m2 > m || (m2 == m && am2 < am) ? am2 : am;
+    m = mm;
+  };
+  for (int t = lane; t < ntiles; t += 32) {
+    const float4 v = tiles[(size_t)row * ntiles + t];
+    fold(v.x, v.y, v.z, __float_as_int(v.w));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    fold(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), __shfl_xor_sync(0xffffffffu, st, o),
+         __shfl_xor_sync(0xffffffffu, am, o));
+  const float l2s1 = log2_row(s), l2st = log2_row(st);
+  float acc = 0.f;
+  for (int j = lane; j < a.K; j += 32) {
+    const float p = a.t_prob[(size_t)row * a.K + j];
+    if (p > 0.f) acc += p * ((a.cols_z[(size_t)row * a.K + j] - m) * inv_tau - l2st * kLn2);
+  }
+  acc = warp_sum(acc);
+  if (lane == 0) {
+    const float w = a.mask != nullptr ? a.mask[row] : 1.f;
+    const float2 tr = a.t_row[row];
+    const int tgt = a.target[row];
+    const float w_ce = tgt >= 0 && tgt < a.V ? w : 0.f, w_kd = tr.y > 0.f ? w : 0.f;
+    a.ce[row] = w_ce != 0.f ? w_ce * (l2s1 * kLn2 - (a.target_z[row] - m)) : 0.f;
+    a.kd[row] = w_kd != 0.f ? w_kd * a.tau * a.tau * (tr.x - acc) : 0.f;
+    a.l2[row] = 0.5e-4f * m * m;
+    a.ce_count[row] = w_ce;
+    a.stat[row] = make_float4(m, l2s1, l2st, 0.f);
+    a.weight[row] = make_float2(w_ce, w_kd);
+    a.argmax[row] = am;
+  }
+}
+
+__global__ void __launch_bounds__(256) head_prob_fix_kernel(HeadFix a) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows || a.g0 == nullptr) return;
+  const int id = a.target[row];
+  const float gl = a.g0[row], gh = a.g1 != nullptr ? a.g1[row] : 0.f;
+  if (id < 0 || id >= a.V || gl == 0.f) return;
+  const float inv_tau = 1.f / a.tau;
+  const float4 s = a.stat[row];
+  const float l = (a.target_z[row] - s.x) * (kLog2e * inv_tau) - s.z;
+  const float A = inv_tau * (-gl - (gh != 0.f ? gh * s.w : 0.f)), B = -gh * inv_tau * kLn2;
+  reinterpret_cast<bf16*>(a.dz)[(size_t)row * a.ld + id] = f2bf(fmaf(exp2_fast(l), fmaf(B, l, A), gl * inv_tau));
+}
+
+// One warp per row.  The teacher's ids are sorted, so equal ones are neighbours and the first of a run writes for all.
+__global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= a.rows) return;
+  const float inv_tau = 1.f / a.tau, c = kLog2e * inv_tau;
+  const float4 s = a.stat[row];
+  const float2 w = a.weight[row];
+  const float g_ce = a.g0 != nullptr ? a.g0[0] * w.x : 0.f, g_kd = a.g1 != nullptr ? a.g1[0] * w.y * a.tau : 0.f;
+  const float g_l2 = a.g_l2 != nullptr ? a.g_l2[0] * 1e-4f * s.x : 0.f;
+  const int tgt = w.x != 0.f ? a.target[row] : -1, am = a.argmax[row];
+  bf16* dz = reinterpret_cast<bf16*>(a.dz) + (size_t)row * a.ld;
+  auto value = [&](int col, float z, float p) {
+    float d = 0.f;
+    if (g_kd != 0.f) d = g_kd * (exp2_fast((z - s.x) * c - s.z) - p);
+    if (g_ce != 0.f) d += g_ce * (exp2_fast((z - s.x) * kLog2e - s.y) - (col == tgt ? 1.f : 0.f));
+    if (col == am) d += g_l2;
+    return f2bf(d);
+  };
+  bool tgt_done = tgt < 0, am_done = false;
+  for (int j0 = 0; j0 < a.K; j0 += 32) {
+    const int j = j0 + lane;
+    const size_t at = (size_t)row * a.K + j;
+    const int id = j < a.K ? a.t_ids[at] : INT_MAX;
+    if (id != INT_MAX && (j == 0 || a.t_ids[at - 1] != id)) {
+      float p = a.t_prob[at];
+      for (int i = 1; j + i < a.K && a.t_ids[at + i] == id; ++i) p += a.t_prob[at + i];
+      dz[id] = value(id, a.cols_z[at], p);
+    }
+    tgt_done = tgt_done || __any_sync(0xffffffffu, id == tgt);
+    am_done = am_done || __any_sync(0xffffffffu, id == am);
+  }
+  if (lane == 0 && !tgt_done) dz[tgt] = value(tgt, a.target_z[row], 0.f);
+  if (lane == 0 && !am_done && am != tgt && am >= 0 && am < a.V) dz[am] = value(am, s.x, 0.f);
 }
 
 }  // namespace
@@ -523,7 +639,32 @@ int teacher_prepare(const int* ids, const void* logits, bool logits_bf16, int ro
 }
 
 int row_totals(const RowTotalsArgs& a, cudaStream_t st) {
-  row_totals_kernel<<<1, 1024, 0, st>>>(a);
+  row_totals_kernel<<<a.count, 1024, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+int head_prob_combine(const float4* tiles, int ntiles, const int* target, const float* target_z, int rows, int V, float tau,
+                      float* logprob, float* entropy, float4* stat, cudaStream_t st) {
+  if (rows <= 0) return 0;
+  head_prob_combine_kernel<<<(rows + 7) / 8, 256, 0, st>>>(tiles, ntiles, target, target_z, rows, V, 1.f / tau, logprob, entropy, stat);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+int head_distill_combine(const float4* tiles, int ntiles, const HeadDistillRows& a, cudaStream_t st) {
+  if (a.rows <= 0) return 0;
+  head_distill_combine_kernel<<<(a.rows + 7) / 8, 256, 0, st>>>(tiles, ntiles, a);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+int head_prob_fix(const HeadFix& a, cudaStream_t st) {
+  if (a.rows <= 0) return 0;
+  head_prob_fix_kernel<<<(a.rows + 255) / 256, 256, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+int head_distill_fix(const HeadFix& a, cudaStream_t st) {
+  if (a.rows <= 0) return 0;
+  head_distill_fix_kernel<<<(a.rows + 7) / 8, 256, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 

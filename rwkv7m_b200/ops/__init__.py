@@ -353,6 +353,51 @@ def distill_loss(logits, teacher_ids, teacher_logits, mask=None, *, temperature=
     return reference.distill_loss(logits, teacher_ids, teacher_logits, mask, temperature)
 
 
+def _check_head(name, hidden, head_w):
+    _check_vocab_input(name, hidden, "hidden states")
+    if not torch.is_tensor(head_w) or not head_w.is_floating_point():
+        raise TypeError(f"{name}: the head's weight must be a floating-point tensor")
+    if head_w.dim() != 2 or head_w.shape[0] < 1 or head_w.shape[1] != hidden.shape[-1]:
+        raise ValueError(f"{name}: the head's weight must be [V, {hidden.shape[-1]}], got {tuple(head_w.shape)}")
+    if head_w.device != hidden.device:
+        raise ValueError(f"{name}: the head's weight is on {head_w.device}, the hidden states are on {hidden.device}")
+    if use_cuda(hidden) and head_w.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{name}: the head's weight on a GPU is bfloat16 or float32, got {head_w.dtype}")
+
+
+def head_token_logprobs(hidden, head_w, ids, *, temperature=1.0):
+    """``(logprob, entropy)`` of :func:`token_logprobs` for the logits ``hidden`` [..., C] @ ``head_w`` [V, C].T, which are not
+    kept: forward reduces them where the product leaves them, in fp32, backward recomputes them.  ``hidden`` is what the head
+    reads (behind the final layer norm).  Differentiable in both."""
+    name = "head_token_logprobs"
+    _check_head(name, hidden, head_w)
+    _check_ids(name, ids, hidden.shape[:-1], hidden.device)
+    temperature = _check_temperature(temperature)
+    if use_cuda(hidden):
+        return _cuda().head_token_logprobs(hidden, head_w, ids, temperature)
+    return reference.token_logprobs(reference.linear(hidden, head_w), ids, 0, temperature)[:2]
+
+
+def head_distill_loss(hidden, head_w, targets, mask, teacher_ids, teacher_logits, *, temperature=1.0):
+    """The loss pieces of :func:`head_loss` and of :func:`distill_loss` in one pass over the head: ``(ce_total, ce_count,
+    l2_total, l2_count, kd_total, kd_count)`` for the logits ``hidden`` [..., C] @ ``head_w`` [V, C].T, which are not kept.
+
+    Cross-entropy (at temperature 1) runs over positions with mask != 0 and a target inside the vocabulary, L2Wrap over
+    every position, distillation (at ``temperature``) over positions with mask != 0 and a teacher that is not empty;
+    ``kd_count`` is the sum of the mask.  ``hidden`` is what the head reads (behind the final layer norm).  Differentiable
+    in ``hidden`` and ``head_w``."""
+    name = "head_distill_loss"
+    _check_head(name, hidden, head_w)
+    lead = hidden.shape[:-1]
+    _check_ids(name, targets, lead, hidden.device, "targets")
+    _check_mask(name, mask, lead, hidden.device)
+    _check_teacher(name, lead, hidden.device, teacher_ids, teacher_logits)
+    temperature = _check_temperature(temperature)
+    if use_cuda(hidden):
+        return _cuda().head_distill_loss(hidden, head_w, targets, mask, teacher_ids, teacher_logits, temperature)
+    return reference.distill_components(reference.linear(hidden, head_w), targets, mask, teacher_ids, teacher_logits, temperature)
+
+
 def screening_scan(mod, q_r, q_w, gate, delta_xh, delta_slot, h_base, state, **scalars):
     """Slot-dependent part of the screening memory, sequential over time."""
     if use_cuda(h_base):
@@ -387,4 +432,6 @@ __all__ = [
     "token_logprobs",
     "distill_loss",
     "TokenLogprobs",
+    "head_token_logprobs",
+    "head_distill_loss",
 ]

@@ -1178,6 +1178,141 @@ def distill_loss(logits, teacher_ids, teacher_logits, mask, tau):
     return DistillLossFn.apply(logits, teacher_ids, teacher_logits, mask, tau)
 
 
+# Rows of the [rows, V] bf16 gradient of the logits that a backward pass through the head holds at a time.
+HEAD_GRAD_ROWS = 8192
+
+
+def _aligned_rows(x):
+    """A bf16 matrix whose base and row pitch suit bulk-tensor copies."""
+    ok = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1] and x.data_ptr() % 16 == 0
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+def _head_operands(hidden, head_w):
+    return _aligned_rows(hidden.detach().reshape(-1, hidden.shape[-1])), _aligned_rows(_compute_weight(head_w))
+
+
+def _head_kernels_apply(hidden):
+    return _bf16(hidden) and GEMM_BACKEND == "tcgen05" and hidden.shape[-1] % 8 == 0 and hidden.numel() > 0
+
+
+def _head_logits(hidden, head_w):
+    """Logits for widths and dtypes without a head kernel: fp32, so nothing is rounded on the way into the softmax."""
+    return hidden.float() @ head_w.float().T
+
+
+def _head_backward(ctx, h2, wc, fill):
+    """dh and dW from the gradient of the logits, which ``fill(begin, end, dz)`` writes chunk by chunk of rows into one
+    buffer.  A single chunk stores dW in the weight's dtype; several accumulate it in fp32, as does a bound main gradient."""
+    w = ctx.weight
+    M, C = h2.shape
+    V = wc.shape[0]
+    dev = h2.device
+    need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+    step = min(HEAD_GRAD_ROWS, M)
+    buf = torch.empty(step, (V + 7) // 8 * 8, dtype=torch.bfloat16, device=dev)
+    dh = torch.empty(M, C, dtype=torch.bfloat16, device=dev) if need_h else None
+    main = getattr(w, "_main_grad", None) if need_w else None
+    if main is not None and main.dtype != torch.float32:
+        main = None
+    dw = None
+    if need_w and main is None:
+        direct = step == M and w.dtype == torch.bfloat16
+        dw = torch.empty(V, C, dtype=torch.bfloat16 if direct else torch.float32, device=dev)
+    for s in range(0, M, step):
+        e = min(M, s + step)
+        dz = buf[: e - s, :V]
+        fill(s, e, dz)
+        if need_h:
+            gemm(dz, wc, dh[s:e], GEMM_NN, EPI_BF16)
+        if main is not None:
+            gemm(dz, h2[s:e], main, GEMM_WGRAD, EPI_ACC_F32)
+        elif need_w:
+            epi = EPI_BF16 if dw.dtype == torch.bfloat16 else (EPI_F32 if s == 0 else EPI_ACC_F32)
+            gemm(dz, h2[s:e], dw, GEMM_WGRAD, epi)
+    return (None if dh is None else dh.view(ctx.h_shape)), (None if dw is None else dw.to(w.dtype))
+
+
+class HeadTokenLogprobsFn(torch.autograd.Function):
+    """Log-probability and entropy through the head.  Forward: one product whose epilogue reduces every 256-column tile of
+    the fp32 logits to (maximum, sum of exponentials, their sum weighted by the exponent), one kernel that folds the tiles.
+    Backward: the same product again with an epilogue that turns the fp32 logits into their gradient, rounded once to bf16
+    as the operand of the two gradient products."""
+
+    @staticmethod
+    def forward(ctx, hidden, head_w, ids, tau):
+        ctx.set_materialize_grads(False)
+        h2, wc = _head_operands(hidden, head_w)
+        idr = _id_rows(ids, -1)
+        lp, ent, stat, tz = _C.head_prob_stats(h2, wc, idr, tau, int(GEMM_PAIR))
+        _count(2)
+        ctx.tau, ctx.weight, ctx.h_shape = tau, head_w, hidden.shape
+        ctx.save_for_backward(h2, wc, idr, stat, tz)
+        return lp.view(ids.shape), ent.view(ids.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent):
+        if g_lp is None and g_ent is None:
+            return None, None, None, None
+        h2, wc, ids, stat, tz = ctx.saved_tensors
+        g_lp, g_ent = (None if g is None else g.float().reshape(-1).contiguous() for g in (g_lp, g_ent))
+
+        def fill(s, e, dz):
+            _C.head_prob_grad(h2[s:e], wc, ids[s:e], stat[s:e], tz[s:e], None if g_lp is None else g_lp[s:e],
+                              None if g_ent is None else g_ent[s:e], ctx.tau, dz, int(GEMM_PAIR))
+            _count(2)
+
+        return _head_backward(ctx, h2, wc, fill) + (None, None)
+
+
+def head_token_logprobs(hidden, head_w, ids, tau):
+    if _head_kernels_apply(hidden):
+        return HeadTokenLogprobsFn.apply(hidden, head_w, ids, tau)
+    return token_logprobs(_head_logits(hidden, head_w), ids, 0, tau)[:2]
+
+
+class HeadDistillLossFn(torch.autograd.Function):
+    """Cross-entropy, L2Wrap and distillation through the head: one product forward (its epilogue also writes the logits of
+    the target and of the teacher's alternatives), three backward, as :class:`HeadTokenLogprobsFn`."""
+
+    @staticmethod
+    def forward(ctx, hidden, head_w, targets, mask, teacher_ids, teacher_logits, tau):
+        ctx.set_materialize_grads(False)
+        h2, wc = _head_operands(hidden, head_w)
+        ids, p, trow = _teacher_rows(teacher_ids, teacher_logits, wc.shape[0], tau)
+        tgt = _id_rows(targets, -1)
+        out = _C.head_distill_stats(h2, wc, tgt, _mask_rows(mask), ids, p, trow, tau, int(GEMM_PAIR))
+        _count(3)
+        ctx.tau, ctx.weight, ctx.h_shape = tau, head_w, hidden.shape
+        ctx.save_for_backward(h2, wc, tgt, ids, p, *out[6:])
+        ctx.mark_non_differentiable(out[1], out[3], out[5])
+        return tuple(out[:6])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_ce, _n0, g_l2, _n1, g_kd, _n2):
+        if g_ce is None and g_l2 is None and g_kd is None:
+            return (None,) * 7
+        h2, wc, tgt, ids, p, *saved = ctx.saved_tensors
+        g_ce, g_l2, g_kd = (None if g is None else _scalar_grad(g) for g in (g_ce, g_l2, g_kd))
+
+        def fill(s, e, dz):
+            _C.head_distill_grad(h2[s:e], wc, tgt[s:e], [x[s:e] for x in saved], ids[s:e], p[s:e], g_ce, g_l2, g_kd, ctx.tau,
+                                 dz, int(GEMM_PAIR))
+            _count(2)
+
+        return _head_backward(ctx, h2, wc, fill) + (None,) * 5
+
+
+def head_distill_loss(hidden, head_w, targets, mask, teacher_ids, teacher_logits, tau):
+    if _head_kernels_apply(hidden):
+        return HeadDistillLossFn.apply(hidden, head_w, targets, mask, teacher_ids, teacher_logits, tau)
+    logits = _head_logits(hidden, head_w)
+    kd = distill_loss(logits, teacher_ids, teacher_logits, mask, tau)
+    return R.distill_components(logits, targets, mask, teacher_ids, teacher_logits, tau, kd=kd)
+
+
 def _screen_write_targets(delta_xh, delta_slot, slot_embed, W, dk, dv, tensor_core=False):
     """D[b,t,m] = tanh(delta_xh[b,t] + delta_slot[m]) and its raw projections PD = D W^T (fp32), with slot_embed Wkw^T
     added on the write-key columns and the slot axis zero-padded to 16 (the layout the scan kernels read).

@@ -276,6 +276,26 @@ def distill_loss(logits, teacher_ids, teacher_logits, mask=None, temperature=1.0
     return (rows * weight).sum(), weight.sum()
 
 
+def distill_components(logits, targets, mask, teacher_ids, teacher_logits, temperature=1.0, kd=None):
+    """(ce_total, ce_count, l2_total, l2_count, kd_total, kd_count) of a block of logits: cross-entropy over the masked
+    positions whose target lies in the vocabulary, L2Wrap over all positions, distillation (``kd``: the pair, if it has been
+    computed already)."""
+    z = _wide(logits)
+    V = z.shape[-1]
+    idx = targets.long().unsqueeze(-1)
+    inside = ((idx >= 0) & (idx < V)).squeeze(-1)
+    weight = inside.to(z.dtype) if mask is None else mask.to(z.dtype) * inside
+    used = weight != 0
+    logp = torch.log_softmax(z.masked_fill(~used.unsqueeze(-1), 0.0), dim=-1)
+    nll = -logp.gather(-1, idx.clamp(0, V - 1)).squeeze(-1)
+    ce = (torch.where(used, nll, torch.zeros_like(nll)) * weight).sum()
+    mx = z.max(dim=-1).values if z.numel() else z.new_zeros(z.shape[:-1])
+    l2 = 0.5 * L2WRAP_FACTOR * (mx * mx).sum()
+    if kd is None:
+        kd = distill_loss(logits, teacher_ids, teacher_logits, mask, temperature)
+    return (ce, weight.sum(), l2, torch.full((), float(mx.numel()), dtype=z.dtype, device=z.device)) + tuple(kd)
+
+
 def compute_age_mask(ages, cfg):
     """Soft age gate of the read relevance: ``sigmoid((age_ref - age) / (age_sigma + eps))``
     (src/rwkv7m/model/screening.py:378-380)."""

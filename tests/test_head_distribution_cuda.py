@@ -1,0 +1,282 @@
+"""Log-probabilities and distillation through the head against the same definitions in 64 bits.
+
+Tolerances count roundings.  A logit is a sum of C exact products of bf16 numbers in fp32, 16 of them and the accumulator in
+one step that may drop what lies 2^-23 below its largest term: at most 17 (C / 16 + 1) 2^-23 of sum |h w|.  A row's results
+add the roundings of its sum of exponentials (one tile of 256 columns adds 2 x 16 per chunk, then 8 chunks and the tiles).
+The gradient of the logits is rounded once to bf16 (2^-8 relative) before the two products, whose results are rounded once.
+"""
+
+import math
+
+import pytest
+import torch
+
+from rwkv7m_b200 import ops
+from rwkv7m_b200.ops import reference as R
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def _K():
+    from rwkv7m_b200.ops import cuda as K
+
+    return K
+
+
+@pytest.fixture(params=[0, 1], ids=["single", "pair"], autouse=True)
+def _pair_mode(request):
+    kk = _K()
+    old = kk.GEMM_PAIR
+    kk.set_gemm_pair(bool(request.param))
+    kk.gemm_error_reset(torch.zeros(1, device="cuda"))
+    yield
+    kk.set_gemm_pair(old)
+    assert kk.gemm_error_code(torch.zeros(1, device="cuda")) == 0
+
+
+def _operands(M, V, C, seed=0, w_dtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(M, C, generator=g).to(torch.bfloat16).cuda()
+    w = (torch.randn(V, C, generator=g) * (2.0 / math.sqrt(C))).to(torch.bfloat16).to(w_dtype).cuda()
+    ids = torch.randint(0, V, (M,), generator=g).cuda()
+    return h.requires_grad_(), w.requires_grad_(), ids
+
+
+def _double(*xs):
+    return [x.detach().double().requires_grad_() for x in xs]
+
+
+def _z_error(h, w):
+    C = h.shape[1]
+    return 17 * (C / 16 + 1) * 2 * U * float((h.detach().double().abs() @ w.detach().double().abs().T).max())
+
+
+def _row_tol(h, w, z, tau):
+    span = float((z.detach().amax(-1) - z.detach().amin(-1)).max()) / tau
+    return 2 * _z_error(h, w) / tau + (8 * span + 100 + 4 * math.log(z.shape[1])) * U
+
+
+def _check_grads(got, want, dz, row_tol, h, w):
+    """``dz``: the gradient of the logits in 64 bits, ``row_tol``: how far an exponent may be off."""
+    mag = dz.abs() + 1e-30
+    rel = 2.0 ** -8 + 2 * row_tol
+    # absolute part: q (A + B ln q) with a rounded sum of two terms of opposite sign is covered by their magnitudes
+    for g, wt, mass in ((got[0], want[0], mag @ w.detach().double().abs()),
+                        (got[1], want[1], mag.T @ h.detach().double().abs())):
+        if g is None:
+            continue
+        tol = rel * mass + (2.0 ** -8 if g.dtype == torch.bfloat16 else 4 * U) * wt.abs() + 1e-12
+        # accumulation of the products in fp32, as for the logits
+        tol = tol + 17 * (dz.shape[1] / 16 + 1) * 2 * U * mass
+        bad = (g.double() - wt).abs() > tol
+        assert not bad.any(), float(((g.double() - wt).abs() / tol).max())
+
+
+SHAPES = [(1, 1, 8), (1, 7, 16), (3, 256, 64), (5, 300, 64), (64, 1000, 512), (130, 1003, 136), (257, 513, 576), (300, 4099, 512),
+          (1000, 9001, 768), (2, 65536, 1024)]
+
+
+@pytest.mark.parametrize("M,V,C", SHAPES)
+@pytest.mark.parametrize("tau", [1.0, 2.3])
+def test_head_token_logprobs(M, V, C, tau):
+    h, w, ids = _operands(M, V, C, seed=M)
+    if M > 4:
+        ids[1], ids[3] = -1, V
+    g = torch.Generator().manual_seed(1)
+    up = [torch.randn(M, generator=g).cuda() for _ in range(2)]
+    lp, ent = ops.head_token_logprobs(h, w, ids, temperature=tau)
+    got = torch.autograd.grad((lp, ent), (h, w), up)
+    hd, wd = _double(h, w)
+    zd = hd @ wd.T
+    lp2, ent2, _, _ = R.token_logprobs(zd, ids, 0, tau)
+    tol = _row_tol(h, w, zd, tau)
+    assert (lp.double() - lp2).abs().max() <= tol
+    assert (ent.double() - ent2).abs().max() <= tol * 2 * (math.log(V) + 2)
+    loss = (lp2 * up[0].double()).sum() + (ent2 * up[1].double()).sum()
+    dz, = torch.autograd.grad(loss, zd, retain_graph=True)
+    want = torch.autograd.grad(loss, (hd, wd))
+    # terms of an element of dz may cancel: bound by their magnitudes
+    q = torch.softmax(zd.detach() / tau, -1)
+    mass = q * (up[0].abs()[:, None] + up[1].abs()[:, None] * (2 * math.log(V) + 2 - q.log())) / tau
+    mass.scatter_add_(1, ids.clamp(0, V - 1)[:, None], up[0].abs()[:, None].double() / tau)
+    _check_grads(got, want, torch.maximum(dz.abs(), mass * (2 * tol)), tol, h, w)
+    if M > 4:
+        assert lp[1] == 0 and lp[3] == 0
+
+
+def _teacher(M, V, K, seed, ids=None):
+    g = torch.Generator().manual_seed(seed)
+    t_ids = torch.randint(0, V, (M, K), generator=g).cuda()
+    t = (torch.randn(M, K, generator=g) * 3).cuda()
+    if M > 6:
+        t_ids[0] = -1                                # no teacher
+        t_ids[1, 0] = V + 5                          # absent alternative
+        t[2, K // 2:] = -math.inf
+        t_ids[3] = t_ids[3, 0]                       # one id in every place
+        t_ids[4, K - 1] = ids[4] if ids is not None else 0
+    return t_ids, t
+
+
+@pytest.mark.parametrize("M,V,C,K", [(1, 1, 8, 1), (2, 9, 16, 4), (8, 300, 64, 3), (130, 1003, 136, 33), (300, 4099, 512, 16),
+                                     (257, 513, 576, 256), (1000, 9001, 768, 128), (64, 65536, 512, 64)])
+@pytest.mark.parametrize("tau", [1.0, 2.0])
+def test_head_distill_loss(M, V, C, K, tau):
+    h, w, tgt = _operands(M, V, C, seed=K)
+    t_ids, t = _teacher(M, V, K, seed=M, ids=tgt)
+    g = torch.Generator().manual_seed(2)
+    mask = torch.rand(M, generator=g).cuda()
+    if M > 6:
+        mask[5] = 0.0
+        tgt[6] = -100
+    out = ops.head_distill_loss(h, w, tgt, mask, t_ids, t, temperature=tau)
+    coef = (0.6 / M, 1.0 / M, 0.4 / M)
+    got = torch.autograd.grad(out[0] * coef[0] + out[2] * coef[1] + out[4] * coef[2], (h, w))
+    hd, wd = _double(h, w)
+    zd = hd @ wd.T
+    ref = R.distill_components(zd, tgt, mask.double(), t_ids, t.double(), tau)
+    tol = _row_tol(h, w, zd, 1.0) + _row_tol(h, w, zd, tau)
+    t_span = float((t.nan_to_num(neginf=0.0).amax() - t.nan_to_num(neginf=0.0).amin())) / tau
+    kd_tol = tau * tau * (tol + (8 * t_span + 600) * U)
+    msum = float(mask.sum()) + 1
+    for i, bound in ((0, tol * msum), (1, 4 * U * msum), (2, 1e-4 * float(zd.max().abs()) * 2 * _z_error(h, w) * M + 1e-9), (3, 0.0),
+                     (4, kd_tol * msum), (5, 4 * U * msum)):
+        assert abs(float(out[i].detach()) - float(ref[i].detach())) <= bound + 4 * U * abs(float(ref[i].detach())), i
+    loss = ref[0] * coef[0] + ref[2] * coef[1] + ref[4] * coef[2]
+    dz, = torch.autograd.grad(loss, zd, retain_graph=True)
+    want = torch.autograd.grad(loss, (hd, wd))
+    m = mask.double()[:, None]
+    ids, p = R.teacher_distribution(t_ids, t.double(), V, tau)
+    mass = torch.softmax(zd.detach() / tau, -1) * (coef[2] * tau * m) + torch.softmax(zd.detach(), -1) * (coef[0] * m)
+    mass = mass.scatter_add(1, ids, p * coef[2] * tau * m).scatter_add(1, tgt.clamp(0, V - 1)[:, None], coef[0] * m)
+    _check_grads(got, want, torch.maximum(dz.abs(), mass * (2 * tol + (8 * t_span + 600) * U)), tol, h, w)
+
+
+def test_several_chunks_and_main_gradient(monkeypatch):
+    kk = _K()
+    h, w, ids = _operands(150, 1003, 256)
+    up = torch.ones(150, device="cuda") / 150
+
+    def grads(weight):
+        lp, ent = ops.head_token_logprobs(h, weight, ids)
+        return torch.autograd.grad((lp, ent), (h, weight), (up, up), allow_unused=True)
+
+    one = grads(w)
+    monkeypatch.setattr(kk, "HEAD_GRAD_ROWS", 64)
+    many = grads(w)
+    # the same roundings of dz; dW is added up in another order in fp32 and rounded once either way
+    assert torch.equal(one[0], many[0])
+    assert (one[1].double() - many[1].double()).abs().max() <= 2 * 2.0 ** -8 * float(one[1].abs().max())
+    w32 = w.detach().float().requires_grad_()
+    g32 = grads(w32)
+    assert g32[1].dtype == torch.float32
+    assert (g32[1].double() - one[1].double()).abs().max() <= 1.01 * 2.0 ** -8 * float(one[1].abs().max())
+    held = w.detach().float().requires_grad_()
+    held._main_grad = torch.full((1003, 256), 0.5, device="cuda")
+    got = grads(held)
+    assert got[1] is None
+    # fp32 sums of the same terms on top of 0.5: half a step of numbers near 0.5 per chunk
+    assert (held._main_grad - 0.5 - g32[1]).abs().max() <= 3 * 2.0 ** -24 + 4 * U * float(g32[1].abs().max())
+
+
+def test_frozen_sides():
+    h, w, ids = _operands(70, 500, 128)
+    both = torch.autograd.grad(ops.head_token_logprobs(h, w, ids)[0].sum(), (h, w))
+    only_h, = torch.autograd.grad(ops.head_token_logprobs(h, w.detach(), ids)[0].sum(), (h,))
+    only_w, = torch.autograd.grad(ops.head_token_logprobs(h.detach(), w, ids)[0].sum(), (w,))
+    assert torch.equal(both[0], only_h) and torch.equal(both[1], only_w)
+    with torch.no_grad():
+        assert not ops.head_token_logprobs(h, w, ids)[0].requires_grad
+
+
+def test_layouts_and_other_types():
+    h, w, ids = _operands(48, 300, 64)
+    want = ops.head_token_logprobs(h.detach(), w.detach(), ids)
+    wide = torch.zeros(48, 130, dtype=torch.bfloat16, device="cuda")
+    wide[:, 1:65] = h.detach()
+    views = [wide[:, 1:65], h.detach().view(6, 8, 64), h.detach().t().contiguous().t()]
+    for v in views:
+        lp, ent = ops.head_token_logprobs(v, w.detach(), ids.view(v.shape[:-1]))
+        assert lp.shape == v.shape[:-1]
+        assert torch.equal(lp.reshape(-1), want[0]) and torch.equal(ent.reshape(-1), want[1])
+    pad = torch.zeros(300, 72, dtype=torch.bfloat16, device="cuda")
+    pad[:, :64] = w.detach()
+    assert torch.equal(ops.head_token_logprobs(h.detach(), pad[:, :64], ids)[0], want[0])
+    # widths and types without a head kernel go through fp32 logits
+    for hh, ww in ((h.detach().float(), w.detach().float()), (h.detach()[:, :59], w.detach()[:, :59])):
+        lp, ent = ops.head_token_logprobs(hh, ww, ids)
+        ref = R.token_logprobs(hh.double() @ ww.double().T, ids)
+        # an fp32 product of at most 64 terms: 64 roundings of sum |h w|
+        tol = 2 * 64 * U * float((hh.double().abs() @ ww.double().abs().T).max()) + 500 * U
+        assert (lp - ref[0]).abs().max() <= tol and (ent - ref[1]).abs().max() <= 12 * tol
+    t_ids, t = _teacher(48, 300, 5, 1)
+    a = ops.head_distill_loss(h, w, ids, None, t_ids, t)
+    b = ops.head_distill_loss(h.detach().float(), w.detach().float(), ids, None, t_ids, t)
+    for x, y in zip(a, b):
+        assert abs(float(x.detach()) - float(y)) <= 48 * 2e-4
+    e = ops.head_distill_loss(h[:0], w, ids[:0], None, t_ids[:0], t[:0])
+    assert [float(x.detach()) for x in e] == [0.0] * 6
+    lp, ent = ops.head_token_logprobs(h[:0], w, ids[:0])
+    assert lp.shape == (0,) and ent.shape == (0,)
+
+
+def test_gradient_against_differences():
+    # hidden states on a grid of 1/8 and steps of 1/16 are exact in bf16
+    g = torch.Generator().manual_seed(9)
+    h = (torch.randint(-8, 9, (6, 64), generator=g) / 8).bfloat16().cuda()
+    w = (torch.randn(90, 64, generator=g) * 0.2).bfloat16().cuda()
+    d = torch.randint(-1, 2, (6, 64), generator=g).bfloat16().cuda()
+    ids = torch.randint(0, 90, (6,), generator=g).cuda()
+    t_ids, t = _teacher(6, 90, 4, 3)
+
+    def f(x):
+        lp, ent = ops.head_token_logprobs(x, w, ids)
+        out = ops.head_distill_loss(x, w, ids, None, t_ids, t, temperature=2.0)
+        return lp.sum() + 0.3 * ent.sum() + out[0] + 0.5 * out[4] + out[2]
+
+    leaf = h.clone().requires_grad_()
+    grad, = torch.autograd.grad(f(leaf), leaf)
+    s = 1 / 16
+    diff = (float(f(h + s * d)) - float(f(h - s * d))) / (2 * s)
+    want = float((grad.double() * d.double()).sum())
+    # along d a logit moves by |w d| <= 0.2 * 64^0.5 * 3 = 4.8 a unit, 0.3 a step: the third-order term is at most
+    # 6 rows * 4 terms * 4.8^3 / 6 * s^2 = 1.7; the gradient's own rounding is 2^-8 of its mass
+    assert abs(diff - want) <= 1.7 + 2.0 ** -6 * float((grad.double().abs() * d.double().abs()).sum())
+
+
+def test_captured_together_and_replayed():
+    h, w, ids = _operands(40, 3000, 256)
+    t_ids, t = _teacher(40, 3000, 9, 2)
+    mask = torch.ones(40, device="cuda")
+
+    def step():
+        lp, ent = ops.head_token_logprobs(h, w, ids)
+        out = ops.head_distill_loss(h, w, ids, mask, t_ids, t, temperature=2.0)
+        grads = torch.autograd.grad(lp.sum() + ent.sum() + out[0] + out[4] + out[2], (h, w))
+        return [lp.detach(), out[4].detach(), *grads]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    with torch.no_grad():
+        h.mul_(-0.5)
+        mask[3] = 0.0
+    graph.replay()
+    for a, b in zip(held, step()):
+        assert torch.equal(a, b)
+
+
+def test_refusals_on_a_gpu():
+    h, w, ids = _operands(4, 32, 16)
+    with pytest.raises(TypeError):
+        ops.head_token_logprobs(h.half(), w, ids)
+    with pytest.raises(TypeError):
+        ops.head_token_logprobs(h, w.half(), ids)
+    with pytest.raises(ValueError):
+        ops.head_token_logprobs(h, w.cpu(), ids)

@@ -147,3 +147,61 @@ def test_refusals():
     for kind, call in bad:
         with pytest.raises(kind):
             call()
+
+
+def test_head_operators_are_the_logit_operators_behind_a_product():
+    z, ids, t_ids, t, mask = _case()
+    g = torch.Generator().manual_seed(3)
+    h = torch.randn(5, 6, generator=g, dtype=torch.float64, requires_grad=True)
+    w = torch.randn(11, 6, generator=g, dtype=torch.float64, requires_grad=True)
+    ids = ids.clone()
+    ids[2] = -1
+    lp, ent = ops.head_token_logprobs(h, w, ids, temperature=1.3)
+    ref = ops.token_logprobs(h @ w.T, ids, temperature=1.3)
+    assert torch.allclose(lp, ref.logprob) and torch.allclose(ent, ref.entropy)
+    out = ops.head_distill_loss(h, w, ids, mask, t_ids, t, temperature=1.3)
+    z = h @ w.T
+    kd = ops.distill_loss(z, t_ids, t, mask, temperature=1.3)
+    logp = torch.log_softmax(z, -1)
+    weight = mask * (ids >= 0)
+    assert torch.allclose(out[0], -(logp[torch.arange(5), ids.clamp(min=0)] * weight).sum())
+    assert torch.allclose(out[1], weight.sum())
+    assert torch.allclose(out[2], 0.5e-4 * z.max(-1).values.square().sum()) and float(out[3]) == 5.0
+    assert torch.allclose(out[4], kd[0]) and torch.allclose(out[5], mask.sum())
+    assert torch.autograd.gradcheck(lambda a, b: ops.head_token_logprobs(a, b, ids), (h, w))
+    assert torch.autograd.gradcheck(lambda a, b: ops.head_distill_loss(a, b, ids, mask, t_ids, t, temperature=2.0)[::2], (h, w))
+
+
+def test_head_distill_agrees_with_the_head_loss():
+    g = torch.Generator().manual_seed(5)
+    h, w = torch.randn(2, 6, 8, generator=g), torch.randn(30, 8, generator=g)
+    tgt = torch.randint(0, 30, (2, 6), generator=g)
+    mask = (torch.rand(2, 6, generator=g) > 0.4).float()
+    t_ids, t = torch.randint(0, 30, (2, 6, 4), generator=g), torch.randn(2, 6, 4, generator=g)
+    ln_w, ln_b = torch.ones(8), torch.zeros(8)
+    want = ops.head_loss(h, ln_w, ln_b, w, tgt, mask)
+    got = ops.head_distill_loss(ops.layer_norm(h, ln_w, ln_b), w, tgt, mask, t_ids, t)
+    for a, b in zip(got[:4], want):
+        assert torch.allclose(a, b, rtol=1e-5)
+
+
+def test_head_refusals():
+    z, ids, t_ids, t, mask = _case()
+    h, w = torch.randn(5, 6), torch.randn(11, 6)
+    bad = [
+        (TypeError, lambda: ops.head_token_logprobs(h.long(), w, ids)),
+        (TypeError, lambda: ops.head_token_logprobs(h, w.long(), ids)),
+        (ValueError, lambda: ops.head_token_logprobs(h, w[:, :5], ids)),
+        (ValueError, lambda: ops.head_token_logprobs(h, w[0], ids)),
+        (ValueError, lambda: ops.head_token_logprobs(h, w[:0], ids)),
+        (ValueError, lambda: ops.head_token_logprobs(h, w, ids[:2])),
+        (ValueError, lambda: ops.head_token_logprobs(h, w, ids, temperature=0)),
+        (ValueError, lambda: ops.head_token_logprobs(h, w.to("meta"), ids)),
+        (ValueError, lambda: ops.head_distill_loss(h, w, ids[:2], mask, t_ids, t)),
+        (ValueError, lambda: ops.head_distill_loss(h, w, ids, mask[:1], t_ids, t)),
+        (ValueError, lambda: ops.head_distill_loss(h, w, ids, mask, t_ids[:, :0], t[:, :0])),
+        (TypeError, lambda: ops.head_distill_loss(h, w, ids.float(), mask, t_ids, t)),
+    ]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
