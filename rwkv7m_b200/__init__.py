@@ -2,6 +2,7 @@
 trained and served with hand-written sm_100a kernels."""
 
 from .api import (
+    DistillConfig,
     RWKV7MRuntime,
     create_runtime,
     create_train_runtime,
@@ -11,6 +12,9 @@ from .api import (
     infer_prefill,
     load_runtime_params,
     reset_runtime_state,
+    score_ids,
+    set_distillation,
+    teacher_targets,
     train_batch,
     train_binidx,
 )
@@ -49,7 +53,15 @@ from .models import (
 )
 from .config import RWKV7Config
 from .models.model import create_model_variables
-from .ops import wkv7, wkv7_sharded
+from .ops import (
+    TokenLogprobs,
+    distill_loss,
+    head_distill_loss,
+    head_token_logprobs,
+    token_logprobs,
+    wkv7,
+    wkv7_sharded,
+)
 from .ops.backends import (
     WKVBackend,
     WKVFFIBackend,

@@ -14,13 +14,13 @@ import torch
 
 from .config import ModelConfig, load_model_config, tiny_config
 from .data import BinIdxBatchDataset, create_binidx_dataset
-from .infer.generate import decode_one, generate, prefill
+from .infer.generate import decode_one, generate, prefill, score
 from .io.names import PortableParams
 from .io.safetensors_io import load_params_into_model
 from .models.model import ScreenedRWKVModel, initialize_model
 from .state import init_rwkv_state, init_screen_state
 from .tokenizer import RWKVTokenizer
-from .train.train_step import initialize_train_state, train_step
+from .train.train_step import DistillConfig, initialize_train_state, set_distillation, train_step
 
 
 @dataclass
@@ -197,14 +197,50 @@ def infer_next(runtime: RWKV7MRuntime, token_ids, *, phase="read_screening_only"
 
 
 def generate_ids(runtime: RWKV7MRuntime, prompt_ids, *, max_new_tokens=50, temperature=1.0, top_p=0.9,
-                 rng_key=None, phase="read_screening_only"):
+                 rng_key=None, phase="read_screening_only", top_logprobs: int | None = None):
+    """New ids [B, max_new_tokens]; with ``top_logprobs`` (a number of alternatives, 0 for none) a pair of those and their
+    scores under the model's own distribution (``ops.TokenLogprobs``)."""
     _match_state_batch(runtime, _ids(runtime, prompt_ids))
-    ids, runtime.rwkv_state, runtime.screen_state = generate(
+    ids, runtime.rwkv_state, runtime.screen_state, *scores = generate(
         runtime.model, _ids(runtime, prompt_ids), runtime.rwkv_state, runtime.screen_state,
         max_new_tokens=max_new_tokens, temperature=temperature, top_p=top_p, rng_key=rng_key, phase=phase,
-        context_parallel=runtime.context_parallel,
+        context_parallel=runtime.context_parallel, top_logprobs=top_logprobs,
     )
-    return ids
+    return (ids, scores[0]) if scores else ids
+
+
+def _fresh_state(runtime, batch_size):
+    if batch_size == runtime.batch_size:
+        return runtime.initial_rwkv_state, runtime.initial_screen_state
+    tp = getattr(runtime.model, "tp", None)
+    cfg = runtime.config
+    rwkv = (tp.init_rwkv_state(batch_size, cfg, device=runtime.device) if tp is not None
+            else init_rwkv_state(batch_size, cfg, device=runtime.device))
+    return rwkv, init_screen_state(batch_size, cfg.screening if cfg.use_screening else _no_screen(cfg), device=runtime.device)
+
+
+def score_ids(runtime: RWKV7MRuntime, ids, *, top_k: int = 0, temperature: float = 1.0, phase="read_screening_only"):
+    """Scores of a text of T >= 2 tokens ([T] or [B, T]) from the zero state: ``ops.TokenLogprobs`` with [B, T - 1] entries,
+    the log-probability of each token but the first, the entropy of its prediction and ``top_k`` alternatives.  The
+    runtime's held state is neither read nor changed."""
+    ids = _ids(runtime, ids)
+    rwkv_state, screen_state = _fresh_state(runtime, int(ids.shape[0]))
+    return score(runtime.model, ids, rwkv_state, screen_state, top_k=top_k, temperature=temperature, phase=phase)
+
+
+@torch.no_grad()
+def teacher_targets(runtime: RWKV7MRuntime, input_ids, *, top_k: int, phase="read_screening_only"):
+    """What a student needs from this model as its teacher: ``{"teacher_ids", "teacher_logits"}``, [B, T, top_k] each, the
+    most likely next tokens at every position of ``input_ids`` with their log-probabilities.  Add them to a training batch
+    (see :func:`set_distillation`)."""
+    if top_k < 1:
+        raise ValueError("a teacher gives at least one alternative")
+    ids = _ids(runtime, input_ids)
+    rwkv_state, screen_state = _fresh_state(runtime, int(ids.shape[0]))
+    runtime.model.eval()
+    hidden, _, _, _ = runtime.model.compute_recurrent_hidden(ids, rwkv_state, screen_state, phase=phase)
+    out = runtime.model.compute_token_logprobs(hidden, ids, top_k=top_k)
+    return {"teacher_ids": out.top_ids, "teacher_logits": out.top_logprobs}
 
 
 def generate_text(runtime: RWKV7MRuntime, prompt: str, *, tokenizer: RWKVTokenizer | None = None,
@@ -237,6 +273,7 @@ def train_batch(train_state, batch, runtime: RWKV7MRuntime, *, phase="read_scree
     ``carry_state=False`` starts from the zero state (the runtime's reusable
     initial state when the batch size matches); ``carry_state=True`` starts
     from and writes back ``runtime.rwkv_state`` / ``runtime.screen_state``.
+    A batch with ``teacher_ids`` / ``teacher_logits`` [B, T, K] trains on the teacher as :func:`set_distillation` says.
     """
     device = runtime.device
     batch = _batch_to_device(batch, device)
@@ -315,6 +352,7 @@ def reset_runtime_state(runtime: RWKV7MRuntime, config: ModelConfig | None = Non
 
 __all__ = [
     "RWKV7MRuntime", "create_runtime", "create_train_runtime", "load_runtime_params", "infer_prefill",
-    "infer_next", "generate_ids", "generate_text", "train_batch", "train_binidx", "reset_runtime_state",
+    "infer_next", "generate_ids", "generate_text", "score_ids", "teacher_targets", "DistillConfig", "set_distillation",
+    "train_batch", "train_binidx", "reset_runtime_state",
     "tiny_config", "BinIdxBatchDataset", "create_binidx_dataset",
 ]

@@ -31,12 +31,16 @@ def parse_args(argv=None):
     p.add_argument("--context-parallel-size", type=int, default=1,
                    help="split the prefill of the prompt along time over this many processes (under torch.distributed.run); "
                         "all of them then decode the same continuation and the first one prints it")
+    p.add_argument("--top-logprobs", type=int, default=None, metavar="K",
+                   help="record every new token's log-probability, the entropy of its prediction and K alternatives in --json-out")
     p.add_argument("--json-out", default=None)
     args = parse_args_with_config(p, argv)
     if not args.prompt and not args.prompt_file:
         p.error("give at least one --prompt or a --prompt-file")
     if args.num_samples < 1:
         p.error("--num-samples must be positive")
+    if args.top_logprobs is not None and not (args.json_out and 0 <= args.top_logprobs <= 64):
+        p.error("--top-logprobs takes 0 to 64 alternatives and needs --json-out")
     return args
 
 
@@ -80,6 +84,34 @@ def build_runtime(args):
     return load_runtime_params(runtime, params)      # a tensor-parallel runtime keeps this rank's slices of the full tensors
 
 
+def _token_records(tokenizer, ids, scores):
+    """One entry per new token: id, text, log-probability, entropy, and the alternatives with their log-probabilities."""
+    def text(i):
+        return tokenizer.decode([i]) if i >= 0 else ""
+
+    out = []
+    for t, i in enumerate(ids):
+        rec = {"id": i, "text": text(i), "logprob": float(scores.logprob[0, t]), "entropy": float(scores.entropy[0, t])}
+        if scores.top_ids is not None:
+            rec["top"] = [{"id": int(a), "text": text(int(a)), "logprob": float(b)}
+                          for a, b in zip(scores.top_ids[0, t].tolist(), scores.top_logprobs[0, t].tolist())]
+        out.append(rec)
+    return out
+
+
+def _generate_scored(runtime, prompt, tokenizer, args, seed):
+    from ..api import generate_ids
+
+    prompt_ids = tokenizer.encode(prompt)
+    if not prompt_ids:
+        raise ValueError("prompt must encode to at least one token")
+    new, scores = generate_ids(runtime, [prompt_ids], max_new_tokens=args.max_new_tokens, temperature=args.temperature,
+                               top_p=args.top_p, rng_key=seed, phase=args.phase, top_logprobs=args.top_logprobs)
+    ids = [int(x) for x in new[0].tolist()]
+    text = tokenizer.decode(ids if args.continuation_only else prompt_ids + ids)
+    return text, _token_records(tokenizer, ids, scores)
+
+
 def main(argv=None):
     from ..api import generate_text
     from ..parallel.mesh import process_info
@@ -92,10 +124,14 @@ def main(argv=None):
     for prompt in collect_prompts(args):
         for sample in range(args.num_samples):
             seed = args.seed + sample
-            text = generate_text(runtime, prompt, tokenizer=tokenizer, max_new_tokens=args.max_new_tokens,
-                                 temperature=args.temperature, top_p=args.top_p, rng_key=seed, phase=args.phase,
-                                 include_prompt=not args.continuation_only)
-            records.append({"prompt": prompt, "sample": sample, "seed": seed, "text": text})
+            record = {"prompt": prompt, "sample": sample, "seed": seed}
+            if args.top_logprobs is not None:
+                record["text"], record["tokens"] = _generate_scored(runtime, prompt, tokenizer, args, seed)
+            else:
+                record["text"] = generate_text(runtime, prompt, tokenizer=tokenizer, max_new_tokens=args.max_new_tokens,
+                                               temperature=args.temperature, top_p=args.top_p, rng_key=seed, phase=args.phase,
+                                               include_prompt=not args.continuation_only)
+            records.append(record)
     first = process_info()["process_index"] == 0
     if first:
         for r in records:

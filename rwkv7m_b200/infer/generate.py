@@ -47,6 +47,17 @@ def sample_next(last_logits, temperature, top_p, generator=None):
 
 
 @torch.no_grad()
+def score(model, ids, rwkv_state, screen_state, *, top_k=0, temperature=1.0, phase="read_screening_only"):
+    """Scores of a text [B, T] (T >= 2) under the model: the log-probability of every token but the first given those before
+    it, the entropy of each of those predictions and their ``top_k`` alternatives, [B, T - 1] each."""
+    if ids.shape[1] < 2:
+        raise ValueError("scoring needs at least two tokens: the first one is only read")
+    model.eval()
+    hidden, _, _, _ = model.compute_recurrent_hidden(ids[:, :-1], rwkv_state, screen_state, phase=phase)
+    return model.compute_token_logprobs(hidden, ids[:, 1:].contiguous(), top_k=top_k, temperature=temperature)
+
+
+@torch.no_grad()
 def prefill_last(model, prompt_ids, rwkv_state, screen_state, *, phase="read_screening_only", context_parallel=None):
     """Prefill that projects only the last position onto the vocabulary (the [B, T, V] logits of a long
     prompt are never materialised).  Returns (last logits [B, V], rwkv_state, screen_state).
@@ -152,9 +163,28 @@ def _graph_ok(model, prompt_ids):
 
 @torch.no_grad()
 def generate(model, prompt_ids, rwkv_state, screen_state, *, max_new_tokens=50, temperature=1.0,
-             top_p=0.9, rng_key=None, phase="read_screening_only", use_cuda_graph=None, context_parallel=None):
+             top_p=0.9, rng_key=None, phase="read_screening_only", use_cuda_graph=None, context_parallel=None,
+             top_logprobs=None):
     """Returns (new ids [B, max_new_tokens], rwkv_state, screen_state).  ``context_parallel``: split the prefill of a long
-    prompt over the processes of that group (see ``prefill_last``); they all decode the same continuation."""
+    prompt over the processes of that group (see ``prefill_last``); they all decode the same continuation.
+
+    ``top_logprobs`` (a number of alternatives, 0 for none): a fourth result with the scores of every new token under the
+    model's own distribution (temperature 1, before nucleus filtering), a ``TokenLogprobs`` of [B, max_new_tokens] entries."""
+    from .. import ops
+
+    scores = []
+
+    def pick(last):
+        nxt = sample_next(last, temperature, top_p, generator)
+        if top_logprobs is not None:
+            scores.append(ops.token_logprobs(last.unsqueeze(1), nxt, top_k=top_logprobs))
+        return nxt
+
+    def result(ids, rwkv_state, screen_state):
+        if top_logprobs is None:
+            return ids, rwkv_state, screen_state
+        return ids, rwkv_state, screen_state, ops.TokenLogprobs.join(scores)
+
     if rng_key is None:
         rng_key = 0
     if isinstance(rng_key, torch.Generator):
@@ -169,13 +199,13 @@ def generate(model, prompt_ids, rwkv_state, screen_state, *, max_new_tokens=50, 
     if use_cuda_graph:
         dec = GraphDecoder(model, rwkv_state, phase=phase)
         for _ in range(max_new_tokens):
-            nxt = sample_next(last, temperature, top_p, generator)
+            nxt = pick(last)
             out.append(nxt)
             last = dec.step(nxt)
         rwkv_state = tuple(s.detach() for s in dec.state)
-        return torch.cat(out, dim=1).to(torch.int32), rwkv_state, screen_state
+        return result(torch.cat(out, dim=1).to(torch.int32), rwkv_state, screen_state)
     for _ in range(max_new_tokens):
-        nxt = sample_next(last, temperature, top_p, generator)
+        nxt = pick(last)
         out.append(nxt)
         last, rwkv_state, screen_state, _ = decode_one(model, nxt, rwkv_state, screen_state, phase=phase)
-    return torch.cat(out, dim=1).to(torch.int32), rwkv_state, screen_state
+    return result(torch.cat(out, dim=1).to(torch.int32), rwkv_state, screen_state)

@@ -181,6 +181,48 @@ class ScreenedRWKVModel(nn.Module):
             ce_total = hook.mark_leave(ce_total, hook.unit_of("head"))
         return {"ce_total": ce_total, "ce_count": ce_count, "l2_total": l2_total, "l2_count": l2_count}
 
+    def compute_distill_loss(self, hidden, targets, mask, teacher_ids, teacher_logits, *, temperature=1.0):
+        """The pieces of :meth:`compute_training_loss` plus ``kd_total`` / ``kd_count`` of a distillation from a teacher's top
+        logits [B, T, K], in one pass over the head."""
+        tp = getattr(self, "tp", None)
+        if tp is not None and tp.vocab_parallel:
+            raise ValueError("distillation needs the whole head on every rank (vocab_parallel=False)")
+        hook = getattr(self, "unit_hook", None)
+        if hook is not None:
+            hook.pre_forward(hook.unit_of("head"))
+            hidden = hook.mark_enter(hidden, hook.unit_of("head"))
+        if tp is not None:
+            targets, teacher_ids, teacher_logits = (tp.local_time_slice(t) for t in (targets, teacher_ids, teacher_logits))
+            mask = None if mask is None else tp.local_time_slice(mask)
+        with nvtx_range("head_distill_loss"):
+            parts = ops.head_distill_loss(self.ln_out(hidden), self.head.weight, targets, mask, teacher_ids, teacher_logits,
+                                          temperature=temperature)
+        if tp is not None:
+            parts = tuple(tp.sum_scalar(p.float().reshape(())) for p in parts)
+        ce_total, ce_count, l2_total, l2_count, kd_total, kd_count = parts
+        check_finite("head_distill_loss", ce_total, l2_total, kd_total)
+        if hook is not None:
+            ce_total = hook.mark_leave(ce_total, hook.unit_of("head"))
+        return {"ce_total": ce_total, "ce_count": ce_count, "l2_total": l2_total, "l2_count": l2_count,
+                "kd_total": kd_total, "kd_count": kd_count}
+
+    def compute_token_logprobs(self, hidden, ids, *, top_k=0, temperature=1.0):
+        """Log-probability of ``ids`` [B, T], entropy and ``top_k`` alternatives at every position of ``hidden`` [B, T, C]
+        (:class:`rwkv7m_b200.ops.TokenLogprobs`).  Without alternatives no logits are kept; with them the positions go
+        through :meth:`compute_logits` a slice of time at a time."""
+        tp = getattr(self, "tp", None)
+        if top_k == 0 and tp is None and getattr(self, "unit_hook", None) is None:
+            return ops.TokenLogprobs(*ops.head_token_logprobs(self.ln_out(hidden), self.head.weight, ids, temperature=temperature))
+        T = hidden.shape[1]
+        # under tensor parallelism the hidden states are a time slice that the head gathers, so they stay in one piece
+        step = T if tp is not None else max(1, min(T, 4096 // max(1, hidden.shape[0])))
+        parts = []
+        for s in range(0, T, step):
+            logits = self.compute_logits(hidden[:, s : s + step])
+            parts.append(ops.token_logprobs(logits, ids if tp is not None else ids[:, s : s + step], top_k=top_k,
+                                            temperature=temperature))
+        return ops.TokenLogprobs.join(parts)
+
     def _tp_training_loss(self, hidden, targets, mask, chunk, tp):
         """Loss pieces under tensor parallelism; ``hidden`` is this rank's time slice."""
         if tp.vocab_parallel:

@@ -260,6 +260,13 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor | None = None
     top_logprobs: torch.Tensor | None = None
 
+    @classmethod
+    def join(cls, parts, dim=1):
+        """The scores of consecutive slices (of time, by default) as one."""
+        if len(parts) == 1:
+            return parts[0]
+        return cls(*(None if field[0] is None else torch.cat(field, dim=dim) for field in zip(*parts)))
+
 
 TOP_K_MAX = 64            # alternatives of token_logprobs
 TEACHER_K_MAX = 256       # alternatives a teacher may give per position

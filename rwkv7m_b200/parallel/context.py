@@ -118,9 +118,10 @@ class ContextParallel:
         return tensor.narrow(dim, a, b - a)
 
     def slice_batch(self, batch: dict) -> dict:
-        """This rank's tokens of a ``[B, T]`` batch (inputs, targets and mask; other entries pass through)."""
+        """This rank's tokens of a ``[B, T]`` batch (inputs, targets, mask and a teacher's top logits; other
+        entries pass through)."""
         out = dict(batch)
-        for key in ("input_ids", "target_ids", "mask"):
+        for key in ("input_ids", "target_ids", "mask", "teacher_ids", "teacher_logits"):
             if out.get(key) is not None:
                 out[key] = self.local_time_slice(out[key]).contiguous()
         return out

@@ -43,14 +43,17 @@ def global_loss_scales(batch, world: int, group=None):
 
 
 def reduce_loss_metrics(metrics, scales, group=None):
-    """Turn the per-rank ``loss`` / ``total_loss`` into their global-batch values with one 2-element all-reduce."""
+    """Turn the per-rank ``loss`` / ``total_loss`` into their global-batch values with one all-reduce of those
+    two numbers (three with a distillation term)."""
     ce_s, _ = scales
     scaled_total = metrics.pop("scaled_total_loss", None)
     if scaled_total is None:
         scaled_total = metrics["total_loss"] * ce_s
-    pair = torch.stack([(metrics["loss"].detach() * ce_s).reshape(()).float(), scaled_total.detach().reshape(()).float()])
-    dist.all_reduce(pair, group=group)
-    metrics["loss"], metrics["total_loss"] = pair[0], pair[1]
+    names = ["loss"] + (["distill_loss"] if "distill_loss" in metrics else [])
+    sums = torch.stack([(metrics[n].detach() * ce_s).reshape(()).float() for n in names] + [scaled_total.detach().reshape(()).float()])
+    dist.all_reduce(sums, group=group)
+    for i, name in enumerate(names + ["total_loss"]):
+        metrics[name] = sums[i]
     return metrics
 
 

@@ -9,11 +9,13 @@ from .optimizer import (
     warmup_cosine_decay_schedule,
 )
 from .train_step import (
+    DistillConfig,
     TrainState,
     accumulate_gradients,
     generate_toy_batch,
     initialize_train_state,
     model_loss,
+    set_distillation,
     train_step,
 )
 
@@ -65,5 +67,5 @@ __all__ = [
     "initialize_nnx_train_state", "nnx_train_step",
     "AdamWChain", "FlatParams", "create_optimizer", "decay_mask", "is_w0", "make_schedule",
     "rwkv_warmup_cosine_schedule", "warmup_cosine_decay_schedule", "TrainState", "accumulate_gradients",
-    "generate_toy_batch", "initialize_train_state", "model_loss", "train_step",
+    "generate_toy_batch", "initialize_train_state", "model_loss", "train_step", "DistillConfig", "set_distillation",
 ]

@@ -77,10 +77,50 @@ class TrainMetrics:
         return cls(**{f: torch.as_tensor(metrics.get(f, zero)) for f in cls.__dataclass_fields__})
 
 
+@dataclass(frozen=True)
+class DistillConfig:
+    """How a student trains on a teacher: ``weight`` of the distillation term (the cross-entropy keeps ``1 - weight``) and the
+    ``temperature`` of both distributions in it."""
+
+    weight: float = 0.5
+    temperature: float = 1.0
+
+    def __post_init__(self):
+        if not 0.0 <= self.weight <= 1.0:
+            raise ValueError("the distillation weight must lie between 0 and 1")
+        if not 0.0 < self.temperature < float("inf"):
+            raise ValueError("the distillation temperature must be positive and finite")
+
+
+def set_distillation(model, config: DistillConfig | None):
+    """Train ``model`` on batches that carry a teacher's top logits (``teacher_ids`` and ``teacher_logits``, [B, T, K]) with
+    these settings; None turns it off."""
+    model.distill = config
+
+
+def _head_loss_parts(model, hidden, batch, hchunk):
+    """(loss pieces, main term of the loss, metrics): the cross-entropy alone, or its mixture with the distillation term
+    when the batch carries a teacher."""
+    mask = batch.get("mask")
+    if batch.get("teacher_ids") is None:
+        parts = model.compute_training_loss(hidden, batch["target_ids"], mask, chunk=hchunk)
+        ce = parts["ce_total"] / torch.clamp(parts["ce_count"], min=1.0)
+        return parts, ce, {"loss": ce.detach()}
+    cfg = getattr(model, "distill", None)
+    if cfg is None:
+        raise ValueError("the batch carries a teacher's logits: choose the settings with set_distillation(model, DistillConfig(...))")
+    parts = model.compute_distill_loss(hidden, batch["target_ids"], mask, batch["teacher_ids"], batch["teacher_logits"],
+                                       temperature=cfg.temperature)
+    ce = parts["ce_total"] / torch.clamp(parts["ce_count"], min=1.0)
+    kd = parts["kd_total"] / torch.clamp(parts["kd_count"], min=1.0)
+    return parts, (1.0 - cfg.weight) * ce + cfg.weight * kd, {"loss": ce.detach(), "distill_loss": kd.detach()}
+
+
 def model_loss(model, batch, rwkv_state, screen_state, *, phase, include_l2wrap=True,
                ce_loss_scale=1.0, l2_loss_scale=1.0, loss_parts=None):
     """Returns (total_loss, (metrics, new_rwkv_state, new_screen_state)).  A dict passed as ``loss_parts`` receives
-    the unscaled cross-entropy and L2Wrap terms under ``"ce"`` and ``"l2"``."""
+    the unscaled main term (the cross-entropy, or its mixture with the distillation term when the batch carries a teacher) and
+    the L2Wrap term under ``"ce"`` and ``"l2"``."""
     cfg = model.config
     input_ids = batch["input_ids"]
     T = int(input_ids.shape[1])
@@ -105,13 +145,11 @@ def model_loss(model, batch, rwkv_state, screen_state, *, phase, include_l2wrap=
         else:
             stats_total = {k: stats_total[k] + v * weight for k, v in stats.items()}
     hidden = hidden_chunks[0] if len(hidden_chunks) == 1 else torch.cat(hidden_chunks, dim=1)
-    parts = model.compute_training_loss(hidden, batch["target_ids"], batch.get("mask"), chunk=hchunk)
-    ce_loss = parts["ce_total"] / torch.clamp(parts["ce_count"], min=1.0)
+    parts, ce_loss, metrics = _head_loss_parts(model, hidden, batch, hchunk)
     l2_loss = parts["l2_total"] / torch.clamp(parts["l2_count"], min=1.0)
     total = ce_loss * ce_loss_scale
     if include_l2wrap:
         total = total + l2_loss * l2_loss_scale
-    metrics = {"loss": ce_loss.detach()}
     if loss_parts is not None:
         loss_parts["ce"], loss_parts["l2"] = ce_loss.detach(), l2_loss.detach()
     for k, v in (stats_total or {}).items():
@@ -200,7 +238,7 @@ def accumulate_gradients(model, batch, rwkv_state, screen_state, *, phase, gradi
             ops.flush_deferred()
         check_finite("loss", loss)
         local = parts["ce"] * ce_w + parts["l2"] * pos_w
-        weighted = {k: v * (ce_w if k == "loss" else pos_w) for k, v in metrics.items()}
+        weighted = {k: v * (ce_w if k in ("loss", "distill_loss") else pos_w) for k, v in metrics.items()}
         acc_metrics = weighted if acc_metrics is None else {k: acc_metrics[k] + weighted[k] for k in weighted}
         acc_loss = local if acc_loss is None else acc_loss + local
         acc_scaled = loss.detach() if acc_scaled is None else acc_scaled + loss.detach()
