@@ -10,7 +10,9 @@
 // Log-probabilities (w = their upstream gradients) and distillation (w_j = -g mask tau^2 p_j, g_H = 0) share both
 // kernels.  A row is kept as the pair (m, log2 S) and not as one log-sum-exp: with logits around 1000 the sum m + ln S
 // would round off 3e-5 of every log-probability.
+#include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -32,8 +34,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Once per row, so in 64 bits: the build's fast-math logarithm loses half the digits close to 1.
-__device__ __forceinline__ float log2_row(float s) { return (float)log2((double)s); }
+// log2 of a row's sum.  The build's fast-math logarithm has an absolute error, which is everything when the sum is close to
+// 1 (a confident prediction); this is s = 2^e f with f in [0.71, 1.42) and log f = 2 atanh u, u = (f - 1) / (f + 1), by
+// atanh's power series: |u| < 0.172, the first term left out is below 2^-31 of the sum.
+__device__ __forceinline__ float log2_row(float s) {
+  if (!(s > 0.f && s < INFINITY)) return s == 0.f ? -INFINITY : s;
+  const int e = (__float_as_int(s) - 0x3f3504f3) >> 23;
+  const float f = __int_as_float(__float_as_int(s) - (e << 23));
+  const float u = __fdiv_rn(f - 1.f, f + 1.f), v = u * u;
+  float p = fmaf(v, 1.f / 11.f, 1.f / 9.f);
+  p = fmaf(v, p, 1.f / 7.f);
+  p = fmaf(v, p, 1.f / 5.f);
+  p = fmaf(v, p, 1.f / 3.f);
+  return fmaf(2.f * kLog2e * u, fmaf(v, p, 1.f), (float)e);
+}
 
 // A row seen as 16-byte units of the aligned addresses that hold it; the first and the last unit may be partly outside.
 template <typename T>
@@ -97,17 +111,258 @@ __device__ __forceinline__ Stat shfl_xor(const Stat& a, int o) {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
-constexpr int kCandidates = 1024;
+constexpr int kFewRowsThreads = 512;
+constexpr int kCandidates = 512;
+constexpr int kMaxTop = 64;
+// The fast pass lifts columns below this to it (probability zero either way), so that 0 * t stays finite without a test of
+// every exponent; a row whose maximum is that low itself is done again by the exact pass.
+constexpr float kFloor = -1e30f;
+// The fast pass keeps its reference until a logit exceeds it by this exponent (a thread then rescales once or twice a row):
+// with the maximum itself as reference some lane of a warp would rescale in two of three units.
+constexpr float kSlack = 8.f;
 
-// Forward: one CTA per row.  Every thread keeps the statistics of its units and, for the alternatives, its largest logit
-// and the first unit that holds it.  The k-th largest of the 256 thread maxima bounds the k-th largest column from
-// below, so only the k threads above the bound are looked at again (k 256-element groups of a 65536-wide row, from L2).
+using f2 = unsigned long long;     // two fp32 numbers: the packed instructions of sm_100 halve the arithmetic of the pass
+__device__ __forceinline__ f2 pack2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ void unpack2(f2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint32_t max_bf2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+// One thread's statistics in the fast pass: t = z c - ref (one rounding, whatever the size of the logits), the sums in two
+// halves, the largest logit and the first unit that holds it.
+struct Running {
+  float ref, limit, m;
+  f2 s1, s2;
+  int bu;
+};
+
+// A whole unit into the running statistics.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) row_stats_kernel(RowStatsArgs a) {
+__device__ __forceinline__ void take_fast(Running& st, uint4 raw, int u, float c, float slack) {
+  f2 z[Row<T>::E / 2];
+  float cm;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t low = 0xf149f149u;            // bf16 pair of about -1e30
+    const uint32_t w[4] = {max_bf2(raw.x, low), max_bf2(raw.y, low), max_bf2(raw.z, low), max_bf2(raw.w, low)};
+    const uint32_t mx = max_bf2(max_bf2(w[0], w[1]), max_bf2(w[2], w[3]));
+    cm = fmaxf(__uint_as_float(mx << 16), __uint_as_float(mx & 0xffff0000u));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = pack2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+  } else {
+    const float w[4] = {max_nan(__uint_as_float(raw.x), kFloor), max_nan(__uint_as_float(raw.y), kFloor),
+                        max_nan(__uint_as_float(raw.z), kFloor), max_nan(__uint_as_float(raw.w), kFloor)};
+    cm = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+    z[0] = pack2(w[0], w[1]);
+    z[1] = pack2(w[2], w[3]);
+  }
+  if (cm > st.limit) {
+    const float ref = cm * c;
+    // from no reference at all the sums are zero; a rise that overflows leaves a NaN, which the exact pass settles
+    const float d = st.limit == -INFINITY ? 0.f : st.ref - ref, f = exp2_fast(d);
+    const f2 ff = pack2(f, f);
+    st.s2 = mul2(ff, fma2(pack2(d, d), st.s1, st.s2));
+    st.s1 = mul2(ff, st.s1);
+    st.ref = ref;
+    st.limit = cm + slack;
+  }
+  if (TOP) { if (cm > st.m) { st.m = cm; st.bu = u; } }
+  else st.m = fmaxf(st.m, cm);
+  const f2 nr = pack2(-st.ref, -st.ref), cc = pack2(c, c);
+#pragma unroll
+  for (int j = 0; j < Row<T>::E / 2; ++j) {
+    const f2 t = fma2(z[j], cc, nr);
+    float x, y;
+    unpack2(t, x, y);
+    const f2 p = pack2(exp2_fast(x), exp2_fast(y));
+    st.s1 = add2(st.s1, p);
+    st.s2 = fma2(p, t, st.s2);
+  }
+}
+
+// Any unit, any values: columns at -inf, a row without a finite number, NaN.
+template <typename T>
+__device__ __forceinline__ void take_exact(Stat& st, int& bu, const float (&v)[Row<T>::E], int u, float c) {
+  constexpr int E = Row<T>::E;
+  float cm = v[0];
+#pragma unroll
+  for (int e = 1; e < E; ++e) cm = fmaxf(cm, v[e]);
+  if (cm > st.m) {
+    if (st.m != -INFINITY) {
+      const float d = fmaxf((st.m - cm) * c, kMinExponent), f = exp2_fast(d);
+      st.s2 = f * (st.s2 + d * st.s1);
+      st.s1 *= f;
+    }
+    st.m = cm;
+    bu = u;
+  }
+  if (st.m == -INFINITY) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) if (v[e] != v[e]) st.s1 = v[e];
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float t = (v[e] - st.m) * c;
+    const float tc = t < kMinExponent ? kMinExponent : t;      // keeps a NaN
+    const float p = exp2_fast(tc);
+    st.s1 += p;
+    st.s2 = fmaf(p, tc, st.s2);
+  }
+}
+
+template <int NT>
+struct TopShared {
+  int sel[NT], nsel, n, ntop, last;
+  uint2 cand[kCandidates];
+  uint2 top[kMaxTop];                 // the k largest in order: {value, column}
+};
+
+// The k largest columns of a row, into sh.top in order.  Thread t holds the units t, t + NT, ... and brings the key of its
+// largest logit and the first unit that holds it.  The k-th largest of those keys bounds the k-th largest column from below,
+// and only the threads above the bound are looked at again (k groups of 64 or 256 elements of a 65536-wide row, from L2):
+// their elements above it are the candidates, ranked by counting.  Returns false, having chosen nothing, when the bound is
+// not above `floor_key`.
+template <typename T, int NT>
+__device__ bool row_top(TopShared<NT>& sh, const Row<T>& r, int k, uint32_t key, int bu, uint32_t floor_key) {
   constexpr int E = Row<T>::E;
   constexpr int SH = sizeof(T) == 2 ? 16 : 0;     // bf16 orders by the upper half of the key
+  const int tid = threadIdx.x;
+  const bool has = tid < r.units;
+  key >>= SH;
+  if (!has) key = 0u;                             // a thread without units has none
+  // a bound that at least k thread maxima reach, the largest one or one that exactly k reach
+  uint32_t bound = 0u;
+  bool exact = false;
+  for (int b = 31 - SH; b >= 0 && !exact; --b) {
+    const uint32_t t = bound | (1u << b);
+    const int n = __syncthreads_count(key >= t);
+    if (n >= k) bound = t;
+    exact = n == k;
+  }
+  if (bound > 0u && bound <= (floor_key >> SH)) return false;
+  if (tid == 0) { sh.nsel = 0; sh.n = 0; }
+  __syncthreads();
+  int last = INT_MAX;                             // maxima equal to the bound count up to this unit
+  if (!exact && bound > 0u) {
+    // several threads share the bound: of those the ones with the lowest units, ranked by counting
+    const int above = __syncthreads_count(key > bound);
+    const bool tie = key == bound;
+    if (tie) sh.sel[atomicAdd(&sh.n, 1)] = bu;
+    if (tid == 0) sh.last = INT_MAX;
+    __syncthreads();
+    const int ties = sh.n;
+    if (tie && ties > k - above) {
+      int before = 0;
+      for (int i = 0; i < ties; ++i) before += sh.sel[i] < bu;
+      if (before == k - above - 1) sh.last = bu;
+    }
+    __syncthreads();
+    last = sh.last;
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+  }
+  if (has && (key > bound || (key == bound && bu <= last))) sh.sel[atomicAdd(&sh.nsel, 1)] = tid;
+  __syncthreads();
+  const int nsel = sh.nsel, per = (r.units + NT - 1) / NT;
+  // every element of the chosen threads' units, in any order
+  auto each = [&](auto&& f) {
+    for (int i = tid; i < nsel * per; i += NT) {
+      const int u = sh.sel[i % nsel] + (i / nsel) * NT;
+      if (u >= r.units) continue;
+      float v[E];
+      r.load(u, v);
+      const int i0 = r.first(u);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int idx = i0 + e;
+        if (idx >= 0 && idx < r.V && v[e] == v[e]) f(order_key(v[e]) >> SH, idx, u, v[e]);
+      }
+    }
+  };
+  auto total = [&](int mine) {                    // sum over the CTA
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    atomicAdd(&sh.n, mine);
+    __syncthreads();
+    const int n = sh.n;
+    __syncthreads();
+    return n;
+  };
+  auto push = [&](float v, int idx) {
+    const int at = atomicAdd(&sh.n, 1);
+    if (at < kCandidates) sh.cand[at] = make_uint2(__float_as_uint(v), (uint32_t)idx);
+  };
+  each([&](uint32_t kk, int idx, int u, float v) { if (kk > bound || (kk == bound && u <= last)) push(v, idx); });
+  __syncthreads();
+  int n = sh.n;
+  __syncthreads();
+  if (n > kCandidates) {
+    // the chosen threads hold long runs above the bound (sorted or blockwise rows): the exact k-th of their elements, by
+    // bisection over the value and then over the index
+    uint32_t kth = 0u;
+    for (int b = 31 - SH; b >= 0; --b) {
+      const uint32_t t = kth | (1u << b);
+      int cnt = 0;
+      each([&](uint32_t kk, int, int, float) { cnt += kk >= t; });
+      if (total(cnt) >= k) kth = t;
+    }
+    int gt = 0;
+    each([&](uint32_t kk, int, int, float) { gt += kk > kth; });
+    const int need = k - total(gt);
+    int lim = 0;                                  // elements equal to the k-th count up to this index
+    for (int b = 30; b >= 0; --b) {
+      int cnt = 0;
+      each([&](uint32_t kk, int idx, int, float) { cnt += kk == kth && idx < (lim | (1 << b)); });
+      if (total(cnt) < need) lim |= 1 << b;
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    each([&](uint32_t kk, int idx, int, float v) { if (kk > kth || (kk == kth && idx <= lim)) push(v, idx); });
+    __syncthreads();
+    n = min(sh.n, kCandidates);
+  }
+  for (int i = tid; i < n; i += NT) {
+    const uint2 mine = sh.cand[i];
+    const float v = __uint_as_float(mine.x);
+    int rank = 0;
+    for (int j = 0; j < n; ++j) {
+      const float w = __uint_as_float(sh.cand[j].x);
+      rank += w > v || (w == v && sh.cand[j].y < mine.y);
+    }
+    if (rank < k) sh.top[rank] = mine;
+  }
+  if (tid == 0) sh.ntop = min(n, k);
+  __syncthreads();
+  return true;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// How far a thread of the forward kernel reads ahead (kStages batches of kBatch units), and how many CTAs share an SM.
+template <int NT> struct Ahead { static constexpr int kBatch = 2, kStages = 5, kResident = 1280 / NT; };
+template <> struct Ahead<kFewRowsThreads> { static constexpr int kBatch = 1, kStages = 4, kResident = 2; };
+
+// Forward: one CTA per row, its threads over the row's 16-byte units.  A thread copies its own units into its own places of
+// shared memory, several batches ahead, so that no thread waits for another and the copies in flight cost no registers.
+// Bound by memory: 4096 x 65536 bf16 take 90.9 us, 5.9 TB/s (a plain read of them 75.6 us), of which the row's start and end
+// leave the rest.  With two register buffers of four units instead of the ring it was 106 us; one CTA going from row to row
+// and reading ahead into the next one 113 us, for the registers that costs.
+template <typename T, bool TOP, int NT>
+__global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(RowStatsArgs a) {
+  constexpr int E = Row<T>::E;
+  constexpr int W = NT / 32;
+  constexpr int kBatch = Ahead<NT>::kBatch, kStages = Ahead<NT>::kStages;
   const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Row<T> r(reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld, a.V);
   const float c = kLog2e * a.inv_tau;
   if (a.mask != nullptr && a.mask[row] == 0.f) {
     // a row that does not count is not read: whatever it holds stays out of the sums
@@ -117,223 +372,174 @@ __global__ void __launch_bounds__(kThreads) row_stats_kernel(RowStatsArgs a) {
     }
     return;
   }
+  __shared__ float sm_m[W];
+  __shared__ float2 sm_s[W], sm_l[W];
+  __shared__ float sm_ln;
+  __shared__ __align__(16) uint4 ring[kStages * kBatch][NT];
+  using Top = typename std::conditional<TOP, TopShared<NT>, int>::type;
+  static_assert(sizeof(Top) <= sizeof(ring), "the alternatives are chosen when the ring has been read");
+  Top& sh = *reinterpret_cast<Top*>(&ring[0][0]);
+  const Row<T> r(reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld, a.V);
 
-  Stat st{-INFINITY, 0.f, 0.f};
-  int bu = tid;
-  auto take = [&](int u, const float (&v)[E]) {
-    float cm = v[0];
+  auto block_max = [&](float m) {
+    m = warp_max(m);
+    if (lane == 0) sm_m[warp] = m;
+    __syncthreads();
+    m = sm_m[0];
 #pragma unroll
-    for (int e = 1; e < E; ++e) cm = fmaxf(cm, v[e]);
-    if (cm > st.m) {
-      if (st.m != -INFINITY) {
-        const float d = fmaxf((st.m - cm) * c, kMinExponent), f = exp2_fast(d);
-        st.s2 = f * (st.s2 + d * st.s1);
-        st.s1 *= f;
-      }
-      st.m = cm;
-      bu = u;
-    }
-    if (st.m == -INFINITY) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) if (v[e] != v[e]) st.s1 = v[e];
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float t = (v[e] - st.m) * c;
-      const float tc = t < kMinExponent ? kMinExponent : t;      // keeps a NaN
-      const float p = exp2_fast(tc);
-      st.s1 += p;
-      st.s2 = fmaf(p, tc, st.s2);
-    }
+    for (int w = 1; w < W; ++w) m = fmaxf(m, sm_m[w]);
+    return m;
   };
-  // first and last unit may be partly outside the row; the whole ones between them are loaded kUnroll at a time
-  const int u_begin = r.whole(0) ? 0 : 1, u_end = r.whole(r.units - 1) ? r.units : r.units - 1;
-  if (u_begin == 1 && tid == 0) { float v[E]; r.load(0, v); take(0, v); }
-  for (int u = tid; u < u_end; u += kUnroll * kThreads) {
-    uint4 raw[kUnroll];
+  auto block_sum2 = [&](float2 (&sm)[W], float x, float y) {
+    x = warp_sum(x);
+    y = warp_sum(y);
+    if (lane == 0) sm[warp] = make_float2(x, y);
+    __syncthreads();
+    float2 t = sm[0];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int ui = u + i * kThreads;
-      if (ui >= u_begin && ui < u_end) raw[i] = *reinterpret_cast<const uint4*>(r.x + r.first(ui));
-    }
+    for (int w = 1; w < W; ++w) { t.x += sm[w].x; t.y += sm[w].y; }
+    return t;
+  };
+  // whole units are [b0, b1); the row's first and last unit may be partly outside of it
+  const int b0 = r.whole(0) ? 0 : 1, b1 = r.whole(r.units - 1) ? r.units : r.units - 1;
+  const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(r.x) & ~uintptr_t(15)) + tid;
+  const uint32_t mine = smem_u32(&ring[0][tid]);
+  const int nb = (b1 + kBatch * NT - 1) / (kBatch * NT);
+  auto issue = [&](int blk, int stage) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int ui = u + i * kThreads;
-      if (ui >= u_begin && ui < u_end) { float v[E]; Row<T>::unpack(raw[i], v); take(ui, v); }
+    for (int i = 0; i < kBatch; ++i) {
+      const int at = (blk * kBatch + i) * NT;
+      if (at + tid >= b0 && at + tid < b1) cp_async16(mine + (uint32_t)((stage * kBatch + i) * NT * 16), base + at);
     }
+    cp_async_commit();                                // past the row's end an empty group
+  };
+#pragma unroll
+  for (int j = 0; j < kStages; ++j) issue(j, j);
+  Running st{0.f, -INFINITY, -INFINITY, 0ull, 0ull, tid};
+  const float slack = kSlack / c;
+  // lifted to the floor, the columns outside of the row have no part
+  auto ragged = [&](int u) {
+    float v[E];
+    r.load(u, v);
+    uint4 raw;
+    if constexpr (sizeof(T) == 2) {
+      __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+    } else {
+      raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    take_fast<T, TOP>(st, raw, u, c, slack);
+  };
+  if (b0 == 1 && tid == 0) ragged(0);
+  int stage = 0;
+  for (int j = 0; j < nb; ++j) {
+    cp_async_wait<kStages - 1>();
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) raw[i] = ring[stage * kBatch + i][tid];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int u = (j * kBatch + i) * NT + tid;
+      if (u >= b0 && u < b1) take_fast<T, TOP>(st, raw[i], u, c, slack);
+    }
+    issue(j + kStages, stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
-  if (u_end < r.units && r.units > 1 && tid == (r.units - 1) % kThreads) { float v[E]; r.load(r.units - 1, v); take(r.units - 1, v); }
+  cp_async_wait<0>();
+  if (b1 < r.units && r.units - 1 >= b0 && tid == (r.units - 1) % NT) ragged(r.units - 1);
 
-  __shared__ Stat sm_stat[kThreads / 32];
-  Stat tot = st;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) tot = merge(tot, shfl_xor(tot, o), c);
-  if (lane == 0) sm_stat[warp] = tot;
-  __syncthreads();
-  tot = sm_stat[0];
-#pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) tot = merge(tot, sm_stat[w], c);
-  const float m = tot.m;
-  const float l2s = log2_row(tot.s1);                 // -inf for a row without a number, NaN for a row with one
-  const float ln_s = tot.s1 > 0.f ? l2s * kLn2 : __int_as_float(0x7fffffff);
+  float m = block_max(st.m);
+  float x0, x1, y0, y1;
+  unpack2(st.s1, x0, x1);
+  unpack2(st.s2, y0, y1);
+  // from the thread's reference to the row's maximum
+  const float d = st.limit == -INFINITY ? 0.f : fmaf(-m, c, st.ref), f = exp2_fast(d), s1 = x0 + x1;
+  float2 tot = block_sum2(sm_s, f * s1, f * fmaf(d, s1, y0 + y1));
+  // overflow, -inf times zero, NaN, a row at the floor: the exact pass below
+  bool done = m > 0.1f * kFloor && fabsf(tot.x) < INFINITY && fabsf(tot.y) < INFINITY;
+  if constexpr (TOP) {
+    if (done) done = row_top<T, NT>(sh, r, a.top_k, order_key(st.m), st.bu, order_key(kFloor * 0.99f));
+  }
+  if (!done) {
+    Stat se{-INFINITY, 0.f, 0.f};
+    int bu = tid;
+    for (int u = tid; u < r.units; u += NT) { float v[E]; r.load(u, v); take_exact<T>(se, bu, v, u, c); }
+    __syncthreads();
+    m = block_max(se.m);
+    const float de = se.m == -INFINITY ? 0.f : fmaxf((se.m - m) * c, kMinExponent), fe = exp2_fast(de);
+    tot = block_sum2(sm_s, fe * se.s1, fe * fmaf(de, se.s1, se.s2));
+    if constexpr (TOP) row_top<T, NT>(sh, r, a.top_k, order_key(se.m), bu, 0u);
+  }
   if (tid == 0) {
+    const float l2s = log2_row(tot.x);                // -inf for a row without a number, NaN for a row with one
+    const float ln_s = tot.x > 0.f ? l2s * kLn2 : __int_as_float(0x7fffffff);
     a.stats[row] = make_float2(m, l2s);
-    if (a.entropy != nullptr) a.entropy[row] = tot.s1 > 0.f ? ln_s - kLn2 * (tot.s2 / tot.s1) : ln_s;
+    if (a.entropy != nullptr) a.entropy[row] = tot.x > 0.f ? ln_s - kLn2 * (tot.y / tot.x) : ln_s;
     if (a.logprob != nullptr) {
       const int id = a.ids[row];
       // an id outside the vocabulary is no token: nothing to score
       a.logprob[row] = (id >= 0 && id < a.V) ? (to_float(r.x[id]) - m) * a.inv_tau - ln_s : 0.f;
     }
+    sm_ln = ln_s;
   }
   if (a.row_loss != nullptr) {
     // distillation: mask tau^2 (sum p ln p - sum p ln q) over the teacher's alternatives
-    float acc = 0.f;
-    for (int j = tid; j < a.K; j += kThreads) {
-      const float p = a.t_prob[(size_t)row * a.K + j];
-      const int id = a.t_ids[(size_t)row * a.K + j];
-      if (p > 0.f) acc += p * ((to_float(r.x[id]) - m) * a.inv_tau - ln_s);
+    float acc = 0.f, psum = 0.f;
+    for (int i = tid; i < a.K; i += NT) {
+      const float p = a.t_prob[(size_t)row * a.K + i];
+      const int id = a.t_ids[(size_t)row * a.K + i];
+      if (p > 0.f) { acc += p * ((to_float(r.x[id]) - m) * a.inv_tau); psum += p; }
     }
-    acc = warp_sum(acc);
-    __shared__ float sm_acc[kThreads / 32];
-    if (lane == 0) sm_acc[warp] = acc;
-    __syncthreads();
+    const float2 t = block_sum2(sm_l, acc, psum);
     if (tid == 0) {
-      float s = 0.f;
-      for (int w = 0; w < kThreads / 32; ++w) s += sm_acc[w];
-      const float2 t = a.t_row[row];                  // sum p ln p, and 1 or 0 for a row without alternatives
-      a.row_loss[row] = t.y > 0.f ? (a.mask != nullptr ? a.mask[row] : 1.f) * a.tau * a.tau * (t.x - s) : 0.f;
+      const float2 tr = a.t_row[row];                 // sum p ln p, and 1 or 0 for a row without alternatives
+      a.row_loss[row] = tr.y > 0.f ? (a.mask != nullptr ? a.mask[row] : 1.f) * a.tau * a.tau * (tr.x - (t.x - t.y * sm_ln)) : 0.f;
     }
   }
   if constexpr (TOP) {
-    __shared__ int sm_sel[kThreads], sm_nsel, sm_n;
-    __shared__ uint2 sm_cand[kCandidates];
-    const int k = a.top_k;
-    const uint32_t key = tid < r.units ? order_key(st.m) >> SH : 0u;     // a thread without units has none
-    // largest bound that at least k thread maxima reach; among equal ones the lowest units
-    uint32_t bound = 0u;
-    for (int b = 31 - SH; b >= 0; --b) {
-      const uint32_t t = bound | (1u << b);
-      if (__syncthreads_count(key >= t) >= k) bound = t;
-    }
-    const int above = __syncthreads_count(key > bound), equal = __syncthreads_count(key == bound && tid < r.units);
-    int last = INT_MAX;                               // equal maxima count up to this unit
-    if (bound > 0u && above + equal > k) {
-      last = 0;
-      for (int b = 30; b >= 0; --b)                   // smallest unit with enough equal maxima at or below it, minus one
-        if (__syncthreads_count(key == bound && bu < (last | (1 << b))) < k - above) last |= 1 << b;
-    }
-    if (tid == 0) { sm_nsel = 0; sm_n = 0; }
-    for (int i = tid; i < k; i += kThreads) {
-      a.top_ids[(size_t)row * k + i] = -1;            // stays where the row has fewer than k numbers
-      a.top_logprobs[(size_t)row * k + i] = __int_as_float(0x7fffffff);
-    }
     __syncthreads();
-    if (tid < r.units && (key > bound || (key == bound && bu <= last))) sm_sel[atomicAdd(&sm_nsel, 1)] = tid;
-    __syncthreads();
-    const int nsel = sm_nsel, per = (r.units + kThreads - 1) / kThreads;
-    // every element of the chosen threads' units, in any order
-    auto each = [&](auto&& f) {
-      for (int i = tid; i < nsel * per; i += kThreads) {
-        const int uu = sm_sel[i % nsel] + (i / nsel) * kThreads;
-        if (uu >= r.units) continue;
-        float v[E];
-        r.load(uu, v);
-        const int i0 = r.first(uu);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int idx = i0 + e;
-          if (idx >= 0 && idx < a.V && v[e] == v[e]) f(order_key(v[e]) >> SH, idx, uu, v[e]);
-        }
-      }
-    };
-    each([&](uint32_t kk, int idx, int uu, float v) {
-      if (kk > bound || (kk == bound && uu <= last)) {
-        const int at = atomicAdd(&sm_n, 1);
-        if (at < kCandidates) sm_cand[at] = make_uint2(__float_as_uint(v), (uint32_t)idx);
-      }
-    });
-    __syncthreads();
-    int n = sm_n;
-    __syncthreads();
-    if (n > kCandidates) {
-      // a row whose chosen threads hold long runs above the bound (sorted or blockwise data): the exact k-th element of
-      // them, by bisection over the value and then over the index
-      uint32_t kth = 0u;
-      for (int b = 31 - SH; b >= 0; --b) {
-        const uint32_t t = kth | (1u << b);
-        int cnt = 0;
-        each([&](uint32_t kk, int, int, float) { cnt += kk >= t; });
-        if (tid == 0) sm_n = 0;
-        __syncthreads();
-        atomicAdd(&sm_n, cnt);
-        __syncthreads();
-        if (sm_n >= k) kth = t;
-        __syncthreads();
-      }
-      int gt = 0;
-      each([&](uint32_t kk, int, int, float) { gt += kk > kth; });
-      if (tid == 0) sm_n = 0;
-      __syncthreads();
-      atomicAdd(&sm_n, gt);
-      __syncthreads();
-      const int need = k - sm_n;
-      __syncthreads();
-      int lim = 0;                                    // elements equal to the k-th count below this index, inclusive
-      for (int b = 30; b >= 0; --b) {
-        int cnt = 0;
-        each([&](uint32_t kk, int idx, int, float) { cnt += kk == kth && idx < (lim | (1 << b)); });
-        if (tid == 0) sm_n = 0;
-        __syncthreads();
-        atomicAdd(&sm_n, cnt);
-        __syncthreads();
-        if (sm_n < need) lim |= 1 << b;
-        __syncthreads();
-      }
-      if (tid == 0) sm_n = 0;
-      __syncthreads();
-      each([&](uint32_t kk, int idx, int, float v) {
-        if (kk > kth || (kk == kth && idx <= lim)) {
-          const int at = atomicAdd(&sm_n, 1);
-          if (at < kCandidates) sm_cand[at] = make_uint2(__float_as_uint(v), (uint32_t)idx);
-        }
-      });
-      __syncthreads();
-      n = min(sm_n, kCandidates);
-    }
-    for (int i = tid; i < n; i += kThreads) {
-      const float v = __uint_as_float(sm_cand[i].x);
-      const uint32_t idx = sm_cand[i].y;
-      int rank = 0;
-      for (int j = 0; j < n; ++j) {
-        const float w = __uint_as_float(sm_cand[j].x);
-        rank += w > v || (w == v && sm_cand[j].y < idx);
-      }
-      if (rank < k) {
-        a.top_ids[(size_t)row * k + rank] = (int)idx;
-        a.top_logprobs[(size_t)row * k + rank] = (v - m) * a.inv_tau - ln_s;
-      }
+    for (int i = tid; i < a.top_k; i += NT) {
+      const bool there = i < sh.ntop;                 // fewer than k numbers in the row: -1, NaN
+      a.top_ids[(size_t)row * a.top_k + i] = there ? (int)sh.top[i].y : -1;
+      a.top_logprobs[(size_t)row * a.top_k + i] =
+          there ? (__uint_as_float(sh.top[i].x) - m) * a.inv_tau - sm_ln : __int_as_float(0x7fffffff);
     }
   }
 }
 
-// Backward: one CTA per kThreads * kUnroll units of a row.  Dense part first, then the columns of the sparse list that lie
-// in this CTA's part are written again with their whole value (the list may name a column more than once).
-template <typename T>
-__global__ void __launch_bounds__(kThreads) row_grad_kernel(RowGradArgs a) {
+// Backward: a CTA takes `iters` blocks of kThreads * kUnroll units of a row, the next block's logits in flight while one is
+// written.  Dense part first, then the columns of the sparse list that lie in this CTA's part are written again with their
+// whole value (the list may name a column more than once).  Rows go from the last to the first: behind a forward pass the
+// end of the logits is what L2 still holds.  Bound by memory: 4096 x 65536 bf16 take 163 us behind the forward pass, 6.6 TB/s
+// of reading and writing, the rate of a plain copy.
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kThreads, 4) row_grad_kernel(RowGradArgs a, int iters) {
   constexpr int E = Row<T>::E;
-  const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int B0 = kThreads * kUnroll;
+  const int row = a.rows - 1 - (int)blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* x = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld;
   T* out = reinterpret_cast<T*>(a.dlogits) + (size_t)row * a.ldd;
   const Row<T> o(out, a.V);                           // units by the output's alignment
-  const int u0 = blockIdx.x * kThreads * kUnroll;
-  if (u0 >= o.units) return;
+  const int u0 = blockIdx.x * B0 * iters, u1 = min(o.units, u0 + B0 * iters);
+  if (u0 >= u1) return;
+  const bool congruent = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  auto fetch = [&](uint4 (&buf)[kUnroll], int u) {
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      const int ui = u + i * kThreads;
+      if (congruent && ui < u1 && o.whole(ui)) buf[i] = __ldg(reinterpret_cast<const uint4*>(x + o.first(ui)));
+    }
+  };
+  // the logits are requested before anything else, so that the row's scalars arrive in their shadow
+  uint4 cur[kUnroll];
+  fetch(cur, u0 + tid);
   float scale = a.weight_mul;
   if (a.g_scale != nullptr) scale *= a.g_scale[0];
   if (a.mask != nullptr) scale = a.mask[row] == 0.f ? 0.f : scale * a.mask[row];
-  const float g_h = a.g_entropy != nullptr ? a.g_entropy[row] : 0.f;
+  const float g_h = ENTROPY ? a.g_entropy[row] : 0.f;
+  const float2 st = a.stats[row];
   __shared__ float sm_w[kThreads / 32];
-  __shared__ int sm_any;
   float wsum = 0.f;
   int any = g_h != 0.f;
   if (scale != 0.f)
@@ -342,68 +548,81 @@ __global__ void __launch_bounds__(kThreads) row_grad_kernel(RowGradArgs a) {
       const float w = a.w[(size_t)row * a.K + j];
       if (id >= 0 && id < a.V && w != 0.f) { wsum += w; any = 1; }
     }
-  any = __syncthreads_or(any);
   wsum = warp_sum(wsum);
   if (lane == 0) sm_w[warp] = wsum;
-  __syncthreads();
+  any = __syncthreads_or(any);
   wsum = 0.f;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) wsum += sm_w[w];
-  const float2 st = a.stats[row];
   const float c = kLog2e * a.inv_tau;
   const float m = st.x, l2s = st.y;
-  const float A = any ? a.inv_tau * (-scale * wsum - (g_h != 0.f ? g_h * a.entropy[row] : 0.f)) : 0.f;
+  const float A = a.inv_tau * (-scale * wsum - (ENTROPY && g_h != 0.f ? g_h * a.entropy[row] : 0.f));
   const float B = -g_h * a.inv_tau * kLn2;            // times log2 q
-  auto value = [&](float z) {
-    float t = (z - m) * c - l2s;
-    t = t < kMinExponent ? kMinExponent : t;
-    return exp2_fast(t) * fmaf(B, t, A);
+  const f2 nm = pack2(-m, -m), cc = pack2(c, c), nl = pack2(-l2s, -l2s), A2 = pack2(A, A), B2 = pack2(B, B);
+  auto value2 = [&](float& z0, float& z1) {
+    f2 t = fma2(add2(pack2(z0, z1), nm), cc, nl);
+    float t0, t1;
+    unpack2(t, t0, t1);
+    if (ENTROPY) {                                    // a column at -inf: 0 * B t
+      t0 = t0 < kMinExponent ? kMinExponent : t0;
+      t1 = t1 < kMinExponent ? kMinExponent : t1;
+      t = pack2(t0, t1);
+    }
+    const f2 q = pack2(exp2_fast(t0), exp2_fast(t1));
+    unpack2(mul2(q, ENTROPY ? fma2(B2, t, A2) : A2), z0, z1);
   };
-  const bool congruent = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const Row<T> r(x, a.V);
+  for (int ub = u0; ub < u1; ub += B0) {
+    uint4 nxt[kUnroll];
+    fetch(nxt, ub + B0 + tid);
 #pragma unroll
-  for (int i = 0; i < kUnroll; ++i) {
-    const int u = u0 + tid + i * kThreads;
-    if (u >= o.units) break;
-    const int i0 = o.first(u);
-    float v[E];
-    if (!any) {
-      // nothing flows into this row (padding, a masked row): its logits are not read, so they may hold anything
+    for (int i = 0; i < kUnroll; ++i) {
+      const int u = ub + tid + i * kThreads;
+      if (u >= u1) break;
+      const int i0 = o.first(u);
+      const bool whole = o.whole(u);
+      float v[E];
+      if (!any) {
+        // nothing flows into this row (padding, a masked row): its logits are not used, so they may hold anything
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = 0.f;
-    } else {
-      if (congruent) r.load(u, v);
-      else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = (i0 + e >= 0 && i0 + e < a.V) ? to_float(x[i0 + e]) : -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = value(v[e]);
-    }
-    if (o.whole(u)) {
-      uint4 raw;
-      if constexpr (sizeof(T) == 2) {
-        __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        for (int e = 0; e < E; ++e) v[e] = 0.f;
       } else {
-        raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-      }
-      *reinterpret_cast<uint4*>(out + i0) = raw;
-    } else {
+        if (congruent && whole) Row<T>::unpack(cur[i], v);
+        else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) if (i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = from_float<T>(v[e]);
+          for (int e = 0; e < E; ++e) v[e] = (i0 + e >= 0 && i0 + e < a.V) ? to_float(x[i0 + e]) : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e += 2) value2(v[e], v[e + 1]);
+      }
+      if (whole) {
+        uint4 w;
+        if constexpr (sizeof(T) == 2) {
+          __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        } else {
+          w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        }
+        *reinterpret_cast<uint4*>(out + i0) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) if (i0 + e >= 0 && i0 + e < a.V) out[i0 + e] = from_float<T>(v[e]);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) cur[i] = nxt[i];
   }
   if (!any) return;
   __syncthreads();
-  const int lo = o.first(u0), hi = o.first(u0 + kThreads * kUnroll);
+  const int lo = o.first(u0), hi = o.first(u1);
   for (int j = tid; j < a.K; j += kThreads) {
     const int id = a.ids[(size_t)row * a.K + j];
     if (id < 0 || id >= a.V || id < lo || id >= hi) continue;
     float w = 0.f;
     for (int i = 0; i < a.K; ++i) if (a.ids[(size_t)row * a.K + i] == id) w += a.w[(size_t)row * a.K + i];
-    out[id] = from_float<T>(value(to_float(x[id])) + scale * w * a.inv_tau);
+    float d = to_float(x[id]), unused = d;
+    value2(d, unused);
+    out[id] = from_float<T>(d + scale * w * a.inv_tau);
   }
 }
 
@@ -591,25 +810,42 @@ __global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
 
 }  // namespace
 
+namespace {
+
+template <typename T, bool TOP, int NT>
+void launch_row_stats_threads(const RowStatsArgs& a, cudaStream_t st) { row_stats_kernel<T, TOP, NT><<<a.rows, NT, 0, st>>>(a); }
+
+// No more rows than SMs: a row is a matter of latency and takes the larger CTA (one bf16 row of 65536: 8.3 us with 512
+// threads, 12.4 with 128).  Many rows: small CTAs, whose starts and ends fall apart (4096 such rows: 90.9 us with 128, 97.6
+// with 256, 117 with 512), but for the alternatives, where a smaller CTA looks at larger groups again (20 of them: 154 us
+// with 128, 139 with 256, 188 with 512).
+template <typename T, bool TOP>
+int launch_row_stats(const RowStatsArgs& a, cudaStream_t st) {
+  if (a.rows <= 148) launch_row_stats_threads<T, TOP, kFewRowsThreads>(a, st);
+  else launch_row_stats_threads<T, TOP, TOP ? kThreads : kThreads / 2>(a, st);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+}  // namespace
+
 int row_stats(const RowStatsArgs& a, cudaStream_t st) {
   if (a.rows <= 0) return 0;
-  if (a.top_k > 0) {
-    if (a.is_bf16) row_stats_kernel<bf16, true><<<a.rows, kThreads, 0, st>>>(a);
-    else row_stats_kernel<float, true><<<a.rows, kThreads, 0, st>>>(a);
-  } else {
-    if (a.is_bf16) row_stats_kernel<bf16, false><<<a.rows, kThreads, 0, st>>>(a);
-    else row_stats_kernel<float, false><<<a.rows, kThreads, 0, st>>>(a);
-  }
-  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+  if (a.top_k > 0) return a.is_bf16 ? launch_row_stats<bf16, true>(a, st) : launch_row_stats<float, true>(a, st);
+  return a.is_bf16 ? launch_row_stats<bf16, false>(a, st) : launch_row_stats<float, false>(a, st);
 }
 
 int row_grad(const RowGradArgs& a, cudaStream_t st) {
   if (a.rows <= 0) return 0;
   const int E = a.is_bf16 ? 8 : 4;
   const int units = (a.V + 2 * E - 2) / E;            // the most a row can touch, whatever its alignment
-  const int parts = (units + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+  const int blocks = (units + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+  // up to four blocks per CTA, as long as that leaves a few waves of CTAs (4096 bf16 rows of 65536: 226 us with one, 179
+  // with two, 163 with four, 164 with eight)
+  int iters = 1;
+  while (iters < 4 && iters < blocks && (int64_t)a.rows * blocks >= 8ll * iters * 4 * 148) iters *= 2;
+  const int parts = (blocks + iters - 1) / iters;
   // the grid's second axis ends at 65535 rows
-  for (int r0 = 0; r0 < a.rows; r0 += 65535) {
+  for (int r0 = (a.rows - 1) / 65535 * 65535; r0 >= 0; r0 -= 65535) {
     RowGradArgs b = a;
     b.rows = a.rows - r0 < 65535 ? a.rows - r0 : 65535;
     const size_t es = a.is_bf16 ? 2 : 4;
@@ -621,8 +857,14 @@ int row_grad(const RowGradArgs& a, cudaStream_t st) {
     if (a.entropy != nullptr) b.entropy = a.entropy + r0;
     if (a.g_entropy != nullptr) b.g_entropy = a.g_entropy + r0;
     if (a.mask != nullptr) b.mask = a.mask + r0;
-    if (a.is_bf16) row_grad_kernel<bf16><<<dim3(parts, b.rows), kThreads, 0, st>>>(b);
-    else row_grad_kernel<float><<<dim3(parts, b.rows), kThreads, 0, st>>>(b);
+    const dim3 grid(parts, b.rows);
+    if (a.g_entropy != nullptr) {
+      if (a.is_bf16) row_grad_kernel<bf16, true><<<grid, kThreads, 0, st>>>(b, iters);
+      else row_grad_kernel<float, true><<<grid, kThreads, 0, st>>>(b, iters);
+    } else {
+      if (a.is_bf16) row_grad_kernel<bf16, false><<<grid, kThreads, 0, st>>>(b, iters);
+      else row_grad_kernel<float, false><<<grid, kThreads, 0, st>>>(b, iters);
+    }
   }
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
