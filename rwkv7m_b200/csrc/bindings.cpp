@@ -2,6 +2,8 @@
 // the launchers declared in kernels.h.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -518,6 +520,307 @@ void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, 
   f.g_l2 = rows_ptr(g_l2, H, 1, "g_l2");
   f.t_ids = t_ids.data_ptr<int>(); f.t_prob = t_prob.data_ptr<float>();
   TORCH_CHECK(rk::head_distill_fix(f, stream()) == 0, "head_distill_loss backward: launch failed");
+}
+
+// ---- the four operators as autograd nodes -----------------------------------------------
+// In C++ because a call on few rows is bound by the host: neither direction enters the Python interpreter.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// [..., V] as a matrix with contiguous rows, a view wherever the strides allow one
+Tensor vocab_rows(const Tensor& x) {
+  Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)});
+  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+Tensor id_rows(const Tensor& ids) { return ids.reshape({-1}).to(at::kInt).contiguous(); }
+c10::optional<Tensor> mask_rows(const c10::optional<Tensor>& mask) {
+  if (!mask.has_value()) return c10::nullopt;
+  return mask->reshape({-1}).to(at::kFloat).contiguous();
+}
+c10::optional<Tensor> grad_rows(const Tensor& g) {
+  if (!g.defined()) return c10::nullopt;
+  return g.reshape({-1}).to(at::kFloat).contiguous();
+}
+c10::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
+std::vector<int64_t> with_last(at::IntArrayRef lead, int64_t k) {
+  std::vector<int64_t> v = lead.vec();
+  v.push_back(k);
+  return v;
+}
+// The kernels have no second derivative: asking for one raises when it is used, as torch's once_differentiable does.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  std::vector<Tensor> defined;
+  for (Tensor& g : grads) if (g.defined()) defined.push_back(g);
+  auto delayed = std::make_shared<torch::autograd::DelayedError>("this operator can be differentiated only once", (int)defined.size());
+  for (Tensor& d : defined) d.requires_grad_(true);
+  variable_list out = (*delayed)(std::move(defined));
+  size_t i = 0;
+  for (Tensor& g : grads) if (g.defined()) g = out[i++];
+  return grads;
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static variable_list run(const Tensor& logits, const Tensor& ids, int64_t top_k, double tau, AutogradContext* ctx) {
+    Tensor z = vocab_rows(logits), idr = id_rows(ids);
+    std::vector<Tensor> out = token_logprobs_fwd(z, idr, top_k, tau);
+    const at::IntArrayRef lead = ids.sizes();
+    if (ctx != nullptr) {
+      ctx->set_materialize_grads(false);
+      ctx->save_for_backward({z, idr, out[0], out[2], top_k > 0 ? out[3] : Tensor()});
+      ctx->saved_data["tau"] = tau;
+      ctx->saved_data["shape"] = logits.sizes().vec();
+    }
+    variable_list res = {out[1].view(lead), out[2].view(lead)};
+    if (top_k > 0) {
+      res.push_back(out[3].view(with_last(lead, top_k)));
+      res.push_back(out[4].view(with_last(lead, top_k)));
+      if (ctx != nullptr) ctx->mark_non_differentiable({res[2]});
+    }
+    return res;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& ids, int64_t top_k, double tau) {
+    return run(logits, ids, top_k, tau, ctx);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &z = saved[0], &stats = saved[2], &ent = saved[3], &top_ids = saved[4];
+    const Tensor g_top = g.size() > 3 ? g[3] : Tensor();
+    if (!g[0].defined() && !g[1].defined() && !g_top.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const double tau = ctx->saved_data["tau"].toDouble();
+    Tensor dz;
+    {
+      at::NoGradGuard no_grad;
+      c10::cuda::CUDAGuard guard(z.device());
+      const int64_t R = z.size(0);
+      Tensor ids = saved[1].view({R, 1});
+      Tensor w = g[0].defined() ? grad_rows(g[0])->view({R, 1}) : torch::zeros({R, 1}, stats.options());
+      if (g_top.defined()) {
+        const int64_t k = top_ids.size(1);
+        ids = torch::cat({ids, top_ids}, 1);
+        w = torch::cat({w, g_top.reshape({R, k}).to(at::kFloat)}, 1);
+      }
+      dz = logits_grad(z, stats, ids, w, tau, 1.0, ent, grad_rows(g[1]), c10::nullopt, c10::nullopt)
+               .view(ctx->saved_data["shape"].toIntVector());
+    }
+    return once({dz, Tensor(), Tensor(), Tensor()});
+  }
+};
+
+variable_list token_logprobs(const Tensor& logits, const Tensor& ids, int64_t top_k, double tau) {
+  c10::cuda::CUDAGuard guard(logits.device());
+  if (wants_grad(logits)) return TokenLogprobs::apply(logits, ids, top_k, tau);
+  at::NoGradGuard no_grad;
+  return TokenLogprobs::run(logits, ids, top_k, tau, nullptr);
+}
+
+// {ids, p, {sum p ln p, any}} sorted by id
+std::vector<Tensor> teacher_rows(const Tensor& t_ids, const Tensor& t_logits, int64_t V, double tau) {
+  const int64_t K = t_logits.size(-1), R = t_logits.numel() / K;
+  Tensor t = t_logits.reshape({R, K});
+  if (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kFloat) t = t.to(at::kFloat);
+  return teacher_prepare(t_ids.reshape({R, K}).to(at::kInt).contiguous(), t.contiguous(), V, tau);
+}
+
+struct DistillLoss : torch::autograd::Function<DistillLoss> {
+  static variable_list run(const Tensor& logits, const Tensor& t_ids, const Tensor& t_logits, const c10::optional<Tensor>& mask,
+                           double tau, AutogradContext* ctx) {
+    Tensor z = vocab_rows(logits);
+    const std::vector<Tensor> t = teacher_rows(t_ids, t_logits, z.size(1), tau);
+    const c10::optional<Tensor> msk = mask_rows(mask);
+    std::vector<Tensor> out = distill_fwd(z, t[0], t[1], t[2], msk, tau);
+    if (ctx != nullptr) {
+      ctx->set_materialize_grads(false);
+      ctx->save_for_backward({z, t[0], t[1], out[0], msk.value_or(Tensor())});
+      ctx->saved_data["tau"] = tau;
+      ctx->saved_data["shape"] = logits.sizes().vec();
+      ctx->mark_non_differentiable({out[2]});
+    }
+    return {out[1], out[2]};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& t_ids, const Tensor& t_logits,
+                               const c10::optional<Tensor>& mask, double tau) {
+    return run(logits, t_ids, t_logits, mask, tau, ctx);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined()) return variable_list(5);
+    const variable_list saved = ctx->get_saved_variables();
+    const double tau = ctx->saved_data["tau"].toDouble();
+    Tensor dz;
+    {
+      at::NoGradGuard no_grad;
+      dz = logits_grad(saved[0], saved[3], saved[1], saved[2], tau, -tau * tau, c10::nullopt, c10::nullopt, grad_rows(g[0]),
+                       maybe(saved[4]))
+               .view(ctx->saved_data["shape"].toIntVector());
+    }
+    return once({dz, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+variable_list distill_loss(const Tensor& logits, const Tensor& t_ids, const Tensor& t_logits, const c10::optional<Tensor>& mask,
+                           double tau) {
+  c10::cuda::CUDAGuard guard(logits.device());
+  if (wants_grad(logits)) return DistillLoss::apply(logits, t_ids, t_logits, mask, tau);
+  at::NoGradGuard no_grad;
+  return DistillLoss::run(logits, t_ids, t_logits, mask, tau, nullptr);
+}
+
+// A bf16 matrix whose base and row pitch suit bulk-tensor copies.
+Tensor aligned_rows(const Tensor& x) {
+  const bool ok = x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) &&
+                  reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+// dh and dW from the gradient of the logits, which `fill(begin, rows, dz)` writes chunk by chunk of rows into one buffer.  A
+// single chunk stores dW in the weight's dtype; several accumulate it in fp32, as does a bound main gradient.
+template <typename F>
+std::pair<Tensor, Tensor> head_backward(const Tensor& h, const Tensor& wc, at::ScalarType w_type, const c10::optional<Tensor>& main,
+                                        int64_t chunk, int64_t pair, bool need_h, bool need_w, F&& fill) {
+  const int64_t M = h.size(0), C = h.size(1), V = wc.size(0), step = std::min(chunk, M);
+  Tensor buf = torch::empty({step, (V + 7) / 8 * 8}, h.options());
+  Tensor dh, dw;
+  if (need_h) dh = torch::empty({M, C}, h.options());
+  const bool direct = step == M && w_type == at::kBFloat16;
+  if (need_w && !main.has_value()) dw = torch::empty({V, C}, h.options().dtype(direct ? at::kBFloat16 : at::kFloat));
+  for (int64_t s = 0; s < M; s += step) {
+    const int64_t n = std::min(step, M - s);
+    Tensor dz = buf.narrow(0, 0, n).narrow(1, 0, V), hs = h.narrow(0, s, n);
+    fill(s, n, dz);
+    if (need_h) gemm(dz, wc, dh.narrow(0, s, n), rk::kGemmNN, rk::kEpiStoreBf16, pair, c10::nullopt, 0);
+    if (!need_w) continue;
+    if (main.has_value()) gemm(dz, hs, *main, rk::kGemmNT_wgrad, rk::kEpiAccumF32, pair, c10::nullopt, 0);
+    else gemm(dz, hs, dw, rk::kGemmNT_wgrad, direct ? rk::kEpiStoreBf16 : (s == 0 ? rk::kEpiStoreF32 : rk::kEpiAccumF32), pair, c10::nullopt, 0);
+  }
+  if (dw.defined()) dw = dw.to(w_type);
+  return {dh, dw};
+}
+
+// What every head node saves besides its own tensors.
+void save_head(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const c10::optional<Tensor>& main, double tau, int64_t chunk,
+               int64_t pair) {
+  ctx->set_materialize_grads(false);
+  ctx->saved_data["tau"] = tau;
+  ctx->saved_data["shape"] = hidden.sizes().vec();
+  ctx->saved_data["w_type"] = (int64_t)w.scalar_type();
+  ctx->saved_data["main"] = main;             // written in backward, so not a saved variable
+  ctx->saved_data["chunk"] = chunk;
+  ctx->saved_data["pair"] = pair;
+  ctx->saved_data["need_h"] = hidden.requires_grad();
+  ctx->saved_data["need_w"] = w.requires_grad();
+}
+template <typename F>
+std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, const Tensor& wc, F&& fill) {
+  auto& d = ctx->saved_data;
+  auto r = head_backward(h, wc, (at::ScalarType)d["w_type"].toInt(), d["main"].toOptional<Tensor>(), d["chunk"].toInt(), d["pair"].toInt(),
+                         d["need_h"].toBool(), d["need_w"].toBool(), fill);
+  if (r.first.defined()) r.first = r.first.view(d["shape"].toIntVector());
+  return r;
+}
+c10::optional<Tensor> part(const c10::optional<Tensor>& t, int64_t s, int64_t n) {
+  return t.has_value() ? c10::optional<Tensor>(t->narrow(0, s, n)) : c10::nullopt;
+}
+
+// `wc` is the bf16 weight that the products read (w itself, or the copy kept beside it), `main` a bound fp32 main gradient.
+struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
+  static variable_list run(const Tensor& hidden, const Tensor& w, const Tensor& wc_in, const c10::optional<Tensor>& main,
+                           const Tensor& ids, double tau, int64_t chunk, int64_t pair, AutogradContext* ctx) {
+    Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), idr = id_rows(ids);
+    std::vector<Tensor> out = head_prob_stats(h, wc, idr, tau, pair);
+    if (ctx != nullptr) {
+      save_head(ctx, hidden, w, main, tau, chunk, pair);
+      ctx->save_for_backward({h, wc, idr, out[2], out[3]});
+    }
+    return {out[0].view(ids.sizes()), out[1].view(ids.sizes())};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const Tensor& wc,
+                               const c10::optional<Tensor>& main, const Tensor& ids, double tau, int64_t chunk, int64_t pair) {
+    return run(hidden, w, wc, main, ids, tau, chunk, pair, ctx);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined() && !g[1].defined()) return variable_list(8);
+    const variable_list s = ctx->get_saved_variables();
+    std::pair<Tensor, Tensor> r;
+    {
+      at::NoGradGuard no_grad;
+      c10::cuda::CUDAGuard guard(s[0].device());
+      const c10::optional<Tensor> g_lp = grad_rows(g[0]), g_ent = grad_rows(g[1]);
+      const double tau = ctx->saved_data["tau"].toDouble();
+      const int64_t pair = ctx->saved_data["pair"].toInt();
+      r = head_backward(ctx, s[0], s[1], [&](int64_t b, int64_t n, const Tensor& dz) {
+        head_prob_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(g_lp, b, n),
+                       part(g_ent, b, n), tau, dz, pair);
+      });
+    }
+    variable_list grads(8);
+    grads[0] = r.first;
+    grads[1] = r.second;
+    return once(grads);
+  }
+};
+
+variable_list head_token_logprobs(const Tensor& hidden, const Tensor& w, const Tensor& wc, const c10::optional<Tensor>& main,
+                                  const Tensor& ids, double tau, int64_t chunk, int64_t pair) {
+  c10::cuda::CUDAGuard guard(hidden.device());
+  if (wants_grad(hidden) || wants_grad(w)) return HeadTokenLogprobs::apply(hidden, w, wc, main, ids, tau, chunk, pair);
+  at::NoGradGuard no_grad;
+  return HeadTokenLogprobs::run(hidden, w, wc, main, ids, tau, chunk, pair, nullptr);
+}
+
+struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
+  static variable_list run(const Tensor& hidden, const Tensor& w, const Tensor& wc_in, const c10::optional<Tensor>& main,
+                           const Tensor& targets, const c10::optional<Tensor>& mask, const Tensor& t_ids, const Tensor& t_logits,
+                           double tau, int64_t chunk, int64_t pair, AutogradContext* ctx) {
+    Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), tgt = id_rows(targets);
+    const std::vector<Tensor> t = teacher_rows(t_ids, t_logits, wc.size(0), tau);
+    std::vector<Tensor> out = head_distill_stats(h, wc, tgt, mask_rows(mask), t[0], t[1], t[2], tau, pair);
+    if (ctx != nullptr) {
+      save_head(ctx, hidden, w, main, tau, chunk, pair);
+      ctx->save_for_backward({h, wc, tgt, t[0], t[1], out[6], out[7], out[8], out[9], out[10]});
+      ctx->mark_non_differentiable({out[1], out[3], out[5]});
+    }
+    return {out[0], out[1], out[2], out[3], out[4], out[5]};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const Tensor& wc,
+                               const c10::optional<Tensor>& main, const Tensor& targets, const c10::optional<Tensor>& mask,
+                               const Tensor& t_ids, const Tensor& t_logits, double tau, int64_t chunk, int64_t pair) {
+    return run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, pair, ctx);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined() && !g[2].defined() && !g[4].defined()) return variable_list(11);
+    const variable_list s = ctx->get_saved_variables();
+    std::pair<Tensor, Tensor> r;
+    {
+      at::NoGradGuard no_grad;
+      c10::cuda::CUDAGuard guard(s[0].device());
+      const c10::optional<Tensor> g_ce = grad_rows(g[0]), g_l2 = grad_rows(g[2]), g_kd = grad_rows(g[4]);
+      const double tau = ctx->saved_data["tau"].toDouble();
+      const int64_t pair = ctx->saved_data["pair"].toInt();
+      r = head_backward(ctx, s[0], s[1], [&](int64_t b, int64_t n, const Tensor& dz) {
+        std::vector<Tensor> rows;
+        for (int i = 5; i < 10; ++i) rows.push_back(s[i].narrow(0, b, n));
+        head_distill_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), rows, s[3].narrow(0, b, n), s[4].narrow(0, b, n), g_ce, g_l2,
+                          g_kd, tau, dz, pair);
+      });
+    }
+    variable_list grads(11);
+    grads[0] = r.first;
+    grads[1] = r.second;
+    return once(grads);
+  }
+};
+
+variable_list head_distill_loss(const Tensor& hidden, const Tensor& w, const Tensor& wc, const c10::optional<Tensor>& main,
+                                const Tensor& targets, const c10::optional<Tensor>& mask, const Tensor& t_ids, const Tensor& t_logits,
+                                double tau, int64_t chunk, int64_t pair) {
+  c10::cuda::CUDAGuard guard(hidden.device());
+  if (wants_grad(hidden) || wants_grad(w))
+    return HeadDistillLoss::apply(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, pair);
+  at::NoGradGuard no_grad;
+  return HeadDistillLoss::run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, pair, nullptr);
 }
 
 // Up to four y_i = act_i(A_i B_i^T) with the same number of rows in one launch (bf16 in, bf16 out).  Returns false, having
@@ -1200,14 +1503,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_bwd", &embedding_bwd);
   m.def("ce_fwd", &ce_fwd);
   m.def("gemm_ce_stats", &gemm_ce_stats);
-  m.def("token_logprobs_fwd", &token_logprobs_fwd);
-  m.def("logits_grad", &logits_grad);
-  m.def("teacher_prepare", &teacher_prepare);
-  m.def("distill_fwd", &distill_fwd);
-  m.def("head_prob_stats", &head_prob_stats);
-  m.def("head_prob_grad", &head_prob_grad);
-  m.def("head_distill_stats", &head_distill_stats);
-  m.def("head_distill_grad", &head_distill_grad);
+  m.def("token_logprobs", &token_logprobs, py::call_guard<py::gil_scoped_release>());
+  m.def("distill_loss", &distill_loss, py::call_guard<py::gil_scoped_release>());
+  m.def("head_token_logprobs", &head_token_logprobs, py::call_guard<py::gil_scoped_release>());
+  m.def("head_distill_loss", &head_distill_loss, py::call_guard<py::gil_scoped_release>());
   m.def("ce_bwd", &ce_bwd);
   m.def("dp_step", &dp_step);
   m.def("dp_step_timings", &dp_step_timings);

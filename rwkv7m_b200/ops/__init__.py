@@ -11,7 +11,6 @@ PyTorch bodies on any device and exists for the numerics tests.
 from __future__ import annotations
 
 import contextlib
-import math
 from typing import NamedTuple
 
 import torch
@@ -274,8 +273,8 @@ TEACHER_K_MAX = 256       # alternatives a teacher may give per position
 
 def _check_temperature(temperature):
     t = float(temperature)
-    if not (t > 0.0 and math.isfinite(t)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-4 <= t <= 1e4:
+        raise ValueError(f"temperature must lie between 1e-4 and 1e4, got {temperature}")
     return t
 
 
@@ -356,7 +355,7 @@ def distill_loss(logits, teacher_ids, teacher_logits, mask=None, *, temperature=
     _check_mask("distill_loss", mask, logits.shape[:-1], logits.device)
     temperature = _check_temperature(temperature)
     if use_cuda(logits):
-        return _cuda().distill_loss(logits, teacher_ids, teacher_logits, mask, temperature)
+        return tuple(_cuda().distill_loss(logits, teacher_ids, teacher_logits, mask, temperature))
     return reference.distill_loss(logits, teacher_ids, teacher_logits, mask, temperature)
 
 

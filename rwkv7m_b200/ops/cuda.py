@@ -12,7 +12,6 @@ from __future__ import annotations
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import reference as R
 from .build import load_extension
@@ -1077,119 +1076,22 @@ def head_loss(hidden, ln_w, ln_b, head_w, targets, mask, chunk=None, eps=1e-5):
 # ---------------------------------------------------------------------------
 
 
-def _vocab_rows(x):
-    """[..., V] as a matrix whose rows are contiguous; a view wherever the strides allow one."""
-    x2 = x.reshape(-1, x.shape[-1])
-    return x2 if x2.stride(1) == 1 or x2.shape[1] == 1 else x2.contiguous()
-
-
-def _id_rows(ids, *shape):
-    return ids.reshape(shape).to(torch.int32).contiguous()
-
-
-def _mask_rows(mask):
-    return None if mask is None else mask.detach().reshape(-1).float().contiguous()
-
-
-def _scalar_grad(g):
-    return g.float().reshape(1).contiguous()
-
-
-class TokenLogprobsFn(torch.autograd.Function):
-    """Statistics, log-probability, entropy and alternatives in one pass over the logits; backward one pass more."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, top_k, tau):
-        ctx.set_materialize_grads(False)
-        z = _vocab_rows(logits)
-        idr = _id_rows(ids, -1)
-        out = _C.token_logprobs_fwd(z, idr, top_k, tau)
-        _count()
-        stats, lp, ent = out[:3]
-        top_ids, top_lp = out[3:] if top_k else (None, None)
-        ctx.tau, ctx.shape = tau, logits.shape
-        ctx.save_for_backward(z, idr, stats, ent, top_ids)
-        lead = logits.shape[:-1]
-        res = (lp.view(lead), ent.view(lead))
-        if not top_k:
-            return res + (None, None)
-        top_ids = top_ids.view(*lead, top_k)
-        ctx.mark_non_differentiable(top_ids)
-        return res + (top_ids, top_lp.view(*lead, top_k))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, _g_ids, g_top):
-        z, ids, stats, ent, top_ids = ctx.saved_tensors
-        if g_lp is None and g_ent is None and g_top is None:
-            return None, None, None, None
-        ids = ids.view(-1, 1)
-        w = torch.zeros(ids.shape, device=z.device) if g_lp is None else g_lp.float().reshape(-1, 1).contiguous()
-        if g_top is not None:
-            k = top_ids.shape[-1]
-            ids = torch.cat((ids, top_ids.view(-1, k)), dim=1)
-            w = torch.cat((w, g_top.float().reshape(-1, k)), dim=1)
-        g_ent = None if g_ent is None else g_ent.float().reshape(-1).contiguous()
-        dz = _C.logits_grad(z, stats, ids, w, ctx.tau, 1.0, ent, g_ent, None, None)
-        _count()
-        return dz.view(ctx.shape), None, None, None
+# The four operators are autograd nodes of the extension (csrc/bindings.cpp): a call on few rows is bound by the host, so
+# neither direction enters the interpreter.  The launches of their backward passes are not part of LAUNCH_COUNT.
 
 
 def token_logprobs(logits, ids, top_k, tau):
-    return TokenLogprobsFn.apply(logits, ids, top_k, tau)
-
-
-def _teacher_rows(teacher_ids, teacher_logits, V, tau):
-    """(ids, p, {sum p ln p, any}) of the teacher's alternatives, sorted by id within each row."""
-    K = teacher_logits.shape[-1]
-    t = teacher_logits.detach().reshape(-1, K)
-    if t.dtype not in (torch.bfloat16, torch.float32):
-        t = t.float()
-    out = _C.teacher_prepare(_id_rows(teacher_ids, -1, K), t.contiguous(), V, tau)
     _count()
-    return out
-
-
-class DistillLossFn(torch.autograd.Function):
-    """Distillation from logits: the teacher's rows, one pass over the logits, the totals; backward one pass more."""
-
-    @staticmethod
-    def forward(ctx, logits, teacher_ids, teacher_logits, mask, tau):
-        z = _vocab_rows(logits)
-        ids, p, trow = _teacher_rows(teacher_ids, teacher_logits, z.shape[1], tau)
-        msk = _mask_rows(mask)
-        stats, total, count = _C.distill_fwd(z, ids, p, trow, msk, tau)
-        _count(2)
-        ctx.tau, ctx.shape = tau, logits.shape
-        ctx.save_for_backward(z, ids, p, stats, msk)
-        ctx.mark_non_differentiable(count)
-        return total, count
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_kd, _g_count):
-        z, ids, p, stats, msk = ctx.saved_tensors
-        dz = _C.logits_grad(z, stats, ids, p, ctx.tau, -ctx.tau * ctx.tau, None, None, _scalar_grad(g_kd), msk)
-        _count()
-        return dz.view(ctx.shape), None, None, None, None
+    return _C.token_logprobs(logits, ids, top_k, tau)
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, mask, tau):
-    return DistillLossFn.apply(logits, teacher_ids, teacher_logits, mask, tau)
+    _count(3)
+    return _C.distill_loss(logits, teacher_ids, teacher_logits, mask, tau)
 
 
 # Rows of the [rows, V] bf16 gradient of the logits that a backward pass through the head holds at a time.
 HEAD_GRAD_ROWS = 8192
-
-
-def _aligned_rows(x):
-    """A bf16 matrix whose base and row pitch suit bulk-tensor copies."""
-    ok = x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1] and x.data_ptr() % 16 == 0
-    return x if ok else x.clone(memory_format=torch.contiguous_format)
-
-
-def _head_operands(hidden, head_w):
-    return _aligned_rows(hidden.detach().reshape(-1, hidden.shape[-1])), _aligned_rows(_compute_weight(head_w))
 
 
 def _head_kernels_apply(hidden):
@@ -1201,113 +1103,30 @@ def _head_logits(hidden, head_w):
     return hidden.float() @ head_w.float().T
 
 
-def _head_backward(ctx, h2, wc, fill):
-    """dh and dW from the gradient of the logits, which ``fill(begin, end, dz)`` writes chunk by chunk of rows into one
-    buffer.  A single chunk stores dW in the weight's dtype; several accumulate it in fp32, as does a bound main gradient."""
-    w = ctx.weight
-    M, C = h2.shape
-    V = wc.shape[0]
-    dev = h2.device
-    need_h, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    step = min(HEAD_GRAD_ROWS, M)
-    buf = torch.empty(step, (V + 7) // 8 * 8, dtype=torch.bfloat16, device=dev)
-    dh = torch.empty(M, C, dtype=torch.bfloat16, device=dev) if need_h else None
-    main = getattr(w, "_main_grad", None) if need_w else None
-    if main is not None and main.dtype != torch.float32:
-        main = None
-    dw = None
-    if need_w and main is None:
-        direct = step == M and w.dtype == torch.bfloat16
-        dw = torch.empty(V, C, dtype=torch.bfloat16 if direct else torch.float32, device=dev)
-    for s in range(0, M, step):
-        e = min(M, s + step)
-        dz = buf[: e - s, :V]
-        fill(s, e, dz)
-        if need_h:
-            gemm(dz, wc, dh[s:e], GEMM_NN, EPI_BF16)
-        if main is not None:
-            gemm(dz, h2[s:e], main, GEMM_WGRAD, EPI_ACC_F32)
-        elif need_w:
-            epi = EPI_BF16 if dw.dtype == torch.bfloat16 else (EPI_F32 if s == 0 else EPI_ACC_F32)
-            gemm(dz, h2[s:e], dw, GEMM_WGRAD, epi)
-    return (None if dh is None else dh.view(ctx.h_shape)), (None if dw is None else dw.to(w.dtype))
-
-
-class HeadTokenLogprobsFn(torch.autograd.Function):
-    """Log-probability and entropy through the head.  Forward: one product whose epilogue reduces every 256-column tile of
-    the fp32 logits to (maximum, sum of exponentials, their sum weighted by the exponent), one kernel that folds the tiles.
-    Backward: the same product again with an epilogue that turns the fp32 logits into their gradient, rounded once to bf16
-    as the operand of the two gradient products."""
-
-    @staticmethod
-    def forward(ctx, hidden, head_w, ids, tau):
-        ctx.set_materialize_grads(False)
-        h2, wc = _head_operands(hidden, head_w)
-        idr = _id_rows(ids, -1)
-        lp, ent, stat, tz = _C.head_prob_stats(h2, wc, idr, tau, int(GEMM_PAIR))
-        _count(2)
-        ctx.tau, ctx.weight, ctx.h_shape = tau, head_w, hidden.shape
-        ctx.save_for_backward(h2, wc, idr, stat, tz)
-        return lp.view(ids.shape), ent.view(ids.shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent):
-        if g_lp is None and g_ent is None:
-            return None, None, None, None
-        h2, wc, ids, stat, tz = ctx.saved_tensors
-        g_lp, g_ent = (None if g is None else g.float().reshape(-1).contiguous() for g in (g_lp, g_ent))
-
-        def fill(s, e, dz):
-            _C.head_prob_grad(h2[s:e], wc, ids[s:e], stat[s:e], tz[s:e], None if g_lp is None else g_lp[s:e],
-                              None if g_ent is None else g_ent[s:e], ctx.tau, dz, int(GEMM_PAIR))
-            _count(2)
-
-        return _head_backward(ctx, h2, wc, fill) + (None, None)
+def _head_operands(hidden, head_w):
+    """(hidden, weight, the bf16 weight that the products read, its bound fp32 main gradient or None)."""
+    main = getattr(head_w, "_main_grad", None)
+    return hidden, head_w, _compute_weight(head_w), main if main is not None and main.dtype == torch.float32 else None
 
 
 def head_token_logprobs(hidden, head_w, ids, tau):
+    """Forward: one product whose epilogue reduces every 256-column tile of the fp32 logits to (maximum, sum of
+    exponentials, their sum weighted by the exponent), one kernel that folds the tiles.  Backward: the same product again with
+    an epilogue that turns the fp32 logits into their gradient, rounded once to bf16 as the operand of the two gradient
+    products."""
     if _head_kernels_apply(hidden):
-        return HeadTokenLogprobsFn.apply(hidden, head_w, ids, tau)
-    return token_logprobs(_head_logits(hidden, head_w), ids, 0, tau)[:2]
-
-
-class HeadDistillLossFn(torch.autograd.Function):
-    """Cross-entropy, L2Wrap and distillation through the head: one product forward (its epilogue also writes the logits of
-    the target and of the teacher's alternatives), three backward, as :class:`HeadTokenLogprobsFn`."""
-
-    @staticmethod
-    def forward(ctx, hidden, head_w, targets, mask, teacher_ids, teacher_logits, tau):
-        ctx.set_materialize_grads(False)
-        h2, wc = _head_operands(hidden, head_w)
-        ids, p, trow = _teacher_rows(teacher_ids, teacher_logits, wc.shape[0], tau)
-        tgt = _id_rows(targets, -1)
-        out = _C.head_distill_stats(h2, wc, tgt, _mask_rows(mask), ids, p, trow, tau, int(GEMM_PAIR))
-        _count(3)
-        ctx.tau, ctx.weight, ctx.h_shape = tau, head_w, hidden.shape
-        ctx.save_for_backward(h2, wc, tgt, ids, p, *out[6:])
-        ctx.mark_non_differentiable(out[1], out[3], out[5])
-        return tuple(out[:6])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_ce, _n0, g_l2, _n1, g_kd, _n2):
-        if g_ce is None and g_l2 is None and g_kd is None:
-            return (None,) * 7
-        h2, wc, tgt, ids, p, *saved = ctx.saved_tensors
-        g_ce, g_l2, g_kd = (None if g is None else _scalar_grad(g) for g in (g_ce, g_l2, g_kd))
-
-        def fill(s, e, dz):
-            _C.head_distill_grad(h2[s:e], wc, tgt[s:e], [x[s:e] for x in saved], ids[s:e], p[s:e], g_ce, g_l2, g_kd, ctx.tau,
-                                 dz, int(GEMM_PAIR))
-            _count(2)
-
-        return _head_backward(ctx, h2, wc, fill) + (None,) * 5
+        _count(2)
+        return tuple(_C.head_token_logprobs(*_head_operands(hidden, head_w), ids, tau, HEAD_GRAD_ROWS, int(GEMM_PAIR)))
+    return tuple(token_logprobs(_head_logits(hidden, head_w), ids, 0, tau)[:2])
 
 
 def head_distill_loss(hidden, head_w, targets, mask, teacher_ids, teacher_logits, tau):
+    """One product forward (its epilogue also writes the logits of the target and of the teacher's alternatives), three
+    backward, as :func:`head_token_logprobs`."""
     if _head_kernels_apply(hidden):
-        return HeadDistillLossFn.apply(hidden, head_w, targets, mask, teacher_ids, teacher_logits, tau)
+        _count(4)
+        return tuple(_C.head_distill_loss(*_head_operands(hidden, head_w), targets, mask, teacher_ids, teacher_logits, tau,
+                                          HEAD_GRAD_ROWS, int(GEMM_PAIR)))
     logits = _head_logits(hidden, head_w)
     kd = distill_loss(logits, teacher_ids, teacher_logits, mask, tau)
     return R.distill_components(logits, targets, mask, teacher_ids, teacher_logits, tau, kd=kd)

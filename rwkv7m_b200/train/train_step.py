@@ -88,8 +88,8 @@ class DistillConfig:
     def __post_init__(self):
         if not 0.0 <= self.weight <= 1.0:
             raise ValueError("the distillation weight must lie between 0 and 1")
-        if not 0.0 < self.temperature < float("inf"):
-            raise ValueError("the distillation temperature must be positive and finite")
+        if not 1e-4 <= self.temperature <= 1e4:
+            raise ValueError("the distillation temperature must lie between 1e-4 and 1e4")
 
 
 def set_distillation(model, config: DistillConfig | None):
