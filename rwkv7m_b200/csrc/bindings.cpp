@@ -380,18 +380,33 @@ void check_head(const Tensor& H, const Tensor& W, const char* name) {
               name, ": bf16 row-major hidden states [M, C] and weight [V, C]");
 }
 
-// -> logprob, entropy [M], and for the backward pass stat [M, 4] and the targets' z [M]
-std::vector<Tensor> head_prob_stats(const Tensor& H, const Tensor& W, const Tensor& ids, double tau, int64_t pair) {
+// The logits of a forward pass kept for its backward pass (undefined = recompute them there).
+Tensor keep_logits(const Tensor& H, const Tensor& W, bool keep) {
+  return keep ? torch::empty({H.size(0), (W.size(0) + 7) / 8 * 8}, H.options().dtype(at::kFloat)) : Tensor();
+}
+void set_kept(rk::GemmArgs& p, const Tensor& z, int64_t row) {
+  if (!z.defined()) return;
+  p.vocab.z = z.data_ptr<float>() + row * z.stride(0);
+  p.vocab.ldz = (int)z.stride(0);
+}
+const float* check_kept(const Tensor& z, const Tensor& H, const Tensor& W) {
+  check_rows(z, H, at::kFloat, {H.size(0), (W.size(0) + 7) / 8 * 8}, "kept logits");
+  return z.data_ptr<float>();
+}
+
+// -> logprob, entropy [M], and for the backward pass stat [M, 4], the targets' z [M] and the kept logits
+std::vector<Tensor> head_prob_stats(const Tensor& H, const Tensor& W, const Tensor& ids, double tau, int64_t pair, bool keep) {
   check_head(H, W, "head_token_logprobs");
   c10::cuda::CUDAGuard guard(H.device());
   const int64_t M = H.size(0), V = W.size(0), tiles = (V + 255) / 256;
   check_rows(ids, H, at::kInt, {M}, "ids");
   auto f32 = H.options().dtype(at::kFloat);
   Tensor lp = torch::empty({M}, f32), ent = torch::empty({M}, f32), stat = torch::empty({M, 4}, f32), tz = torch::empty({M}, f32);
-  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32);
+  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32), kept = keep_logits(H, W, keep);
   for (int64_t r = 0; r < M; r += kHeadStatsRows) {
     const int64_t n = std::min(kHeadStatsRows, M - r);
     rk::GemmArgs p = head_gemm(H, W, r, n, rk::kEpiProbStats, pair, tau);
+    set_kept(p, kept, r);
     p.D = buf.data_ptr(); p.ldd = (int)(tiles * 4);
     p.vocab.target = ids.data_ptr<int>() + r;
     p.vocab.target_z = tz.data_ptr<float>() + r;
@@ -403,7 +418,7 @@ std::vector<Tensor> head_prob_stats(const Tensor& H, const Tensor& W, const Tens
                                       stream()) == 0,
                 "head_token_logprobs: combine launch failed");
   }
-  return {lp, ent, stat, tz};
+  return {lp, ent, stat, tz, kept};
 }
 
 void check_dz(const Tensor& dz, const Tensor& H, const Tensor& W) {
@@ -415,7 +430,8 @@ void check_dz(const Tensor& dz, const Tensor& H, const Tensor& W) {
 
 // Gradient of the rows' log-probabilities and entropies with respect to z, into dz (bf16 [M, V], padded row pitch).
 void head_prob_grad(const Tensor& H, const Tensor& W, const Tensor& ids, const Tensor& stat, const Tensor& tz,
-                    const c10::optional<Tensor>& g_lp, const c10::optional<Tensor>& g_ent, double tau, Tensor dz, int64_t pair) {
+                    const Tensor& kept, const c10::optional<Tensor>& g_lp, const c10::optional<Tensor>& g_ent, double tau, Tensor dz,
+                    int64_t pair) {
   check_head(H, W, "head_token_logprobs");
   c10::cuda::CUDAGuard guard(H.device());
   check_dz(dz, H, W);
@@ -429,18 +445,24 @@ void head_prob_grad(const Tensor& H, const Tensor& W, const Tensor& ids, const T
   p.vocab.stat = reinterpret_cast<const float4*>(stat.data_ptr<float>());
   p.vocab.g0 = rows_ptr(g_lp, H, M, "g_logprob");
   p.vocab.g1 = rows_ptr(g_ent, H, M, "g_entropy");
-  const int rc = rk::gemm_bf16(p, stream());
-  TORCH_CHECK(rc == 0, "head_token_logprobs backward: product launch failed with code ", rc);
   rk::HeadFix f{};
   f.dz = p.D; f.ld = dz.stride(0); f.rows = (int)M; f.V = (int)V; f.tau = (float)tau;
   f.target = p.vocab.target; f.target_z = tz.data_ptr<float>(); f.stat = p.vocab.stat; f.g0 = p.vocab.g0; f.g1 = p.vocab.g1;
+  if (kept.defined()) {
+    TORCH_CHECK(rk::head_prob_grad_kept(f, check_kept(kept, H, W), kept.stride(0), stream()) == 0,
+                "head_token_logprobs backward: launch failed");
+    return;
+  }
+  const int rc = rk::gemm_bf16(p, stream());
+  TORCH_CHECK(rc == 0, "head_token_logprobs backward: product launch failed with code ", rc);
   TORCH_CHECK(rk::head_prob_fix(f, stream()) == 0, "head_token_logprobs backward: launch failed");
 }
 
 // -> scalars ce_total, ce_count, l2_total, l2_count, kd_total, kd_count, then stat [M, 4], weight [M, 2], argmax, target z [M],
-// z of the teacher's alternatives [M, K]
+// z of the teacher's alternatives [M, K], the kept logits
 std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const Tensor& targets, const c10::optional<Tensor>& mask,
-                                       const Tensor& t_ids, const Tensor& t_prob, const Tensor& t_row, double tau, int64_t pair) {
+                                       const Tensor& t_ids, const Tensor& t_prob, const Tensor& t_row, double tau, int64_t pair,
+                                       bool keep) {
   check_head(H, W, "head_distill_loss");
   c10::cuda::CUDAGuard guard(H.device());
   const int64_t M = H.size(0), V = W.size(0), K = t_ids.size(1), tiles = (V + 255) / 256;
@@ -452,11 +474,12 @@ std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const T
   auto f32 = H.options().dtype(at::kFloat);
   Tensor stat = torch::empty({M, 4}, f32), weight = torch::empty({M, 2}, f32), am = torch::empty({M}, f32.dtype(at::kInt));
   Tensor tz = torch::empty({M}, f32), cz = torch::empty({M, K}, f32), rows = torch::empty({4, M}, f32);
-  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32);
+  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32), kept = keep_logits(H, W, keep);
   float* rp = rows.data_ptr<float>();
   for (int64_t r = 0; r < M; r += kHeadStatsRows) {
     const int64_t n = std::min(kHeadStatsRows, M - r);
     rk::GemmArgs p = head_gemm(H, W, r, n, rk::kEpiDistillStats, pair, tau);
+    set_kept(p, kept, r);
     p.D = buf.data_ptr(); p.ldd = (int)(tiles * 4);
     p.vocab.target = targets.data_ptr<int>() + r;
     p.vocab.target_z = tz.data_ptr<float>() + r;
@@ -487,13 +510,13 @@ std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const T
     t.in[i] = in[i]; t.out[i] = out[i].data_ptr<float>();
   }
   TORCH_CHECK(rk::row_totals(t, stream()) == 0, "head_distill_loss: totals launch failed");
-  for (const Tensor& x : {stat, weight, am, tz, cz}) out.push_back(x);
+  for (const Tensor& x : {stat, weight, am, tz, cz, kept}) out.push_back(x);
   return out;
 }
 
 // Gradient of g_ce ce_total + g_l2 l2_total + g_kd kd_total with respect to z, into dz (bf16 [M, V], padded row pitch).
 void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, const std::vector<Tensor>& saved, const Tensor& t_ids,
-                       const Tensor& t_prob, const c10::optional<Tensor>& g_ce, const c10::optional<Tensor>& g_l2,
+                       const Tensor& t_prob, const Tensor& kept, const c10::optional<Tensor>& g_ce, const c10::optional<Tensor>& g_l2,
                        const c10::optional<Tensor>& g_kd, double tau, Tensor dz, int64_t pair) {
   check_head(H, W, "head_distill_loss");
   c10::cuda::CUDAGuard guard(H.device());
@@ -509,8 +532,6 @@ void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, 
   p.vocab.weight = reinterpret_cast<const float2*>(check_rows(saved[1], H, at::kFloat, {M, 2}, "weight").data_ptr<float>());
   p.vocab.g0 = rows_ptr(g_ce, H, 1, "g_ce");
   p.vocab.g1 = rows_ptr(g_kd, H, 1, "g_kd");
-  const int rc = rk::gemm_bf16(p, stream());
-  TORCH_CHECK(rc == 0, "head_distill_loss backward: product launch failed with code ", rc);
   rk::HeadFix f{};
   f.dz = p.D; f.ld = dz.stride(0); f.rows = (int)M; f.V = (int)V; f.K = (int)K; f.tau = (float)tau;
   f.target = targets.data_ptr<int>(); f.stat = p.vocab.stat; f.weight = p.vocab.weight; f.g0 = p.vocab.g0; f.g1 = p.vocab.g1;
@@ -519,6 +540,13 @@ void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, 
   f.cols_z = check_rows(saved[4], H, at::kFloat, {M, K}, "listed logits").data_ptr<float>();
   f.g_l2 = rows_ptr(g_l2, H, 1, "g_l2");
   f.t_ids = t_ids.data_ptr<int>(); f.t_prob = t_prob.data_ptr<float>();
+  if (kept.defined()) {
+    TORCH_CHECK(rk::head_distill_grad_kept(f, check_kept(kept, H, W), kept.stride(0), stream()) == 0,
+                "head_distill_loss backward: launch failed");
+    return;
+  }
+  const int rc = rk::gemm_bf16(p, stream());
+  TORCH_CHECK(rc == 0, "head_distill_loss backward: product launch failed with code ", rc);
   TORCH_CHECK(rk::head_distill_fix(f, stream()) == 0, "head_distill_loss backward: launch failed");
 }
 
@@ -675,6 +703,27 @@ Tensor aligned_rows(const Tensor& x) {
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
+// dh [M, C] = dz [M, V] W [V, C]
+void hidden_grad(const Tensor& dz, const Tensor& wc, Tensor dh, int64_t pair) {
+  const int64_t M = dh.size(0), C = dh.size(1);
+  const int planes = rk::gemm_planes((int)M, (int)C, (int)dz.size(1), pair != 0);
+  if (planes == 1) {
+    gemm(dz, wc, dh, rk::kGemmNN, rk::kEpiStoreBf16, pair, c10::nullopt, 0);
+    return;
+  }
+  Tensor slices = torch::empty({planes, M, C}, dh.options().dtype(at::kFloat));
+  rk::GemmArgs p{};
+  p.A = dz.data_ptr(); p.B = wc.data_ptr(); p.D = slices.data_ptr();
+  p.lda = (int)dz.stride(0); p.ldb = (int)wc.stride(0); p.ldd = (int)C;
+  p.M = (int)M; p.N = (int)C; p.K = (int)dz.size(1);
+  p.layout = rk::kGemmNN; p.epilogue = rk::kEpiStoreF32; p.pair = (int)pair; p.planes = planes;
+  p.error_flag = gemm_error_flag(dz.device()).data_ptr<int>();
+  const int rc = rk::gemm_bf16(p, stream());
+  TORCH_CHECK(rc == 0, "gradient of the hidden states: launch failed with code ", rc);
+  TORCH_CHECK(rk::gemm_sum_planes(slices.data_ptr<float>(), dh.data_ptr(), (size_t)M * C, planes, stream()) == 0,
+              "gradient of the hidden states: sum of the slices failed");
+}
+
 // dh and dW from the gradient of the logits, which `fill(begin, rows, dz)` writes chunk by chunk of rows into one buffer.  A
 // single chunk stores dW in the weight's dtype; several accumulate it in fp32, as does a bound main gradient.
 template <typename F>
@@ -690,7 +739,7 @@ std::pair<Tensor, Tensor> head_backward(const Tensor& h, const Tensor& wc, at::S
     const int64_t n = std::min(step, M - s);
     Tensor dz = buf.narrow(0, 0, n).narrow(1, 0, V), hs = h.narrow(0, s, n);
     fill(s, n, dz);
-    if (need_h) gemm(dz, wc, dh.narrow(0, s, n), rk::kGemmNN, rk::kEpiStoreBf16, pair, c10::nullopt, 0);
+    if (need_h) hidden_grad(dz, wc, dh.narrow(0, s, n), pair);
     if (!need_w) continue;
     if (main.has_value()) gemm(dz, hs, *main, rk::kGemmNT_wgrad, rk::kEpiAccumF32, pair, c10::nullopt, 0);
     else gemm(dz, hs, dw, rk::kGemmNT_wgrad, direct ? rk::kEpiStoreBf16 : (s == 0 ? rk::kEpiStoreF32 : rk::kEpiAccumF32), pair, c10::nullopt, 0);
@@ -720,6 +769,9 @@ std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, c
   if (r.first.defined()) r.first = r.first.view(d["shape"].toIntVector());
   return r;
 }
+// Logits are kept between the passes while they fit into `keep_bytes`.
+bool keeps(const Tensor& h, const Tensor& wc, int64_t keep_bytes) { return h.size(0) * ((wc.size(0) + 7) / 8 * 8) * 4 <= keep_bytes; }
+Tensor part(const Tensor& t, int64_t s, int64_t n) { return t.defined() ? t.narrow(0, s, n) : t; }
 c10::optional<Tensor> part(const c10::optional<Tensor>& t, int64_t s, int64_t n) {
   return t.has_value() ? c10::optional<Tensor>(t->narrow(0, s, n)) : c10::nullopt;
 }
@@ -727,21 +779,21 @@ c10::optional<Tensor> part(const c10::optional<Tensor>& t, int64_t s, int64_t n)
 // `wc` is the bf16 weight that the products read (w itself, or the copy kept beside it), `main` a bound fp32 main gradient.
 struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
   static variable_list run(const Tensor& hidden, const Tensor& w, const Tensor& wc_in, const c10::optional<Tensor>& main,
-                           const Tensor& ids, double tau, int64_t chunk, int64_t pair, AutogradContext* ctx) {
+                           const Tensor& ids, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair, AutogradContext* ctx) {
     Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), idr = id_rows(ids);
-    std::vector<Tensor> out = head_prob_stats(h, wc, idr, tau, pair);
+    std::vector<Tensor> out = head_prob_stats(h, wc, idr, tau, pair, ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {
       save_head(ctx, hidden, w, main, tau, chunk, pair);
-      ctx->save_for_backward({h, wc, idr, out[2], out[3]});
+      ctx->save_for_backward({h, wc, idr, out[2], out[3], out[4]});
     }
     return {out[0].view(ids.sizes()), out[1].view(ids.sizes())};
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const Tensor& wc,
-                               const c10::optional<Tensor>& main, const Tensor& ids, double tau, int64_t chunk, int64_t pair) {
-    return run(hidden, w, wc, main, ids, tau, chunk, pair, ctx);
+                               const c10::optional<Tensor>& main, const Tensor& ids, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
+    return run(hidden, w, wc, main, ids, tau, chunk, keep_bytes, pair, ctx);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    if (!g[0].defined() && !g[1].defined()) return variable_list(8);
+    if (!g[0].defined() && !g[1].defined()) return variable_list(9);
     const variable_list s = ctx->get_saved_variables();
     std::pair<Tensor, Tensor> r;
     {
@@ -751,11 +803,11 @@ struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
       const double tau = ctx->saved_data["tau"].toDouble();
       const int64_t pair = ctx->saved_data["pair"].toInt();
       r = head_backward(ctx, s[0], s[1], [&](int64_t b, int64_t n, const Tensor& dz) {
-        head_prob_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(g_lp, b, n),
+        head_prob_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[5], b, n), part(g_lp, b, n),
                        part(g_ent, b, n), tau, dz, pair);
       });
     }
-    variable_list grads(8);
+    variable_list grads(9);
     grads[0] = r.first;
     grads[1] = r.second;
     return once(grads);
@@ -763,34 +815,35 @@ struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
 };
 
 variable_list head_token_logprobs(const Tensor& hidden, const Tensor& w, const Tensor& wc, const c10::optional<Tensor>& main,
-                                  const Tensor& ids, double tau, int64_t chunk, int64_t pair) {
+                                  const Tensor& ids, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
   c10::cuda::CUDAGuard guard(hidden.device());
-  if (wants_grad(hidden) || wants_grad(w)) return HeadTokenLogprobs::apply(hidden, w, wc, main, ids, tau, chunk, pair);
+  if (wants_grad(hidden) || wants_grad(w)) return HeadTokenLogprobs::apply(hidden, w, wc, main, ids, tau, chunk, keep_bytes, pair);
   at::NoGradGuard no_grad;
-  return HeadTokenLogprobs::run(hidden, w, wc, main, ids, tau, chunk, pair, nullptr);
+  return HeadTokenLogprobs::run(hidden, w, wc, main, ids, tau, chunk, keep_bytes, pair, nullptr);
 }
 
 struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
   static variable_list run(const Tensor& hidden, const Tensor& w, const Tensor& wc_in, const c10::optional<Tensor>& main,
                            const Tensor& targets, const c10::optional<Tensor>& mask, const Tensor& t_ids, const Tensor& t_logits,
-                           double tau, int64_t chunk, int64_t pair, AutogradContext* ctx) {
+                           double tau, int64_t chunk, int64_t keep_bytes, int64_t pair, AutogradContext* ctx) {
     Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), tgt = id_rows(targets);
     const std::vector<Tensor> t = teacher_rows(t_ids, t_logits, wc.size(0), tau);
-    std::vector<Tensor> out = head_distill_stats(h, wc, tgt, mask_rows(mask), t[0], t[1], t[2], tau, pair);
+    std::vector<Tensor> out = head_distill_stats(h, wc, tgt, mask_rows(mask), t[0], t[1], t[2], tau, pair,
+                                                 ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {
       save_head(ctx, hidden, w, main, tau, chunk, pair);
-      ctx->save_for_backward({h, wc, tgt, t[0], t[1], out[6], out[7], out[8], out[9], out[10]});
+      ctx->save_for_backward({h, wc, tgt, t[0], t[1], out[6], out[7], out[8], out[9], out[10], out[11]});
       ctx->mark_non_differentiable({out[1], out[3], out[5]});
     }
     return {out[0], out[1], out[2], out[3], out[4], out[5]};
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const Tensor& wc,
                                const c10::optional<Tensor>& main, const Tensor& targets, const c10::optional<Tensor>& mask,
-                               const Tensor& t_ids, const Tensor& t_logits, double tau, int64_t chunk, int64_t pair) {
-    return run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, pair, ctx);
+                               const Tensor& t_ids, const Tensor& t_logits, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
+    return run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, keep_bytes, pair, ctx);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    if (!g[0].defined() && !g[2].defined() && !g[4].defined()) return variable_list(11);
+    if (!g[0].defined() && !g[2].defined() && !g[4].defined()) return variable_list(12);
     const variable_list s = ctx->get_saved_variables();
     std::pair<Tensor, Tensor> r;
     {
@@ -802,11 +855,11 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
       r = head_backward(ctx, s[0], s[1], [&](int64_t b, int64_t n, const Tensor& dz) {
         std::vector<Tensor> rows;
         for (int i = 5; i < 10; ++i) rows.push_back(s[i].narrow(0, b, n));
-        head_distill_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), rows, s[3].narrow(0, b, n), s[4].narrow(0, b, n), g_ce, g_l2,
+        head_distill_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), rows, s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[10], b, n), g_ce, g_l2,
                           g_kd, tau, dz, pair);
       });
     }
-    variable_list grads(11);
+    variable_list grads(12);
     grads[0] = r.first;
     grads[1] = r.second;
     return once(grads);
@@ -815,12 +868,12 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
 
 variable_list head_distill_loss(const Tensor& hidden, const Tensor& w, const Tensor& wc, const c10::optional<Tensor>& main,
                                 const Tensor& targets, const c10::optional<Tensor>& mask, const Tensor& t_ids, const Tensor& t_logits,
-                                double tau, int64_t chunk, int64_t pair) {
+                                double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
   c10::cuda::CUDAGuard guard(hidden.device());
   if (wants_grad(hidden) || wants_grad(w))
-    return HeadDistillLoss::apply(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, pair);
+    return HeadDistillLoss::apply(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, keep_bytes, pair);
   at::NoGradGuard no_grad;
-  return HeadDistillLoss::run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, pair, nullptr);
+  return HeadDistillLoss::run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, keep_bytes, pair, nullptr);
 }
 
 // Up to four y_i = act_i(A_i B_i^T) with the same number of rows in one launch (bf16 in, bf16 out).  Returns false, having

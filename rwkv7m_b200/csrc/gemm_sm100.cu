@@ -208,6 +208,11 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&v)[32], void* __res
         }
 }
 
+// Output plane of a K slice (kEpiStoreF32 with GemmArgs::planes): slices are kept apart, so their sum has a fixed order.
+__device__ __forceinline__ void* plane_of(void* D, int split, int M, int ldd) {
+  return reinterpret_cast<float*>(D) + (size_t)split * M * ldd;
+}
+
 // Cross-entropy statistics of one output row over the columns of a tile (kEpiCeStats): the logits are rounded to bf16
 // first, so the numbers equal those of a pass over a stored bf16 logits matrix, which the backward recomputes.
 struct CeRow { float m, s, tl; int am; };
@@ -304,38 +309,6 @@ __device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, uint32_t (&v)[32
   st.s2 += b[0] + b[1];
 }
 
-// Statistics of this thread's row over the 256 columns of a tile, from the accumulator at taddr.
-template <int EPI>
-__device__ __forceinline__ void vocab_stats_tile(uint32_t taddr, int n0, int N, int row, int M, float4* __restrict__ out,
-                                                 const GemmVocab& g) {
-  const bool live = row < M;
-  VocabRow st{-INFINITY, 0.f, 0.f, 0, 0, 0x7fffffff, -1};
-  if (live) {
-    st.tgt = g.target[row];
-    if (EPI == kEpiDistillStats) {
-      const int* cols = g.cols + (size_t)row * g.listed;
-      int lo = 0, hi = g.listed;             // first listed column at or right of this tile
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (cols[mid] < n0) lo = mid + 1; else hi = mid;
-      }
-      st.k = lo;
-      if (lo < g.listed) st.next = cols[lo];
-    }
-  }
-#pragma unroll 1
-  for (int c = 0; c < 8; c += 2) {
-    uint32_t v0[32], v1[32];
-    tmem_ld_32x32(taddr + c * 32, v0);
-    tmem_ld_32x32(taddr + c * 32 + 32, v1);
-    tmem_ld_wait();
-    vocab_stats_chunk<EPI>(st, v0, n0 + c * 32, N, (size_t)row, g);
-    vocab_stats_chunk<EPI>(st, v1, n0 + c * 32 + 32, N, (size_t)row, g);
-  }
-  if (live)
-    *out = EPI == kEpiProbStats ? make_float4(st.m, st.s1, st.s2, 0.f) : make_float4(st.m, st.s2, st.s1, __int_as_float(st.am));
-}
-
 // A row's factors of the gradient epilogues: dz = q (A + B log2 q) with log2 q = z c + b, or a1 2^(z log2e + b1) + a 2^(z c + b).
 // A row that nothing flows into has live = false and gets zeros, whatever its z.
 struct VocabCoef { float b, A, B, b1; bool live; };
@@ -382,6 +355,67 @@ __device__ __forceinline__ void vocab_grad_chunk(uint32_t (&v)[32], const VocabC
 constexpr int kOutStageBytes = 128 * 128;   // 128 rows x 64 bf16
 
 __device__ __forceinline__ void epilogue_named_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// A chunk of 32 fp32 columns of this thread's row into a 16 KB staging buffer (128 rows x 128 bytes, 128-byte swizzle).
+__device__ __forceinline__ void stage_f32(const uint32_t (&v)[32], uint8_t* buf, int tile_row) {
+  uint8_t* dst = buf + tile_row * 128;
+  const int sw = tile_row & 7;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(dst + ((j ^ sw) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  fence_proxy_async_smem();
+}
+
+// Statistics of this thread's row over the 256 columns of a tile, from the accumulator at taddr.  With `tm` not null the
+// logits are stored as well, boxes of 128 rows x 32 columns through the staging buffers, while their statistics are taken.
+template <int EPI>
+__device__ __forceinline__ void vocab_stats_tile(uint32_t taddr, int m0, int tile_row, int n0, int N, int M, float4* __restrict__ out,
+                                                 const GemmVocab& g, const CUtensorMap* tm, uint8_t* out_stage, bool issuer) {
+  const int row = m0 + tile_row;
+  const bool live = row < M;
+  VocabRow st{-INFINITY, 0.f, 0.f, 0, 0, 0x7fffffff, -1};
+  if (live) {
+    st.tgt = g.target[row];
+    if (EPI == kEpiDistillStats) {
+      const int* cols = g.cols + (size_t)row * g.listed;
+      int lo = 0, hi = g.listed;             // first listed column at or right of this tile
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (cols[mid] < n0) lo = mid + 1; else hi = mid;
+      }
+      st.k = lo;
+      if (lo < g.listed) st.next = cols[lo];
+    }
+  }
+#pragma unroll 1
+  for (int c = 0; c < 8; c += 2) {
+    uint32_t v0[32], v1[32];
+    tmem_ld_32x32(taddr + c * 32, v0);
+    tmem_ld_32x32(taddr + c * 32 + 32, v1);
+    tmem_ld_wait();
+    if (tm != nullptr && m0 < M) {           // the same for all 128 threads
+      const int c0 = n0 + c * 32;
+      if (c0 < N) {
+        stage_f32(v0, out_stage, tile_row);
+        if (c0 + 32 < N) stage_f32(v1, out_stage + kOutStageBytes, tile_row);
+        epilogue_named_barrier();
+        if (issuer) {
+          tma_store_2d(tm, out_stage, c0, m0);
+          if (c0 + 32 < N) tma_store_2d(tm, out_stage + kOutStageBytes, c0 + 32, m0);
+          tma_store_commit();
+        }
+      }
+    }
+    vocab_stats_chunk<EPI>(st, v0, n0 + c * 32, N, (size_t)row, g);
+    vocab_stats_chunk<EPI>(st, v1, n0 + c * 32 + 32, N, (size_t)row, g);
+    if (tm != nullptr && m0 < M) {           // both buffers are free again before the next round writes them
+      if (issuer) tma_store_wait_read<0>();
+      epilogue_named_barrier();
+    }
+  }
+  if (live)
+    *out = EPI == kEpiProbStats ? make_float4(st.m, st.s1, st.s2, 0.f) : make_float4(st.m, st.s2, st.s1, __int_as_float(st.am));
+}
 
 // aux_row (two-input epilogues): this thread's 64 bf16 of the second input, or nullptr for a row past the matrix edge
 template <int EPI>
@@ -593,7 +627,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (row < M)
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
       } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
-        vocab_stats_tile<EPI>(t0, n0, N, row, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab);
+        vocab_stats_tile<EPI>(t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
+                              tma_out != 0 ? &tmD : nullptr, out_stage, issuer);
       } else if constexpr (BN >= 64) {
         VocabCoef coef;
         if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
@@ -620,22 +655,25 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               obuf ^= 1;
             }
           } else if constexpr (!kVocabGrad) {
-            store_chunk<EPI>(v0, Dptr, row, n0 + c * 32, M, N, ldd, atomic, aux, ldaux, act);
-            store_chunk<EPI>(v1, Dptr, row, n0 + c * 32 + 32, M, N, ldd, atomic, aux, ldaux, act);
+            void* D = EPI == kEpiStoreF32 ? plane_of(Dptr, work / num_tiles, M, ldd) : Dptr;
+            store_chunk<EPI>(v0, D, row, n0 + c * 32, M, N, ldd, atomic, aux, ldaux, act);
+            store_chunk<EPI>(v1, D, row, n0 + c * 32 + 32, M, N, ldd, atomic, aux, ldaux, act);
           }
         }
       } else {
         uint32_t v[32];
         tmem_ld_32x32(t0, v);
         tmem_ld_wait();
-        store_chunk<EPI>(v, Dptr, row, n0, M, N, ldd, atomic, aux, ldaux, act);
+        store_chunk<EPI>(v, EPI == kEpiStoreF32 ? plane_of(Dptr, work / num_tiles, M, ldd) : Dptr, row, n0, M, N, ldd, atomic, aux,
+                         ldaux, act);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty_bar[acc]);
       acc ^= 1; if (acc == 0) acc_phase ^= 1u;
     }
-    if (staged && issuer) tma_store_wait<0>();   // the staging buffers are read until the last store has drained
+    if ((staged || ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && tma_out != 0)) && issuer)
+      tma_store_wait<0>();   // the staging buffers are read until the last store has drained
     if (!ok && lane == 0) { *abort_flag = 1; atomicExch(err, 0x10000 | 3); }
   }
 
@@ -1008,7 +1046,8 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (row < M)
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
       } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
-        vocab_stats_tile<EPI>(t0, n0, N, row, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab);
+        vocab_stats_tile<EPI>(t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
+                              tma_out != 0 ? &tmD : nullptr, out_stage, issuer);
       } else {
       VocabCoef coef;
       if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
@@ -1034,8 +1073,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
             obuf ^= 1;
           }
         } else if constexpr (!kVocabGrad) {
-          store_chunk<EPI>(v0, Dptr, row, n0 + c * 32, M, N, ldd, atomic, aux, ldaux, act);
-          store_chunk<EPI>(v1, Dptr, row, n0 + c * 32 + 32, M, N, ldd, atomic, aux, ldaux, act);
+          void* D = EPI == kEpiStoreF32 ? plane_of(Dptr, work / num_tiles, M, ldd) : Dptr;
+          store_chunk<EPI>(v0, D, row, n0 + c * 32, M, N, ldd, atomic, aux, ldaux, act);
+          store_chunk<EPI>(v1, D, row, n0 + c * 32 + 32, M, N, ldd, atomic, aux, ldaux, act);
         }
       }
       }
@@ -1044,7 +1084,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[acc]), 0));
       acc ^= 1; if (acc == 0) acc_phase ^= 1u;
     }
-    if (staged && issuer) tma_store_wait<0>();
+    if ((staged || ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && tma_out != 0)) && issuer) tma_store_wait<0>();
     if (!ok && lane == 0) { *abort_flag = 1; atomicExch(err, 0x30000 | 3); }
   }
 
@@ -1081,29 +1121,30 @@ EncodeTiledFn encode_fn() {
 }
 
 struct MapKey {
-  const void* ptr; int rows, cols, ld, box_rows;
+  const void* ptr; int rows, cols, ld, box_rows; bool f32;
   bool operator==(const MapKey& o) const {
-    return ptr == o.ptr && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows;
+    return ptr == o.ptr && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows && f32 == o.f32;
   }
 };
 struct MapKeyHash {
   size_t operator()(const MapKey& k) const {
     size_t h = reinterpret_cast<size_t>(k.ptr);
     h ^= (size_t)k.rows * 0x9E3779B97F4A7C15ull + (size_t)k.cols * 0xC2B2AE3D27D4EB4Full;
-    h ^= ((size_t)k.ld << 20) ^ (size_t)k.box_rows;
+    h ^= ((size_t)k.ld << 20) ^ (size_t)k.box_rows ^ ((size_t)k.f32 << 40);
     return h;
   }
 };
 
-// Row-major bf16 matrix [rows, cols] with leading dimension ld; box = 64 columns x box_rows rows, 128B swizzle.
+// Row-major bf16 (or fp32) matrix [rows, cols] with leading dimension ld; box = 128 bytes of columns x box_rows rows, 128B
+// swizzle.
 // The cache stores the 128 descriptor bytes as a plain byte array: CUtensorMap is 64-byte aligned and
 // node-based containers do not honour that alignment under every host compiler configuration.
 struct MapBytes { unsigned char raw[sizeof(CUtensorMap)]; };
 
-bool make_map(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int box_rows) {
+bool make_map(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int box_rows, bool f32 = false) {
   static std::unordered_map<MapKey, MapBytes, MapKeyHash> cache;
   static std::mutex mu;
-  MapKey key{ptr, rows, cols, ld, box_rows};
+  MapKey key{ptr, rows, cols, ld, box_rows, f32};
   {
     std::lock_guard<std::mutex> g(mu);
     auto it = cache.find(key);
@@ -1122,10 +1163,10 @@ bool make_map(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int
     context_bound = true;
   }
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-  cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * (f32 ? 4 : 2)};
+  cuuint32_t box[2] = {f32 ? 32u : 64u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+  CUresult r = fn(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return false;
@@ -1199,6 +1240,10 @@ int launch(const GemmArgs& p, cudaStream_t st) {
       (reinterpret_cast<uintptr_t>(p.D) & 15) == 0 && p.ldd % 8 == 0 &&
       (!kTwoInput || (p.N % 64 == 0 && (reinterpret_cast<uintptr_t>(p.aux) & 15) == 0 && p.ldaux % 8 == 0)))
     tma_out = make_map(&td, p.D, p.M, p.N, p.ldd, BM) ? 1 : 0;
+  if ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && p.vocab.z != nullptr) {
+    if (!make_map(&td, p.vocab.z, p.M, p.N, p.vocab.ldz, BM, true)) return 2;
+    tma_out = 1;
+  }
   if (kVocabGrad && tma_out == 0) return 2;
   RK_TRACE("maps ok\n");
   auto kern = gemm_bf16_kernel<BN, A_MN, B_MN, EPI>;
@@ -1219,6 +1264,7 @@ int launch(const GemmArgs& p, cudaStream_t st) {
     const int per = (num_kb + splits - 1) / splits;
     splits = (num_kb + per - 1) / per;   // no empty split
   }
+  if (EPI == kEpiStoreF32 && p.planes > 1) splits = p.planes;
   const int work = tiles * splits;
   const int grid = work < sm_count() ? work : sm_count();
   RK_TRACE("attr ok grid=%d smem=%d splits=%d\n", grid, TL::kSmemBytes, splits);
@@ -1306,6 +1352,10 @@ int launch_pair(const GemmArgs& p, cudaStream_t st) {
       (reinterpret_cast<uintptr_t>(p.D) & 15) == 0 && p.ldd % 8 == 0 &&
       (!kTwoInput || (p.N % 64 == 0 && (reinterpret_cast<uintptr_t>(p.aux) & 15) == 0 && p.ldaux % 8 == 0)))
     tma_out = make_map(&td, p.D, p.M, p.N, p.ldd, BM) ? 1 : 0;
+  if ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && p.vocab.z != nullptr) {
+    if (!make_map(&td, p.vocab.z, p.M, p.N, p.vocab.ldz, BM, true)) return 2;
+    tma_out = 1;
+  }
   if (kVocabGrad && tma_out == 0) return 2;
   auto kern = gemm_bf16_pair_kernel<A_MN, B_MN, EPI>;
   static bool attr_set = false;
@@ -1329,6 +1379,7 @@ int launch_pair(const GemmArgs& p, cudaStream_t st) {
     const int per = (num_kb + splits - 1) / splits;
     splits = (num_kb + per - 1) / per;   // no empty split
   }
+  if (EPI == kEpiStoreF32 && p.planes > 1) splits = p.planes;
   const int work = tiles * splits;
   const int pairs = work < max_pairs ? work : max_pairs;
   kern<<<2 * pairs, kThreads, TL::kSmemBytes, st>>>(ta, tb, td, tma_out, p.D, p.M, p.N, p.K, p.ldd, raster_rows(p), splits,
@@ -1587,6 +1638,52 @@ int gemm_bf16_group(const GemmArgs* ps, int count, cudaStream_t st) {
   return max_n <= 256 ? launch_group<128>(ps, count, st) : launch_group<256>(ps, count, st);
 }
 
+namespace {
+__global__ void __launch_bounds__(256) sum_planes_kernel(const float4* __restrict__ in, uint2* __restrict__ out, size_t n4, int planes) {
+  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n4; i += (size_t)gridDim.x * blockDim.x) {
+    float4 s = in[i];
+    for (int p = 1; p < planes; ++p) {
+      const float4 v = in[i + (size_t)p * n4];
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const __nv_bfloat162 a = __floats2bfloat162_rn(s.x, s.y), b = __floats2bfloat162_rn(s.z, s.w);
+    out[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  }
+}
+}  // namespace
+
+int gemm_sum_planes(const float* in, void* out_bf16, size_t n, int planes, cudaStream_t st) {
+  if ((n & 3) || (reinterpret_cast<uintptr_t>(in) & 15) || (reinterpret_cast<uintptr_t>(out_bf16) & 7)) return 6;
+  const size_t n4 = n / 4;
+  const int grid = (int)(n4 / 256 + 1 < 148 * 8 ? n4 / 256 + 1 : 148 * 8);
+  sum_planes_kernel<<<grid, 256, 0, st>>>(reinterpret_cast<const float4*>(in), reinterpret_cast<uint2*>(out_bf16), n4, planes);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+// A product with few output tiles and a long reduction (the gradient of the hidden states behind a vocabulary: 65536 terms)
+// leaves SMs idle, or its last wave of tiles does.  Time of s slices: the waves of tiles, each 1 / s as long (a tile of
+// 256 x 256 runs at about 22 TFLOP/s on a pair of SMs, one of 128 x 256 at half of that), plus the slices' way through
+// memory.  At 509 x 768 x 65536 (6 tiles): 431 us with one
+// slice, 49 + 4 us with twelve and their sum; at 4093 x 2560 x 65536 (160 tiles on 74 pairs) 1169 us against 1024 + 23.
+int gemm_planes(int M, int N, int K, bool pair_allowed) {
+  const bool pair = pair_allowed && M >= 256 && N >= 256 && K >= 512;
+  const int units = pair ? sm_count() / 2 : sm_count();
+  const int bm = pair ? 2 * BM : BM, bn = pair || N > 128 ? 256 : 128;
+  const int tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+  const int num_kb = (K + BK - 1) / BK;
+  const double tile_us = 2.0 * 256 * 256 * K / 22e6;
+  double best = 0.0;
+  int planes = 1;
+  for (int s = 1; s <= 64 && num_kb / s >= 16; ++s) {
+    const int per = (num_kb + s - 1) / s;
+    if ((num_kb + per - 1) / per != s) continue;       // an empty slice
+    const double t = (double)((tiles * (long long)s + units - 1) / units) * per / num_kb * tile_us +
+                     (s > 1 ? 3.0 + ((double)s * 8 + 2) * M * N / 6e6 : 0.0);
+    if (s == 1 || t < best * 0.97) { best = t; planes = s; }
+  }
+  return planes;
+}
+
 bool gemm_decode_eligible(const GemmArgs& p) {
   const bool epi_ok = p.epilogue == kEpiStoreBf16 || p.epilogue == kEpiReluSqBf16 || p.epilogue == kEpiAddBf16;
   // with a short reduction (the up-projection of a low-rank pair) there is no chain of dependent MMAs to split and the
@@ -1617,6 +1714,7 @@ int gemm_bf16(const GemmArgs& p, cudaStream_t st) {
   if (p.epilogue == kEpiProbStats || p.epilogue == kEpiDistillStats || p.epilogue == kEpiProbGrad || p.epilogue == kEpiDistillGrad) {
     const bool stats = p.epilogue == kEpiProbStats || p.epilogue == kEpiDistillStats;
     if (p.layout != kGemmTN || (stats ? (p.ldd & 3) || p.ldd < 4 * ((p.N + 255) / 256) : (p.ldd & 7) || p.ldd < p.N)) return 6;
+    if (stats && p.vocab.z != nullptr && ((reinterpret_cast<uintptr_t>(p.vocab.z) & 15) || (p.vocab.ldz & 3) || p.vocab.ldz < p.N)) return 6;
     if (p.error_flag == nullptr) return 7;
     return launch_vocab(p, st);
   }

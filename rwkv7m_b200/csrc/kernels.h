@@ -174,6 +174,9 @@ struct HeadFix {
   const int* t_ids; const float* t_prob; const float* cols_z;
 };
 int head_prob_fix(const HeadFix& a, cudaStream_t st);
+// The whole gradient from kept logits z (fp32, row pitch ldz a multiple of 4 floats): dense part and listed columns.
+int head_prob_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st);
+int head_distill_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st);
 int head_distill_fix(const HeadFix& a, cudaStream_t st);
 
 // ---- data-parallel optimizer step over symmetric memory -------------------------------
@@ -296,6 +299,7 @@ enum GemmEpilogue {
 struct GemmVocab {
   float c;                 // log2(e) / tau: t = (z - max) c
   float inv_tau, tau;
+  float* z; int ldz;       // statistics: the logits themselves as well, fp32 with a row pitch that is a multiple of 4; or null
   int listed;              // columns per row in `cols` (kEpiDistillStats)
   const int* target;       // [M]: the column whose z goes to target_z (statistics)
   float* target_z;
@@ -329,8 +333,12 @@ struct GemmArgs {
   int* error_flag;     // device int, set non-zero if a bounded wait ran out
   int decode_kernel;   // non-zero: shapes with M <= 64 (layout kGemmTN) take the swap-AB cluster split-K kernel
   GemmVocab vocab;     // the vocabulary epilogues only
+  int planes;          // kEpiStoreF32: > 1 cuts the reduction into that many slices, D is [planes, M, N] (ldd = N)
 };
 int gemm_bf16(const GemmArgs& p, cudaStream_t st);
+// How many slices of the reduction a product with a bf16 result is worth (1 = none), and their sum in the order of the slices.
+int gemm_planes(int M, int N, int K, bool pair_allowed);
+int gemm_sum_planes(const float* in, void* out_bf16, size_t n, int planes, cudaStream_t st);
 // Up to four problems of layout kGemmTN with the bf16 store epilogue (each with its own activation) and the same M in one
 // persistent launch; returns 1 when the set does not qualify (the caller then launches them one by one).
 int gemm_bf16_group(const GemmArgs* ps, int count, cudaStream_t st);

@@ -760,52 +760,169 @@ __global__ void __launch_bounds__(256) head_distill_combine_kernel(const float4*
   }
 }
 
-__global__ void __launch_bounds__(256) head_prob_fix_kernel(HeadFix a) {
-  const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row >= a.rows || a.g0 == nullptr) return;
-  const int id = a.target[row];
-  const float gl = a.g0[row], gh = a.g1 != nullptr ? a.g1[row] : 0.f;
-  if (id < 0 || id >= a.V || gl == 0.f) return;
+// The gradient of one logit of a row, dense part.
+struct HeadCoef {
+  float m, c, l2s1, l2st, A, B, g_ce, g_kd;
+  __device__ __forceinline__ float prob(float z) const {
+    const float l = fmaf(z - m, c, -l2st);
+    return exp2_fast(l) * fmaf(B, l, A);
+  }
+  __device__ __forceinline__ float distill(float z) const {
+    const float d = z - m;
+    return fmaf(g_kd, exp2_fast(fmaf(d, c, -l2st)), g_ce * exp2_fast(fmaf(d, kLog2e, -l2s1)));
+  }
+};
+
+// What flows into a row.  `live` is false where nothing does: such a row gets zeros, whatever its logits.
+template <bool DISTILL>
+__device__ __forceinline__ HeadCoef head_coef(const HeadFix& a, int row, float& gl, bool& live) {
   const float inv_tau = 1.f / a.tau;
   const float4 s = a.stat[row];
-  const float l = (a.target_z[row] - s.x) * (kLog2e * inv_tau) - s.z;
-  const float A = inv_tau * (-gl - (gh != 0.f ? gh * s.w : 0.f)), B = -gh * inv_tau * kLn2;
-  reinterpret_cast<bf16*>(a.dz)[(size_t)row * a.ld + id] = f2bf(fmaf(exp2_fast(l), fmaf(B, l, A), gl * inv_tau));
+  HeadCoef k{s.x, kLog2e * inv_tau, s.y, s.z, 0.f, 0.f, 0.f, 0.f};
+  gl = 0.f;
+  if (DISTILL) {
+    const float2 w = a.weight[row];
+    k.g_ce = a.g0 != nullptr ? a.g0[0] * w.x : 0.f;
+    k.g_kd = a.g1 != nullptr ? a.g1[0] * w.y * a.tau : 0.f;
+    live = k.g_ce != 0.f || k.g_kd != 0.f;
+  } else {
+    const int id = a.target[row];
+    gl = a.g0 != nullptr && id >= 0 && id < a.V ? a.g0[row] : 0.f;
+    const float gh = a.g1 != nullptr ? a.g1[row] : 0.f;
+    k.A = inv_tau * (-gl - (gh != 0.f ? gh * s.w : 0.f));
+    k.B = -gh * inv_tau * kLn2;
+    gl *= inv_tau;
+    live = gl != 0.f || gh != 0.f;
+  }
+  return k;
 }
 
-// One warp per row.  The teacher's ids are sorted, so equal ones are neighbours and the first of a run writes for all.
-__global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= a.rows) return;
-  const float inv_tau = 1.f / a.tau, c = kLog2e * inv_tau;
-  const float4 s = a.stat[row];
-  const float2 w = a.weight[row];
-  const float g_ce = a.g0 != nullptr ? a.g0[0] * w.x : 0.f, g_kd = a.g1 != nullptr ? a.g1[0] * w.y * a.tau : 0.f;
-  const float g_l2 = a.g_l2 != nullptr ? a.g_l2[0] * 1e-4f * s.x : 0.f;
-  const int tgt = w.x != 0.f ? a.target[row] : -1, am = a.argmax[row];
+// The listed columns of a row within [lo, hi), by `n` threads of which this is number t: dense part and one-hot terms.
+__device__ __forceinline__ void prob_listed(const HeadFix& a, const HeadCoef& k, float gl, int row, int lo, int hi) {
+  const int id = a.target[row];
+  if (gl != 0.f && id >= lo && id < hi)
+    reinterpret_cast<bf16*>(a.dz)[(size_t)row * a.ld + id] = f2bf(k.prob(a.target_z[row]) + gl);
+}
+__device__ __forceinline__ void distill_listed(const HeadFix& a, const HeadCoef& k, int row, int lo, int hi, int t, int n) {
+  const int tgt = k.g_ce != 0.f ? a.target[row] : -1, am = a.argmax[row];
+  const float g_l2 = a.g_l2 != nullptr ? a.g_l2[0] * 1e-4f * k.m : 0.f;
+  const int* ids = a.t_ids + (size_t)row * a.K;
   bf16* dz = reinterpret_cast<bf16*>(a.dz) + (size_t)row * a.ld;
-  auto value = [&](int col, float z, float p) {
+  auto put = [&](int col, float z, float p) {
     float d = 0.f;
-    if (g_kd != 0.f) d = g_kd * (exp2_fast((z - s.x) * c - s.z) - p);
-    if (g_ce != 0.f) d += g_ce * (exp2_fast((z - s.x) * kLog2e - s.y) - (col == tgt ? 1.f : 0.f));
+    if (k.g_kd != 0.f) d = k.g_kd * (exp2_fast(fmaf(z - k.m, k.c, -k.l2st)) - p);
+    if (k.g_ce != 0.f) d += k.g_ce * (exp2_fast(fmaf(z - k.m, kLog2e, -k.l2s1)) - (col == tgt ? 1.f : 0.f));
     if (col == am) d += g_l2;
-    return f2bf(d);
+    dz[col] = f2bf(d);
   };
-  bool tgt_done = tgt < 0, am_done = false;
-  for (int j0 = 0; j0 < a.K; j0 += 32) {
-    const int j = j0 + lane;
-    const size_t at = (size_t)row * a.K + j;
-    const int id = j < a.K ? a.t_ids[at] : INT_MAX;
-    if (id != INT_MAX && (j == 0 || a.t_ids[at - 1] != id)) {
-      float p = a.t_prob[at];
-      for (int i = 1; j + i < a.K && a.t_ids[at + i] == id; ++i) p += a.t_prob[at + i];
-      dz[id] = value(id, a.cols_z[at], p);
-    }
-    tgt_done = tgt_done || __any_sync(0xffffffffu, id == tgt);
-    am_done = am_done || __any_sync(0xffffffffu, id == am);
+  auto listed = [&](int col) {                        // the ids are in order
+    int l = 0, h = a.K;
+    while (l < h) { const int mid = (l + h) >> 1; if (ids[mid] < col) l = mid + 1; else h = mid; }
+    return l < a.K && ids[l] == col;
+  };
+  for (int j = t; j < a.K; j += n) {
+    const int id = ids[j];
+    if (id < lo || id >= hi || (j > 0 && ids[j - 1] == id)) continue;      // absent ones are INT_MAX; the first of a run writes
+    float p = 0.f;
+    for (int i = j; i < a.K && ids[i] == id; ++i) p += a.t_prob[(size_t)row * a.K + i];
+    put(id, a.cols_z[(size_t)row * a.K + j], p);
   }
-  if (lane == 0 && !tgt_done) dz[tgt] = value(tgt, a.target_z[row], 0.f);
-  if (lane == 0 && !am_done && am != tgt && am >= 0 && am < a.V) dz[am] = value(am, s.x, 0.f);
+  if (t == 0 && tgt >= lo && tgt < hi && !listed(tgt)) put(tgt, a.target_z[row], 0.f);
+  if (t == n - 1 && am >= lo && am < hi && am != tgt && !listed(am)) put(am, k.m, 0.f);
+}
+
+__global__ void __launch_bounds__(256) head_prob_fix_kernel(HeadFix a) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows) return;
+  float gl;
+  bool live;
+  const HeadCoef k = head_coef<false>(a, row, gl, live);
+  prob_listed(a, k, gl, row, 0, a.V);
+}
+
+// One warp per row.
+__global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  float gl;
+  bool live;
+  const HeadCoef k = head_coef<true>(a, row, gl, live);
+  distill_listed(a, k, row, 0, a.V, threadIdx.x & 31, 32);
+}
+
+// Gradient from kept logits: fp32 in, bf16 out.  A thread takes 8 columns at a time (32 bytes in, 16 out), a CTA `iters`
+// blocks of 4096 columns, the next block's logits in flight while one is written.  Rows from the last to the first, as above.
+template <bool DISTILL>
+__global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const float* __restrict__ z, int64_t ldz, int iters) {
+  constexpr int kBlock = 256 * 8 * 2;
+  const int row = a.rows - 1 - (int)blockIdx.y, tid = threadIdx.x;
+  const int c0 = blockIdx.x * kBlock * iters, c1 = min(a.V, c0 + kBlock * iters);
+  if (c0 >= c1) return;
+  const float* x = z + (size_t)row * ldz;
+  bf16* out = reinterpret_cast<bf16*>(a.dz) + (size_t)row * a.ld;
+  // both pitches cover whole groups of 8 columns, so the last group of a row is read and written whole
+  auto fetch = [&](float4 (&buf)[4], int c) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int col = c + (tid + i * 256) * 8;
+      if (col < c1) {
+        buf[2 * i] = __ldg(reinterpret_cast<const float4*>(x + col));
+        buf[2 * i + 1] = __ldg(reinterpret_cast<const float4*>(x + col + 4));
+      }
+    }
+  };
+  float4 cur[4];
+  fetch(cur, c0);
+  float gl;
+  bool live;
+  const HeadCoef k = head_coef<DISTILL>(a, row, gl, live);
+  const f2 nm = pack2(-k.m, -k.m), cc = pack2(k.c, k.c), nl = pack2(-k.l2st, -k.l2st), A2 = pack2(k.A, k.A), B2 = pack2(k.B, k.B);
+  const f2 c1v = pack2(kLog2e, kLog2e), nl1 = pack2(-k.l2s1, -k.l2s1), gk = pack2(k.g_kd, k.g_kd), gc = pack2(k.g_ce, k.g_ce);
+  auto value2 = [&](float z0, float z1) {
+    const f2 d = add2(pack2(z0, z1), nm), l = fma2(d, cc, nl);
+    float l0, l1, r0, r1;
+    unpack2(l, l0, l1);
+    const f2 q = pack2(exp2_fast(l0), exp2_fast(l1));
+    if (DISTILL) {
+      float e0, e1;
+      unpack2(fma2(d, c1v, nl1), e0, e1);
+      unpack2(fma2(gk, q, mul2(gc, pack2(exp2_fast(e0), exp2_fast(e1)))), r0, r1);
+    } else {
+      unpack2(mul2(q, fma2(B2, l, A2)), r0, r1);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(r0, r1);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  };
+  for (int c = c0; c < c1; c += kBlock) {
+    float4 nxt[4];
+    if (c + kBlock < c1) fetch(nxt, c + kBlock);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int col = c + (tid + i * 256) * 8;
+      if (col < c1) {
+        const float4 p = cur[2 * i], q = cur[2 * i + 1];
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (live) w = make_uint4(value2(p.x, p.y), value2(p.z, p.w), value2(q.x, q.y), value2(q.z, q.w));
+        *reinterpret_cast<uint4*>(out + col) = w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) cur[i] = nxt[i];
+  }
+  __syncthreads();
+  if (DISTILL) distill_listed(a, k, row, c0, c1, tid, 256);
+  else if (tid == 0) prob_listed(a, k, gl, row, c0, c1);
+}
+
+template <bool DISTILL>
+int launch_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st) {
+  if (a.rows <= 0) return 0;
+  if (a.rows > 65535 || (ldz & 7) || (a.ld & 7) || ldz < (a.V + 7) / 8 * 8 || a.ld < (a.V + 7) / 8 * 8) return 6;
+  const int blocks = (a.V + 4095) / 4096;
+  int iters = 1;
+  while (iters < 4 && iters < blocks && (int64_t)a.rows * blocks >= 8ll * iters * 4 * 148) iters *= 2;
+  head_grad_kept_kernel<DISTILL><<<dim3((blocks + iters - 1) / iters, a.rows), 256, 0, st>>>(a, z, ldz, iters);
+  return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
 }  // namespace
@@ -908,6 +1025,14 @@ int head_distill_fix(const HeadFix& a, cudaStream_t st) {
   if (a.rows <= 0) return 0;
   head_distill_fix_kernel<<<(a.rows + 7) / 8, 256, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
+}
+
+int head_prob_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st) {
+  return launch_grad_kept<false>(a, z, ldz, st);
+}
+
+int head_distill_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st) {
+  return launch_grad_kept<true>(a, z, ldz, st);
 }
 
 }  // namespace rk

@@ -25,11 +25,14 @@ def _K():
     return K
 
 
-@pytest.fixture(params=[0, 1], ids=["single", "pair"], autouse=True)
-def _pair_mode(request):
+@pytest.fixture(params=[(0, 8 << 30), (1, 8 << 30), (1, 0)], ids=["single", "pair", "recompute"], autouse=True)
+def _modes(request, monkeypatch):
+    """The single-CTA and the CTA-pair product, logits kept for the backward pass and computed again."""
     kk = _K()
     old = kk.GEMM_PAIR
-    kk.set_gemm_pair(bool(request.param))
+    pair, keep = request.param
+    kk.set_gemm_pair(bool(pair))
+    monkeypatch.setattr(kk, "HEAD_KEEP_BYTES", keep)
     kk.gemm_error_reset(torch.zeros(1, device="cuda"))
     yield
     kk.set_gemm_pair(old)
