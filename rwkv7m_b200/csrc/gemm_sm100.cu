@@ -1189,6 +1189,16 @@ int sm_count() {
   return n;
 }
 
+// A kernel's shared-memory limit is an attribute per device: `done` remembers where it has been raised.
+bool allow_smem(const void* kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev < 64 && done[dev]) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (dev < 64) done[dev] = true;
+  return true;
+}
+
 // Height (in m-tiles) of the raster groups; RWKV7M_B200_GEMM_RASTER overrides the default for experiments.
 int raster_rows(const GemmArgs& p) {
   static int forced = -1;
@@ -1247,11 +1257,8 @@ int launch(const GemmArgs& p, cudaStream_t st) {
   if (kVocabGrad && tma_out == 0) return 2;
   RK_TRACE("maps ok\n");
   auto kern = gemm_bf16_kernel<BN, A_MN, B_MN, EPI>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TL::kSmemBytes) != cudaSuccess) return 3;
-    attr_set = true;
-  }
+  static bool smem_set[64] = {};
+  if (!allow_smem(reinterpret_cast<const void*>(kern), TL::kSmemBytes, smem_set)) return 3;
   const int tiles = ((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   // split-K: a weight gradient with few output tiles and a long reduction (LoRA factors, K = tokens) would leave most
   // SMs idle; the accumulating epilogue lets several CTAs add their partial sums to the same tile
@@ -1324,11 +1331,8 @@ int launch_group(const GemmArgs* ps, int count, cudaStream_t st) {
   for (int i = count; i < kMaxGroup; ++i) { g.tmA[i] = g.tmA[0]; g.tmB[i] = g.tmB[0]; g.tmD[i] = g.tmD[0]; g.pr[i].tile_begin = total; }
   g.total_tiles = total;
   auto kern = gemm_bf16_group_kernel<BN>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TL::kSmemBytes) != cudaSuccess) return 3;
-    attr_set = true;
-  }
+  static bool smem_set[64] = {};
+  if (!allow_smem(reinterpret_cast<const void*>(kern), TL::kSmemBytes, smem_set)) return 3;
   const int grid = total < sm_count() ? total : sm_count();
   kern<<<grid, kThreads, TL::kSmemBytes, st>>>(g, ps[0].error_flag);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
@@ -1358,11 +1362,8 @@ int launch_pair(const GemmArgs& p, cudaStream_t st) {
   }
   if (kVocabGrad && tma_out == 0) return 2;
   auto kern = gemm_bf16_pair_kernel<A_MN, B_MN, EPI>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TL::kSmemBytes) != cudaSuccess) return 3;
-    attr_set = true;
-  }
+  static bool smem_set[64] = {};
+  if (!allow_smem(reinterpret_cast<const void*>(kern), TL::kSmemBytes, smem_set)) return 3;
   const int tiles = ((p.M + 2 * BM - 1) / (2 * BM)) * ((p.N + 255) / 256);
   const int max_pairs = sm_count() / 2;
   // split-K for the accumulating epilogue: a weight gradient has few tiles and a long reduction, and 64 or 256 tiles
@@ -1562,12 +1563,8 @@ int launch_decode(const GemmArgs& p, cudaStream_t st) {
   alignas(64) CUtensorMap tx;
   if (!make_map(&tw, p.B, p.N, p.K, p.ldb, 128)) return 2;
   if (!make_map(&tx, p.A, p.M, p.K, p.lda, 64)) return 2;
-  static bool attr_set = false;
-  if (!attr_set) {
-    if (cudaFuncSetAttribute(gemm_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmemBytes) != cudaSuccess)
-      return 3;
-    attr_set = true;
-  }
+  static bool smem_set[64] = {};
+  if (!allow_smem(reinterpret_cast<const void*>(gemm_decode_kernel), kDecSmemBytes, smem_set)) return 3;
   const int tiles_n = (p.N + 127) / 128;
   const int num_kb = (p.K + BK - 1) / BK;
   // cluster size = K slices per n-tile: a power of two up to 8, enough that about every SM streams part of W

@@ -109,6 +109,37 @@ def test_head_token_logprobs(M, V, C, tau):
         assert lp[1] == 0 and lp[3] == 0
 
 
+@pytest.mark.parametrize("M", [1, 2, 31, 32, 33, 63, 64, 65])
+@pytest.mark.parametrize("V,C", [(63, 64), (64, 8), (65, 72), (9473, 128), (9537, 64), (18944, 256), (50021, 64)])
+def test_few_rows(M, V, C):
+    h, w, ids = _operands(M, V, C, seed=V + M)
+    ids[0] = V - 1
+    ids[M - 1] = 0 if M > 1 else V - 1
+    zd = h.detach().double() @ w.detach().double().T
+    lp, ent = ops.head_token_logprobs(h, w, ids, temperature=0.7)
+    lp2, ent2, _, _ = R.token_logprobs(zd, ids, 0, 0.7)
+    tol = _row_tol(h, w, zd, 0.7)
+    assert (lp.double() - lp2).abs().max() <= tol and (ent.double() - ent2).abs().max() <= tol * 2 * (math.log(V) + 2)
+    g, = torch.autograd.grad(lp.sum(), h)
+    q = torch.softmax(zd / 0.7, -1)
+    dz = -q
+    dz[torch.arange(M), ids] += 1.0
+    dz = dz / 0.7
+    want = dz @ w.detach().double()
+    _check_grads((g, None), (want, None), torch.maximum(dz.abs(), q * (4 * tol)), tol, h, w)
+
+
+def test_a_short_last_chunk():
+    """More rows than one launch of the statistics takes."""
+    h, w, ids = _operands(32768 + 3, 300, 64)
+    with torch.no_grad():
+        lp, ent = ops.head_token_logprobs(h, w, ids)
+        tail = ops.head_token_logprobs(h[-3:], w, ids[-3:])
+    assert torch.equal(lp[-3:], tail[0]) and torch.equal(ent[-3:], tail[1])
+    zd = h.detach().double() @ w.detach().double().T
+    assert (lp.double() - R.token_logprobs(zd, ids)[0]).abs().max() <= _row_tol(h, w, zd, 1.0)
+
+
 def _teacher(M, V, K, seed, ids=None):
     g = torch.Generator().manual_seed(seed)
     t_ids = torch.randint(0, V, (M, K), generator=g).cuda()
