@@ -514,10 +514,11 @@ std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const T
   return out;
 }
 
-// Gradient of g_ce ce_total + g_l2 l2_total + g_kd kd_total with respect to z, into dz (bf16 [M, V], padded row pitch).
+// Gradient of g_ce ce_total + g_l2 l2_total + g_kd kd_total with respect to z, in units of `unit` (fp32 [1], written as well),
+// into dz (bf16 [M, V], padded row pitch).
 void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, const std::vector<Tensor>& saved, const Tensor& t_ids,
                        const Tensor& t_prob, const Tensor& kept, const c10::optional<Tensor>& g_ce, const c10::optional<Tensor>& g_l2,
-                       const c10::optional<Tensor>& g_kd, double tau, Tensor dz, int64_t pair) {
+                       const c10::optional<Tensor>& g_kd, double tau, Tensor dz, Tensor unit, int64_t pair) {
   check_head(H, W, "head_distill_loss");
   c10::cuda::CUDAGuard guard(H.device());
   check_dz(dz, H, W);
@@ -540,6 +541,7 @@ void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, 
   f.cols_z = check_rows(saved[4], H, at::kFloat, {M, K}, "listed logits").data_ptr<float>();
   f.g_l2 = rows_ptr(g_l2, H, 1, "g_l2");
   f.t_ids = t_ids.data_ptr<int>(); f.t_prob = t_prob.data_ptr<float>();
+  f.unit = check_rows(unit, H, at::kFloat, {1}, "unit").data_ptr<float>();
   if (kept.defined()) {
     TORCH_CHECK(rk::head_distill_grad_kept(f, check_kept(kept, H, W), kept.stride(0), stream()) == 0,
                 "head_distill_loss backward: launch failed");
@@ -703,32 +705,40 @@ Tensor aligned_rows(const Tensor& x) {
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
-// dh [M, C] = dz [M, V] W [V, C]
-void hidden_grad(const Tensor& dz, const Tensor& wc, Tensor dh, int64_t pair) {
+// D = scale dz W (layout NN) or scale dz^T h (wgrad); `scale` is a device scalar or undefined.
+void scaled_product(const Tensor& A, const Tensor& B, const Tensor& D, int layout, int epilogue, int64_t pair, const Tensor& scale,
+                    int planes) {
+  rk::GemmArgs p{};
+  p.A = A.data_ptr(); p.B = B.data_ptr(); p.D = D.data_ptr();
+  p.lda = (int)A.stride(0); p.ldb = (int)B.stride(0); p.ldd = (int)D.stride(-2);
+  p.M = (int)(layout == rk::kGemmNN ? A.size(0) : A.size(1)); p.K = (int)(layout == rk::kGemmNN ? A.size(1) : A.size(0));
+  p.N = (int)B.size(1);
+  p.layout = layout; p.epilogue = epilogue; p.pair = (int)pair; p.planes = planes;
+  if (scale.defined()) p.vocab.scale = scale.data_ptr<float>();
+  p.error_flag = gemm_error_flag(A.device()).data_ptr<int>();
+  const int rc = rk::gemm_bf16(p, stream());
+  TORCH_CHECK(rc == 0, "gradient product behind the logits: launch failed with code ", rc);
+}
+
+// dh [M, C] = scale dz [M, V] W [V, C]
+void hidden_grad(const Tensor& dz, const Tensor& wc, Tensor dh, const Tensor& scale, int64_t pair) {
   const int64_t M = dh.size(0), C = dh.size(1);
   const int planes = rk::gemm_planes((int)M, (int)C, (int)dz.size(1), pair != 0);
   if (planes == 1) {
-    gemm(dz, wc, dh, rk::kGemmNN, rk::kEpiStoreBf16, pair, c10::nullopt, 0);
+    scaled_product(dz, wc, dh, rk::kGemmNN, rk::kEpiStoreBf16, pair, scale, 1);
     return;
   }
   Tensor slices = torch::empty({planes, M, C}, dh.options().dtype(at::kFloat));
-  rk::GemmArgs p{};
-  p.A = dz.data_ptr(); p.B = wc.data_ptr(); p.D = slices.data_ptr();
-  p.lda = (int)dz.stride(0); p.ldb = (int)wc.stride(0); p.ldd = (int)C;
-  p.M = (int)M; p.N = (int)C; p.K = (int)dz.size(1);
-  p.layout = rk::kGemmNN; p.epilogue = rk::kEpiStoreF32; p.pair = (int)pair; p.planes = planes;
-  p.error_flag = gemm_error_flag(dz.device()).data_ptr<int>();
-  const int rc = rk::gemm_bf16(p, stream());
-  TORCH_CHECK(rc == 0, "gradient of the hidden states: launch failed with code ", rc);
+  scaled_product(dz, wc, slices, rk::kGemmNN, rk::kEpiStoreF32, pair, scale, planes);
   TORCH_CHECK(rk::gemm_sum_planes(slices.data_ptr<float>(), dh.data_ptr(), (size_t)M * C, planes, stream()) == 0,
               "gradient of the hidden states: sum of the slices failed");
 }
 
-// dh and dW from the gradient of the logits, which `fill(begin, rows, dz)` writes chunk by chunk of rows into one buffer.  A
+// dh and dW from the gradient of the logits in units of `scale`, which `fill(begin, rows, dz)` writes chunk by chunk of rows into one buffer.  A
 // single chunk stores dW in the weight's dtype; several accumulate it in fp32, as does a bound main gradient.
 template <typename F>
 std::pair<Tensor, Tensor> head_backward(const Tensor& h, const Tensor& wc, at::ScalarType w_type, const c10::optional<Tensor>& main,
-                                        int64_t chunk, int64_t pair, bool need_h, bool need_w, F&& fill) {
+                                        int64_t chunk, int64_t pair, bool need_h, bool need_w, const Tensor& scale, F&& fill) {
   const int64_t M = h.size(0), C = h.size(1), V = wc.size(0), step = std::min(chunk, M);
   Tensor buf = torch::empty({step, (V + 7) / 8 * 8}, h.options());
   Tensor dh, dw;
@@ -739,10 +749,10 @@ std::pair<Tensor, Tensor> head_backward(const Tensor& h, const Tensor& wc, at::S
     const int64_t n = std::min(step, M - s);
     Tensor dz = buf.narrow(0, 0, n).narrow(1, 0, V), hs = h.narrow(0, s, n);
     fill(s, n, dz);
-    if (need_h) hidden_grad(dz, wc, dh.narrow(0, s, n), pair);
+    if (need_h) hidden_grad(dz, wc, dh.narrow(0, s, n), scale, pair);
     if (!need_w) continue;
-    if (main.has_value()) gemm(dz, hs, *main, rk::kGemmNT_wgrad, rk::kEpiAccumF32, pair, c10::nullopt, 0);
-    else gemm(dz, hs, dw, rk::kGemmNT_wgrad, direct ? rk::kEpiStoreBf16 : (s == 0 ? rk::kEpiStoreF32 : rk::kEpiAccumF32), pair, c10::nullopt, 0);
+    const int epilogue = main.has_value() ? rk::kEpiAccumF32 : direct ? rk::kEpiStoreBf16 : s == 0 ? rk::kEpiStoreF32 : rk::kEpiAccumF32;
+    scaled_product(dz, hs, main.has_value() ? *main : dw, rk::kGemmNT_wgrad, epilogue, pair, scale, 1);
   }
   if (dw.defined()) dw = dw.to(w_type);
   return {dh, dw};
@@ -762,10 +772,10 @@ void save_head(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, cons
   ctx->saved_data["need_w"] = w.requires_grad();
 }
 template <typename F>
-std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, const Tensor& wc, F&& fill) {
+std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, const Tensor& wc, const Tensor& scale, F&& fill) {
   auto& d = ctx->saved_data;
   auto r = head_backward(h, wc, (at::ScalarType)d["w_type"].toInt(), d["main"].toOptional<Tensor>(), d["chunk"].toInt(), d["pair"].toInt(),
-                         d["need_h"].toBool(), d["need_w"].toBool(), fill);
+                         d["need_h"].toBool(), d["need_w"].toBool(), scale, fill);
   if (r.first.defined()) r.first = r.first.view(d["shape"].toIntVector());
   return r;
 }
@@ -802,7 +812,7 @@ struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
       const c10::optional<Tensor> g_lp = grad_rows(g[0]), g_ent = grad_rows(g[1]);
       const double tau = ctx->saved_data["tau"].toDouble();
       const int64_t pair = ctx->saved_data["pair"].toInt();
-      r = head_backward(ctx, s[0], s[1], [&](int64_t b, int64_t n, const Tensor& dz) {
+      r = head_backward(ctx, s[0], s[1], Tensor(), [&](int64_t b, int64_t n, const Tensor& dz) {
         head_prob_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[5], b, n), part(g_lp, b, n),
                        part(g_ent, b, n), tau, dz, pair);
       });
@@ -852,11 +862,12 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
       const c10::optional<Tensor> g_ce = grad_rows(g[0]), g_l2 = grad_rows(g[2]), g_kd = grad_rows(g[4]);
       const double tau = ctx->saved_data["tau"].toDouble();
       const int64_t pair = ctx->saved_data["pair"].toInt();
-      r = head_backward(ctx, s[0], s[1], [&](int64_t b, int64_t n, const Tensor& dz) {
+      Tensor unit = torch::empty({1}, s[0].options().dtype(at::kFloat));
+      r = head_backward(ctx, s[0], s[1], unit, [&](int64_t b, int64_t n, const Tensor& dz) {
         std::vector<Tensor> rows;
         for (int i = 5; i < 10; ++i) rows.push_back(s[i].narrow(0, b, n));
         head_distill_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), rows, s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[10], b, n), g_ce, g_l2,
-                          g_kd, tau, dz, pair);
+                          g_kd, tau, dz, unit, pair);
       });
     }
     variable_list grads(12);

@@ -37,6 +37,15 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Unit in which a head's logit gradients are written as bf16: the larger of the two losses' upstream gradients.  The one-hot
+// terms that dominate every row then have few digits (1, or a ratio of the two), where g / count would round the same way in
+// every row, by up to 2^-8; the products put the unit back in fp32.
+__device__ __forceinline__ float head_unit(const float* g_ce, const float* g_kd, float tau) {
+  const float ce = g_ce != nullptr ? g_ce[0] : 0.f, kd = g_kd != nullptr ? g_kd[0] * tau : 0.f;
+  const float s = fabsf(ce) >= fabsf(kd) ? ce : kd;
+  return s != 0.f ? s : 1.f;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -213,6 +213,13 @@ __device__ __forceinline__ void* plane_of(void* D, int split, int M, int ldd) {
   return reinterpret_cast<float*>(D) + (size_t)split * M * ldd;
 }
 
+template <int EPI> constexpr bool kScales = EPI == kEpiStoreBf16 || EPI == kEpiStoreF32 || EPI == kEpiAccumF32;
+
+__device__ __forceinline__ void scale_chunk(uint32_t (&v)[32], float sc) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * sc);
+}
+
 // Cross-entropy statistics of one output row over the columns of a tile (kEpiCeStats): the logits are rounded to bf16
 // first, so the numbers equal those of a pass over a stored bf16 logits matrix, which the backward recomputes.
 struct CeRow { float m, s, tl; int am; };
@@ -328,8 +335,9 @@ __device__ __forceinline__ VocabCoef vocab_coef(int row, int M, int N, const Gem
   } else {
     const float2 w = g.weight[row];
     k.b1 = -fmaf(s.x, 1.4426950408889634f, s.y);
-    k.B = g.g0 != nullptr ? g.g0[0] * w.x : 0.f;              // cross-entropy
-    k.A = g.g1 != nullptr ? g.g1[0] * w.y * g.tau : 0.f;      // distillation: tau^2 / tau
+    const float unit = head_unit(g.g0, g.g1, g.tau);
+    k.B = g.g0 != nullptr ? __fdiv_rn(g.g0[0], unit) * w.x : 0.f;             // cross-entropy
+    k.A = g.g1 != nullptr ? __fdiv_rn(g.g1[0] * g.tau, unit) * w.y : 0.f;     // distillation: tau^2 / tau
     k.live = k.A != 0.f || k.B != 0.f;
   }
   return k;
@@ -612,6 +620,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       tc_fence_after();
       const int row = m0 + q * 32 + lane;
       const uint32_t t0 = tmem_base + (uint32_t(q * 32) << 16) + acc * BN;
+      const float sc = kScales<EPI> && vocab.scale != nullptr ? *vocab.scale : 1.f;
       if constexpr (EPI == kEpiCeStats) {
         CeRow st{-INFINITY, 0.f, -INFINITY, 0};
         const int tgt = row < M ? reinterpret_cast<const int*>(aux)[row] : -1;
@@ -643,6 +652,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             vocab_grad_chunk<EPI>(v0, coef, vocab.c);
             vocab_grad_chunk<EPI>(v1, coef, vocab.c);
           }
+          if constexpr (kScales<EPI>) {
+            if (vocab.scale != nullptr) { scale_chunk(v0, sc); scale_chunk(v1, sc); }
+          }
           if (kCanStage && staged) {
             if (n0 + c * 32 < N) {   // same for all 128 threads
               uint8_t* buf = out_stage + obuf * kOutStageBytes;
@@ -664,6 +676,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         uint32_t v[32];
         tmem_ld_32x32(t0, v);
         tmem_ld_wait();
+        if constexpr (kScales<EPI>) {
+          if (vocab.scale != nullptr) scale_chunk(v, sc);
+        }
         store_chunk<EPI>(v, EPI == kEpiStoreF32 ? plane_of(Dptr, work / num_tiles, M, ldd) : Dptr, row, n0, M, N, ldd, atomic, aux,
                          ldaux, act);
       }
@@ -1031,6 +1046,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       tc_fence_after();
       const int row = m0 + q * 32 + lane;
       const uint32_t t0 = tmem_base + (uint32_t(q * 32) << 16) + acc * BN2;
+      const float sc = kScales<EPI> && vocab.scale != nullptr ? *vocab.scale : 1.f;
       if constexpr (EPI == kEpiCeStats) {
         CeRow st{-INFINITY, 0.f, -INFINITY, 0};
         const int tgt = row < M ? reinterpret_cast<const int*>(aux)[row] : -1;
@@ -1060,6 +1076,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if constexpr (kVocabGrad) {
           vocab_grad_chunk<EPI>(v0, coef, vocab.c);
           vocab_grad_chunk<EPI>(v1, coef, vocab.c);
+        }
+        if constexpr (kScales<EPI>) {
+          if (vocab.scale != nullptr) { scale_chunk(v0, sc); scale_chunk(v1, sc); }
         }
         if (kCanStage && staged) {
           if (n0 + c * 32 < N && m0 < M) {   // same for all 128 threads

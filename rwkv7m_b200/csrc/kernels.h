@@ -171,6 +171,7 @@ struct HeadFix {
   const float *g0, *g1;                                 // as in GemmVocab
   // distillation only
   const float2* weight; const int* argmax; const float* g_l2;
+  float* unit;                                          // receives head_unit, the unit of dz
   const int* t_ids; const float* t_prob; const float* cols_z;
 };
 int head_prob_fix(const HeadFix& a, cudaStream_t st);
@@ -293,7 +294,7 @@ enum GemmEpilogue {
   kEpiProbStats = 8,      // no matrix output: per (row, 256-column tile) {max, sum 2^t, sum 2^t t, -} into D as above
   kEpiDistillStats = 9,   // the same with {max, sum at temperature 1, sum at tau, arg-max column}
   kEpiProbGrad = 10,      // D = bf16(q (A + B ln q)), the dense part of the gradient with respect to z
-  kEpiDistillGrad = 11    // D = bf16(a1 q_1 + a q_tau)
+  kEpiDistillGrad = 11    // D = bf16(a1 q_1 + a q_tau), in units of head_unit
 };
 // What the vocabulary epilogues read and write besides D, one entry per row of the product.
 struct GemmVocab {
@@ -309,6 +310,7 @@ struct GemmVocab {
   const float2* weight;    // [M] kEpiDistillGrad: weights of the cross-entropy and of the distillation term
   const float* g0;         // upstream gradients: [M] of the log-probability, or the scalar of the cross-entropy; null = 0
   const float* g1;         //                     [M] of the entropy, or the scalar of the distillation loss; null = 0
+  const float* scale;      // kEpiStoreBf16, kEpiStoreF32, kEpiAccumF32: device scalar that multiplies the product; or null
 };
 // Target of the kEpiScatterAddBf16 epilogue (GEMM -> reduce-scatter over time in one kernel): rows are [B, T] tokens,
 // rank r owns tokens [r*Tl, (r+1)*Tl) of every batch row and receives them in out[r] laid out [B, Tl, N].
@@ -332,7 +334,7 @@ struct GemmArgs {
   int pair;            // non-zero: use the CTA-pair (cta_group::2) kernel when the shape allows
   int* error_flag;     // device int, set non-zero if a bounded wait ran out
   int decode_kernel;   // non-zero: shapes with M <= 64 (layout kGemmTN) take the swap-AB cluster split-K kernel
-  GemmVocab vocab;     // the vocabulary epilogues only
+  GemmVocab vocab;     // the vocabulary epilogues and the products of their gradients
   int planes;          // kEpiStoreF32: > 1 cuts the reduction into that many slices, D is [planes, M, N] (ldd = N)
 };
 int gemm_bf16(const GemmArgs& p, cudaStream_t st);

@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(256) head_distill_combine_kernel(const float4*
 
 // The gradient of one logit of a row, dense part.
 struct HeadCoef {
-  float m, c, l2s1, l2st, A, B, g_ce, g_kd;
+  float m, c, l2s1, l2st, A, B, g_ce, g_kd, unit;
   __device__ __forceinline__ float prob(float z) const {
     const float l = fmaf(z - m, c, -l2st);
     return exp2_fast(l) * fmaf(B, l, A);
@@ -778,12 +778,13 @@ template <bool DISTILL>
 __device__ __forceinline__ HeadCoef head_coef(const HeadFix& a, int row, float& gl, bool& live) {
   const float inv_tau = 1.f / a.tau;
   const float4 s = a.stat[row];
-  HeadCoef k{s.x, kLog2e * inv_tau, s.y, s.z, 0.f, 0.f, 0.f, 0.f};
+  HeadCoef k{s.x, kLog2e * inv_tau, s.y, s.z, 0.f, 0.f, 0.f, 0.f, 1.f};
   gl = 0.f;
   if (DISTILL) {
     const float2 w = a.weight[row];
-    k.g_ce = a.g0 != nullptr ? a.g0[0] * w.x : 0.f;
-    k.g_kd = a.g1 != nullptr ? a.g1[0] * w.y * a.tau : 0.f;
+    k.unit = head_unit(a.g0, a.g1, a.tau);
+    k.g_ce = a.g0 != nullptr ? __fdiv_rn(a.g0[0], k.unit) * w.x : 0.f;
+    k.g_kd = a.g1 != nullptr ? __fdiv_rn(a.g1[0] * a.tau, k.unit) * w.y : 0.f;
     live = k.g_ce != 0.f || k.g_kd != 0.f;
   } else {
     const int id = a.target[row];
@@ -805,7 +806,7 @@ __device__ __forceinline__ void prob_listed(const HeadFix& a, const HeadCoef& k,
 }
 __device__ __forceinline__ void distill_listed(const HeadFix& a, const HeadCoef& k, int row, int lo, int hi, int t, int n) {
   const int tgt = k.g_ce != 0.f ? a.target[row] : -1, am = a.argmax[row];
-  const float g_l2 = a.g_l2 != nullptr ? a.g_l2[0] * 1e-4f * k.m : 0.f;
+  const float g_l2 = a.g_l2 != nullptr ? __fdiv_rn(a.g_l2[0], k.unit) * 1e-4f * k.m : 0.f;
   const int* ids = a.t_ids + (size_t)row * a.K;
   bf16* dz = reinterpret_cast<bf16*>(a.dz) + (size_t)row * a.ld;
   auto put = [&](int col, float z, float p) {
@@ -847,6 +848,7 @@ __global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
   float gl;
   bool live;
   const HeadCoef k = head_coef<true>(a, row, gl, live);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.unit = k.unit;
   distill_listed(a, k, row, 0, a.V, threadIdx.x & 31, 32);
 }
 
@@ -876,6 +878,7 @@ __global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const
   float gl;
   bool live;
   const HeadCoef k = head_coef<DISTILL>(a, row, gl, live);
+  if (DISTILL && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.unit = k.unit;
   const f2 nm = pack2(-k.m, -k.m), cc = pack2(k.c, k.c), nl = pack2(-k.l2st, -k.l2st), A2 = pack2(k.A, k.A), B2 = pack2(k.B, k.B);
   const f2 c1v = pack2(kLog2e, kLog2e), nl1 = pack2(-k.l2s1, -k.l2s1), gk = pack2(k.g_kd, k.g_kd), gc = pack2(k.g_ce, k.g_ce);
   auto value2 = [&](float z0, float z1) {

@@ -187,6 +187,26 @@ def test_head_distill_loss(M, V, C, K, tau):
     _check_grads(got, want, torch.maximum(dz.abs(), mass * (2 * tol + (8 * t_span + 600) * U)), tol, h, w)
 
 
+def test_losses_of_one_kind_and_large_differences():
+    """The gradient of the logits is written in units of the larger upstream gradient: one loss alone, weights far apart, a
+    gradient from L2Wrap alone, none at all."""
+    M, V, C, K = 40, 700, 128, 6
+    h, w, tgt = _operands(M, V, C, seed=3)
+    t_ids, t = _teacher(M, V, K, seed=4, ids=tgt)
+    hd, wd = _double(h, w)
+    for coef in ((1.0, 0.0, 0.0), (0.0, 0.0, 1.0), (0.0, 1.0, 0.0), (1e-12, 0.0, 3e-3), (-2.0, 0.0, 1e-20), (0.0, 0.0, 0.0)):
+        out = ops.head_distill_loss(h, w, tgt, None, t_ids, t, temperature=2.0)
+        got = torch.autograd.grad(out[0] * coef[0] + out[2] * coef[1] + out[4] * coef[2], (h, w))
+        zd = hd @ wd.T
+        ref = R.distill_components(zd, tgt, None, t_ids, t.double(), 2.0)
+        loss = ref[0] * coef[0] + ref[2] * coef[1] + ref[4] * coef[2]
+        dz, = torch.autograd.grad(loss, zd, retain_graph=True)
+        want = torch.autograd.grad(loss, (hd, wd))
+        tol = _row_tol(h, w, zd, 1.0)
+        mass = torch.softmax(zd.detach(), -1) * abs(coef[0]) + (torch.softmax(zd.detach() / 2, -1) + 1e-4) * 2 * abs(coef[2])
+        _check_grads(got, want, torch.maximum(dz.abs(), mass * (4 * tol + 3000 * U)), tol, h, w)
+
+
 def test_several_chunks_and_main_gradient(monkeypatch):
     kk = _K()
     h, w, ids = _operands(150, 1003, 256)
