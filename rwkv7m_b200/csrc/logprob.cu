@@ -111,7 +111,7 @@ __device__ __forceinline__ Stat shfl_xor(const Stat& a, int o) {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
-constexpr int kFewRowsThreads = 512;
+constexpr int kFewRowsThreads = 512, kManyRowsThreads = 128;     // of the forward kernel
 constexpr int kCandidates = 512;
 constexpr int kMaxTop = 64;
 // The fast pass lifts columns below this to it (probability zero either way), so that 0 * t stays finite without a test of
@@ -137,7 +137,7 @@ __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.N
 // One thread's statistics in the fast pass: t = z c - ref (one rounding, whatever the size of the logits), the sums in two
 // halves, the largest logit and the first unit that holds it.
 struct Running {
-  float ref, limit, m;
+  float ref, limit, m, run_m;
   f2 s1, s2;
   int bu;
 };
@@ -171,7 +171,7 @@ __device__ __forceinline__ void take_fast(Running& st, uint4 raw, int u, float c
     st.ref = ref;
     st.limit = cm + slack;
   }
-  if (TOP) { if (cm > st.m) { st.m = cm; st.bu = u; } }
+  if (TOP) { st.run_m = fmaxf(st.run_m, cm); if (cm > st.m) { st.m = cm; st.bu = u; } }
   else st.m = fmaxf(st.m, cm);
   const f2 nr = pack2(-st.ref, -st.ref), cc = pack2(c, c);
 #pragma unroll
@@ -216,20 +216,24 @@ __device__ __forceinline__ void take_exact(Stat& st, int& bu, const float (&v)[R
   }
 }
 
+constexpr int kSub = 8;               // a thread's units in eight runs, each with its own maximum
+
 template <int NT>
 struct TopShared {
-  int sel[NT], nsel, n, ntop, last;
+  int sel[NT], nsel, n, ntop, last, ngrp;
+  int grp[kMaxTop * kSub];            // runs to look at again: thread and number of the run
   uint2 cand[kCandidates];
   uint2 top[kMaxTop];                 // the k largest in order: {value, column}
 };
 
 // The k largest columns of a row, into sh.top in order.  Thread t holds the units t, t + NT, ... and brings the key of its
 // largest logit and the first unit that holds it.  The k-th largest of those keys bounds the k-th largest column from below,
-// and only the threads above the bound are looked at again (k groups of 64 or 256 elements of a 65536-wide row, from L2):
-// their elements above it are the candidates, ranked by counting.  Returns false, having chosen nothing, when the bound is
-// not above `floor_key`.
+// and of the threads above the bound the runs whose maximum reaches it are read again (`run` units of a thread each, from L2
+// or memory): their elements above the bound are the candidates, ranked by counting.  Returns false, having chosen nothing,
+// when the bound is not above `floor_key`.
 template <typename T, int NT>
-__device__ bool row_top(TopShared<NT>& sh, const Row<T>& r, int k, uint32_t key, int bu, uint32_t floor_key) {
+__device__ bool row_top(TopShared<NT>& sh, const float (&runs)[kSub][NT], const Row<T>& r, int run, int k, uint32_t key, int bu,
+                        uint32_t floor_key) {
   constexpr int E = Row<T>::E;
   constexpr int SH = sizeof(T) == 2 ? 16 : 0;     // bf16 orders by the upper half of the key
   const int tid = threadIdx.x;
@@ -246,7 +250,7 @@ __device__ bool row_top(TopShared<NT>& sh, const Row<T>& r, int k, uint32_t key,
     exact = n == k;
   }
   if (bound > 0u && bound <= (floor_key >> SH)) return false;
-  if (tid == 0) { sh.nsel = 0; sh.n = 0; }
+  if (tid == 0) { sh.nsel = 0; sh.n = 0; sh.ngrp = 0; }
   __syncthreads();
   int last = INT_MAX;                             // maxima equal to the bound count up to this unit
   if (!exact && bound > 0u) {
@@ -269,11 +273,17 @@ __device__ bool row_top(TopShared<NT>& sh, const Row<T>& r, int k, uint32_t key,
   }
   if (has && (key > bound || (key == bound && bu <= last))) sh.sel[atomicAdd(&sh.nsel, 1)] = tid;
   __syncthreads();
-  const int nsel = sh.nsel, per = (r.units + NT - 1) / NT;
-  // every element of the chosen threads' units, in any order
+  const int nsel = sh.nsel;
+  for (int i = tid; i < nsel * kSub; i += NT) {
+    const int t = sh.sel[i / kSub];
+    if ((order_key(runs[i % kSub][t]) >> SH) >= bound) sh.grp[atomicAdd(&sh.ngrp, 1)] = t * kSub + i % kSub;
+  }
+  __syncthreads();
+  const int items = sh.ngrp * run;
+  // every element of those runs, in any order
   auto each = [&](auto&& f) {
-    for (int i = tid; i < nsel * per; i += NT) {
-      const int u = sh.sel[i % nsel] + (i / nsel) * NT;
+    for (int i = tid; i < items; i += NT) {
+      const int g = sh.grp[i / run], u = g / kSub + ((g % kSub) * run + i % run) * NT;
       if (u >= r.units) continue;
       float v[E];
       r.load(u, v);
@@ -349,8 +359,8 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // How far a thread of the forward kernel reads ahead (kStages batches of kBatch units), and how many CTAs share an SM.
-template <int NT> struct Ahead { static constexpr int kBatch = 2, kStages = 5, kResident = 1280 / NT; };
-template <> struct Ahead<kFewRowsThreads> { static constexpr int kBatch = 1, kStages = 4, kResident = 2; };
+template <int NT, bool TOP> struct Ahead { static constexpr int kBatch = 2, kStages = TOP ? 4 : 5, kResident = 1280 / NT; };
+template <bool TOP> struct Ahead<kFewRowsThreads, TOP> { static constexpr int kBatch = 1, kStages = TOP ? 3 : 4, kResident = 2; };
 
 // Forward: one CTA per row, its threads over the row's 16-byte units.  A thread copies its own units into its own places of
 // shared memory, several batches ahead, so that no thread waits for another and the copies in flight cost no registers.
@@ -358,10 +368,10 @@ template <> struct Ahead<kFewRowsThreads> { static constexpr int kBatch = 1, kSt
 // leave the rest.  With two register buffers of four units instead of the ring it was 106 us; one CTA going from row to row
 // and reading ahead into the next one 113 us, for the registers that costs.
 template <typename T, bool TOP, int NT>
-__global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(RowStatsArgs a) {
+__global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kernel(RowStatsArgs a) {
   constexpr int E = Row<T>::E;
   constexpr int W = NT / 32;
-  constexpr int kBatch = Ahead<NT>::kBatch, kStages = Ahead<NT>::kStages;
+  constexpr int kBatch = Ahead<NT, TOP>::kBatch, kStages = Ahead<NT, TOP>::kStages;
   const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float c = kLog2e * a.inv_tau;
   if (a.mask != nullptr && a.mask[row] == 0.f) {
@@ -379,6 +389,7 @@ __global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(Row
   using Top = typename std::conditional<TOP, TopShared<NT>, int>::type;
   static_assert(sizeof(Top) <= sizeof(ring), "the alternatives are chosen when the ring has been read");
   Top& sh = *reinterpret_cast<Top*>(&ring[0][0]);
+  __shared__ float runs[TOP ? kSub : 1][NT];          // the maximum of each run of a thread's units
   const Row<T> r(reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld, a.V);
 
   auto block_max = [&](float m) {
@@ -404,7 +415,7 @@ __global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(Row
   const int b0 = r.whole(0) ? 0 : 1, b1 = r.whole(r.units - 1) ? r.units : r.units - 1;
   const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(r.x) & ~uintptr_t(15)) + tid;
   const uint32_t mine = smem_u32(&ring[0][tid]);
-  const int nb = (b1 + kBatch * NT - 1) / (kBatch * NT);
+  const int nb = (r.units + kBatch * NT - 1) / (kBatch * NT), run = (nb + kSub - 1) / kSub;   // batches; batches in a run
   auto issue = [&](int blk, int stage) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -415,7 +426,7 @@ __global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(Row
   };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) issue(j, j);
-  Running st{0.f, -INFINITY, -INFINITY, 0ull, 0ull, tid};
+  Running st{0.f, -INFINITY, -INFINITY, -INFINITY, 0ull, 0ull, tid};
   const float slack = kSlack / c;
   // lifted to the floor, the columns outside of the row have no part
   auto ragged = [&](int u) {
@@ -432,7 +443,7 @@ __global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(Row
     take_fast<T, TOP>(st, raw, u, c, slack);
   };
   if (b0 == 1 && tid == 0) ragged(0);
-  int stage = 0;
+  int stage = 0, in_run = 0, which = 0;
   for (int j = 0; j < nb; ++j) {
     cp_async_wait<kStages - 1>();
     uint4 raw[kBatch];
@@ -445,9 +456,17 @@ __global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(Row
     }
     issue(j + kStages, stage);
     stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (TOP && (++in_run == run || j + 1 == nb)) {
+      runs[which++][tid] = st.run_m;
+      st.run_m = -INFINITY;
+      in_run = 0;
+    }
   }
   cp_async_wait<0>();
-  if (b1 < r.units && r.units - 1 >= b0 && tid == (r.units - 1) % NT) ragged(r.units - 1);
+  if (b1 < r.units && r.units - 1 >= b0 && tid == (r.units - 1) % NT) {
+    ragged(r.units - 1);
+    if (TOP) runs[which - 1][tid] = fmaxf(runs[which - 1][tid], st.run_m);      // it lies in the last batch
+  }
 
   float m = block_max(st.m);
   float x0, x1, y0, y1;
@@ -459,7 +478,7 @@ __global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(Row
   // overflow, -inf times zero, NaN, a row at the floor: the exact pass below
   bool done = m > 0.1f * kFloor && fabsf(tot.x) < INFINITY && fabsf(tot.y) < INFINITY;
   if constexpr (TOP) {
-    if (done) done = row_top<T, NT>(sh, r, a.top_k, order_key(st.m), st.bu, order_key(kFloor * 0.99f));
+    if (done) done = row_top<T, NT>(sh, runs, r, run * kBatch, a.top_k, order_key(st.m), st.bu, order_key(kFloor * 0.99f));
   }
   if (!done) {
     Stat se{-INFINITY, 0.f, 0.f};
@@ -469,7 +488,11 @@ __global__ void __launch_bounds__(NT, Ahead<NT>::kResident) row_stats_kernel(Row
     m = block_max(se.m);
     const float de = se.m == -INFINITY ? 0.f : fmaxf((se.m - m) * c, kMinExponent), fe = exp2_fast(de);
     tot = block_sum2(sm_s, fe * se.s1, fe * fmaf(de, se.s1, se.s2));
-    if constexpr (TOP) row_top<T, NT>(sh, r, a.top_k, order_key(se.m), bu, 0u);
+    if constexpr (TOP) {
+      for (int i = 0; i < kSub; ++i) runs[i][tid] = INFINITY;          // every run of a chosen thread
+      __syncthreads();
+      row_top<T, NT>(sh, runs, r, run * kBatch, a.top_k, order_key(se.m), bu, 0u);
+    }
   }
   if (tid == 0) {
     const float l2s = log2_row(tot.x);                // -inf for a row without a number, NaN for a row with one
@@ -936,13 +959,12 @@ template <typename T, bool TOP, int NT>
 void launch_row_stats_threads(const RowStatsArgs& a, cudaStream_t st) { row_stats_kernel<T, TOP, NT><<<a.rows, NT, 0, st>>>(a); }
 
 // No more rows than SMs: a row is a matter of latency and takes the larger CTA (one bf16 row of 65536: 8.3 us with 512
-// threads, 12.4 with 128).  Many rows: small CTAs, whose starts and ends fall apart (4096 such rows: 90.9 us with 128, 97.6
-// with 256, 117 with 512), but for the alternatives, where a smaller CTA looks at larger groups again (20 of them: 154 us
-// with 128, 139 with 256, 188 with 512).
+// threads, 12.4 with 128).  Many rows: small CTAs, whose starts and ends fall apart (4096 such rows: 90.4 us with 128, 97.6
+// with 256, 117 with 512; with 20 alternatives 119, 133 and 188 us).
 template <typename T, bool TOP>
 int launch_row_stats(const RowStatsArgs& a, cudaStream_t st) {
   if (a.rows <= 148) launch_row_stats_threads<T, TOP, kFewRowsThreads>(a, st);
-  else launch_row_stats_threads<T, TOP, TOP ? kThreads : kThreads / 2>(a, st);
+  else launch_row_stats_threads<T, TOP, kManyRowsThreads>(a, st);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
