@@ -330,25 +330,27 @@ std::vector<Tensor> teacher_prepare(const Tensor& ids, const Tensor& logits, int
   return {oid, p, row};
 }
 
-// -> stats [R, 2] and the scalars sum of mask tau^2 KL, sum of mask
-std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& t_ids, const Tensor& t_prob, const Tensor& t_row,
-                                const c10::optional<Tensor>& mask, double tau) {
+// ids int32 [R, K], t_logits bf16/fp32 [R, K] -> stats [R, 2], the scalars sum of mask tau^2 KL and sum of mask, and the
+// teacher's probabilities [R, K]
+std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& t_ids, const Tensor& t_logits, const c10::optional<Tensor>& mask,
+                                double tau) {
   check_logits(logits, "logits");
   c10::cuda::CUDAGuard guard(logits.device());
   const int64_t R = logits.size(0), V = logits.size(1), K = t_ids.size(1);
+  TORCH_CHECK(K >= 1 && K <= 256, "a teacher gives between 1 and 256 alternatives");
   check_rows(t_ids, logits, at::kInt, {R, K}, "teacher ids");
-  check_rows(t_prob, logits, at::kFloat, {R, K}, "teacher probabilities");
-  check_rows(t_row, logits, at::kFloat, {R, 2}, "teacher rows");
+  TORCH_CHECK(t_logits.scalar_type() == at::kBFloat16 || t_logits.scalar_type() == at::kFloat, "teacher logits must be bf16 or fp32");
+  check_rows(t_logits, logits, t_logits.scalar_type(), {R, K}, "teacher logits");
   auto f32 = logits.options().dtype(at::kFloat);
-  Tensor stats = torch::empty({R, 2}, f32), loss = torch::empty({R}, f32);
+  Tensor stats = torch::empty({R, 2}, f32), loss = torch::empty({R}, f32), t_prob = torch::empty({R, K}, f32);
   Tensor total = torch::empty({}, f32), count = torch::empty({}, f32);
   rk::RowStatsArgs a{};
   a.logits = logits.data_ptr(); a.is_bf16 = logits.scalar_type() == at::kBFloat16; a.ld = logits.stride(0);
   a.rows = (int)R; a.V = (int)V; a.tau = (float)tau; a.inv_tau = (float)(1.0 / tau);
   a.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
   a.mask = rows_ptr(mask, logits, R, "mask");
-  a.K = (int)K; a.t_ids = t_ids.data_ptr<int>(); a.t_prob = t_prob.data_ptr<float>();
-  a.t_row = reinterpret_cast<const float2*>(t_row.data_ptr<float>());
+  a.K = (int)K; a.t_ids = t_ids.data_ptr<int>(); a.t_logits = t_logits.data_ptr(); a.t_bf16 = t_logits.scalar_type() == at::kBFloat16;
+  a.t_prob = t_prob.data_ptr<float>();
   a.row_loss = loss.data_ptr<float>();
   TORCH_CHECK(rk::row_stats(a, stream()) == 0, "distill launch failed");
   rk::RowTotalsArgs t{};
@@ -356,7 +358,7 @@ std::vector<Tensor> distill_fwd(const Tensor& logits, const Tensor& t_ids, const
   t.in[0] = a.row_loss; t.in[1] = a.mask;
   t.out[0] = total.data_ptr<float>(); t.out[1] = count.data_ptr<float>();
   TORCH_CHECK(rk::row_totals(t, stream()) == 0, "distill totals launch failed");
-  return {stats, total, count};
+  return {stats, total, count, t_prob};
 }
 
 // Through the head: z = H W^T with H bf16 [M, C] and W bf16 [V, C]; z is never written.
@@ -647,24 +649,24 @@ variable_list token_logprobs(const Tensor& logits, const Tensor& ids, int64_t to
   return TokenLogprobs::run(logits, ids, top_k, tau, nullptr);
 }
 
-// {ids, p, {sum p ln p, any}} sorted by id
-std::vector<Tensor> teacher_rows(const Tensor& t_ids, const Tensor& t_logits, int64_t V, double tau) {
+// A teacher's ids and logits as int32 and bf16 or fp32 matrices
+std::pair<Tensor, Tensor> teacher_rows(const Tensor& t_ids, const Tensor& t_logits) {
   const int64_t K = t_logits.size(-1), R = t_logits.numel() / K;
   Tensor t = t_logits.reshape({R, K});
   if (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kFloat) t = t.to(at::kFloat);
-  return teacher_prepare(t_ids.reshape({R, K}).to(at::kInt).contiguous(), t.contiguous(), V, tau);
+  return {t_ids.reshape({R, K}).to(at::kInt).contiguous(), t.contiguous()};
 }
 
 struct DistillLoss : torch::autograd::Function<DistillLoss> {
   static variable_list run(const Tensor& logits, const Tensor& t_ids, const Tensor& t_logits, const c10::optional<Tensor>& mask,
                            double tau, AutogradContext* ctx) {
     Tensor z = vocab_rows(logits);
-    const std::vector<Tensor> t = teacher_rows(t_ids, t_logits, z.size(1), tau);
+    const std::pair<Tensor, Tensor> t = teacher_rows(t_ids, t_logits);
     const c10::optional<Tensor> msk = mask_rows(mask);
-    std::vector<Tensor> out = distill_fwd(z, t[0], t[1], t[2], msk, tau);
+    std::vector<Tensor> out = distill_fwd(z, t.first, t.second, msk, tau);
     if (ctx != nullptr) {
       ctx->set_materialize_grads(false);
-      ctx->save_for_backward({z, t[0], t[1], out[0], msk.value_or(Tensor())});
+      ctx->save_for_backward({z, t.first, out[3], out[0], msk.value_or(Tensor())});
       ctx->saved_data["tau"] = tau;
       ctx->saved_data["shape"] = logits.sizes().vec();
       ctx->mark_non_differentiable({out[2]});
@@ -837,7 +839,8 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
                            const Tensor& targets, const c10::optional<Tensor>& mask, const Tensor& t_ids, const Tensor& t_logits,
                            double tau, int64_t chunk, int64_t keep_bytes, int64_t pair, AutogradContext* ctx) {
     Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), tgt = id_rows(targets);
-    const std::vector<Tensor> t = teacher_rows(t_ids, t_logits, wc.size(0), tau);
+    const std::pair<Tensor, Tensor> raw = teacher_rows(t_ids, t_logits);
+    const std::vector<Tensor> t = teacher_prepare(raw.first, raw.second, wc.size(0), tau);
     std::vector<Tensor> out = head_distill_stats(h, wc, tgt, mask_rows(mask), t[0], t[1], t[2], tau, pair,
                                                  ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {

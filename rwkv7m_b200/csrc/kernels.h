@@ -120,7 +120,9 @@ struct RowStatsArgs {
   const int* ids; float* logprob;        // [rows]: log-probability of one column each, 0 for an id outside [0, V)
   int top_k; int* top_ids; float* top_logprobs;   // [rows, top_k], largest first, equal logits by index
   const float* mask;                     // [rows] or null: rows at zero are not read
-  int K; const int* t_ids; const float* t_prob; const float2* t_row; float* row_loss;   // teacher_prepare's output; distillation loss
+  // distillation: the teacher's alternatives [rows, K <= 256] as teacher_prepare takes them; its probabilities (for the
+  // gradient, unwritten where the mask is zero) and the loss of every row
+  int K; const int* t_ids; const void* t_logits; bool t_bf16; float* t_prob; float* row_loss;
 };
 int row_stats(const RowStatsArgs& a, cudaStream_t st);
 // dz_i = 1/tau [ sum_j w_j (i = ids_j) - q_i (sum_j w_j + g_H (H + ln q_i)) ] with w_j = weight_mul g_scale mask w[row, j]

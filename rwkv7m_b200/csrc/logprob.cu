@@ -416,6 +416,10 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
   const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(r.x) & ~uintptr_t(15)) + tid;
   const uint32_t mine = smem_u32(&ring[0][tid]);
   const int nb = (r.units + kBatch * NT - 1) / (kBatch * NT), run = (nb + kSub - 1) / kSub;   // batches; batches in a run
+  // the teacher's alternatives of a distillation: this thread's probabilities and columns
+  constexpr int kMine = (256 + NT - 1) / NT;
+  float t_p[kMine], t_plogp = 0.f;
+  int t_col[kMine];
   auto issue = [&](int blk, int stage) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -426,6 +430,37 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
   };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) issue(j, j);
+  if (a.row_loss != nullptr) {                        // while the first units are on their way
+    float x[kMine], m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int j = tid + i * NT;
+      const size_t at = (size_t)row * a.K + j;
+      t_col[i] = j < a.K ? a.t_ids[at] : -1;
+      x[i] = -INFINITY;
+      if (t_col[i] >= 0 && t_col[i] < a.V)
+        x[i] = a.t_bf16 ? to_float(static_cast<const bf16*>(a.t_logits)[at]) : static_cast<const float*>(a.t_logits)[at];
+      m = fmaxf(m, x[i]);                             // absent: outside of the vocabulary, -inf or NaN
+    }
+    m = block_max(m);
+    float s = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const float t = fmaxf((x[i] - m) * c, kMinExponent);
+      t_p[i] = x[i] > -INFINITY ? exp2_fast(t) : 0.f;
+      s += t_p[i];
+      s2 = fmaf(t_p[i], t, s2);
+    }
+    const float2 t = block_sum2(sm_l, s, s2);
+    const float inv = t.x > 0.f ? 1.f / t.x : 0.f;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      t_p[i] *= inv;
+      if (tid + i * NT < a.K) a.t_prob[(size_t)row * a.K + tid + i * NT] = t_p[i];
+    }
+    t_plogp = t.x > 0.f ? kLn2 * (t.y * inv - log2_row(t.x)) : INFINITY;       // sum p ln p; infinite without alternatives
+    __syncthreads();                                  // sm_m and sm_l are written again below
+  }
   Running st{0.f, -INFINITY, -INFINITY, -INFINITY, 0ull, 0ull, tid};
   const float slack = kSlack / c;
   // lifted to the floor, the columns outside of the row have no part
@@ -509,16 +544,12 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
   if (a.row_loss != nullptr) {
     // distillation: mask tau^2 (sum p ln p - sum p ln q) over the teacher's alternatives
     float acc = 0.f, psum = 0.f;
-    for (int i = tid; i < a.K; i += NT) {
-      const float p = a.t_prob[(size_t)row * a.K + i];
-      const int id = a.t_ids[(size_t)row * a.K + i];
-      if (p > 0.f) { acc += p * ((to_float(r.x[id]) - m) * a.inv_tau); psum += p; }
-    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+      if (t_p[i] > 0.f) { acc += t_p[i] * ((to_float(r.x[t_col[i]]) - m) * a.inv_tau); psum += t_p[i]; }
     const float2 t = block_sum2(sm_l, acc, psum);
-    if (tid == 0) {
-      const float2 tr = a.t_row[row];                 // sum p ln p, and 1 or 0 for a row without alternatives
-      a.row_loss[row] = tr.y > 0.f ? (a.mask != nullptr ? a.mask[row] : 1.f) * a.tau * a.tau * (tr.x - (t.x - t.y * sm_ln)) : 0.f;
-    }
+    if (tid == 0)
+      a.row_loss[row] = t_plogp < INFINITY ? (a.mask != nullptr ? a.mask[row] : 1.f) * a.tau * a.tau * (t_plogp - (t.x - t.y * sm_ln)) : 0.f;
   }
   if constexpr (TOP) {
     __syncthreads();

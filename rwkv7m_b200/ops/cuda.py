@@ -1086,7 +1086,7 @@ def token_logprobs(logits, ids, top_k, tau):
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, mask, tau):
-    _count(3)
+    _count(2)
     return _C.distill_loss(logits, teacher_ids, teacher_logits, mask, tau)
 
 
