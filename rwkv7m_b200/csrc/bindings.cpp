@@ -567,7 +567,9 @@ Tensor vocab_rows(const Tensor& x) {
   Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)});
   return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
-Tensor id_rows(const Tensor& ids) { return ids.reshape({-1}).to(at::kInt).contiguous(); }
+// 64-bit ids are saturated, not wrapped: what lies outside of every vocabulary stays outside
+Tensor as_int(const Tensor& ids) { return (ids.scalar_type() == at::kLong ? ids.clamp(-1, INT_MAX) : ids).to(at::kInt).contiguous(); }
+Tensor id_rows(const Tensor& ids) { return as_int(ids.reshape({-1})); }
 c10::optional<Tensor> mask_rows(const c10::optional<Tensor>& mask) {
   if (!mask.has_value()) return c10::nullopt;
   return mask->reshape({-1}).to(at::kFloat).contiguous();
@@ -654,7 +656,7 @@ std::pair<Tensor, Tensor> teacher_rows(const Tensor& t_ids, const Tensor& t_logi
   const int64_t K = t_logits.size(-1), R = t_logits.numel() / K;
   Tensor t = t_logits.reshape({R, K});
   if (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kFloat) t = t.to(at::kFloat);
-  return {t_ids.reshape({R, K}).to(at::kInt).contiguous(), t.contiguous()};
+  return {as_int(t_ids.reshape({R, K})), t.contiguous()};
 }
 
 struct DistillLoss : torch::autograd::Function<DistillLoss> {
@@ -736,13 +738,15 @@ void hidden_grad(const Tensor& dz, const Tensor& wc, Tensor dh, const Tensor& sc
               "gradient of the hidden states: sum of the slices failed");
 }
 
-// dh and dW from the gradient of the logits in units of `scale`, which `fill(begin, rows, dz)` writes chunk by chunk of rows into one buffer.  A
+// dh and dW from the gradient of the logits in units of `scale`, which `fill(begin, rows, dz)` writes chunk by chunk of rows
+// into one buffer of about `grad_bytes` (65535 rows at most, the limit of a launch).  A
 // single chunk stores dW in the weight's dtype; several accumulate it in fp32, as does a bound main gradient.
 template <typename F>
 std::pair<Tensor, Tensor> head_backward(const Tensor& h, const Tensor& wc, at::ScalarType w_type, const c10::optional<Tensor>& main,
-                                        int64_t chunk, int64_t pair, bool need_h, bool need_w, const Tensor& scale, F&& fill) {
-  const int64_t M = h.size(0), C = h.size(1), V = wc.size(0), step = std::min(chunk, M);
-  Tensor buf = torch::empty({step, (V + 7) / 8 * 8}, h.options());
+                                        int64_t grad_bytes, int64_t pair, bool need_h, bool need_w, const Tensor& scale, F&& fill) {
+  const int64_t M = h.size(0), C = h.size(1), V = wc.size(0), pitch = (V + 7) / 8 * 8;
+  const int64_t fits = std::max<int64_t>(256, grad_bytes / (2 * pitch) / 256 * 256), step = std::min({fits, M, (int64_t)65280});
+  Tensor buf = torch::empty({step, pitch}, h.options());
   Tensor dh, dw;
   if (need_h) dh = torch::empty({M, C}, h.options());
   const bool direct = step == M && w_type == at::kBFloat16;
@@ -761,14 +765,14 @@ std::pair<Tensor, Tensor> head_backward(const Tensor& h, const Tensor& wc, at::S
 }
 
 // What every head node saves besides its own tensors.
-void save_head(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const c10::optional<Tensor>& main, double tau, int64_t chunk,
+void save_head(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const c10::optional<Tensor>& main, double tau, int64_t grad_bytes,
                int64_t pair) {
   ctx->set_materialize_grads(false);
   ctx->saved_data["tau"] = tau;
   ctx->saved_data["shape"] = hidden.sizes().vec();
   ctx->saved_data["w_type"] = (int64_t)w.scalar_type();
   ctx->saved_data["main"] = main;             // written in backward, so not a saved variable
-  ctx->saved_data["chunk"] = chunk;
+  ctx->saved_data["grad_bytes"] = grad_bytes;
   ctx->saved_data["pair"] = pair;
   ctx->saved_data["need_h"] = hidden.requires_grad();
   ctx->saved_data["need_w"] = w.requires_grad();
@@ -776,7 +780,7 @@ void save_head(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, cons
 template <typename F>
 std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, const Tensor& wc, const Tensor& scale, F&& fill) {
   auto& d = ctx->saved_data;
-  auto r = head_backward(h, wc, (at::ScalarType)d["w_type"].toInt(), d["main"].toOptional<Tensor>(), d["chunk"].toInt(), d["pair"].toInt(),
+  auto r = head_backward(h, wc, (at::ScalarType)d["w_type"].toInt(), d["main"].toOptional<Tensor>(), d["grad_bytes"].toInt(), d["pair"].toInt(),
                          d["need_h"].toBool(), d["need_w"].toBool(), scale, fill);
   if (r.first.defined()) r.first = r.first.view(d["shape"].toIntVector());
   return r;
@@ -791,18 +795,18 @@ c10::optional<Tensor> part(const c10::optional<Tensor>& t, int64_t s, int64_t n)
 // `wc` is the bf16 weight that the products read (w itself, or the copy kept beside it), `main` a bound fp32 main gradient.
 struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
   static variable_list run(const Tensor& hidden, const Tensor& w, const Tensor& wc_in, const c10::optional<Tensor>& main,
-                           const Tensor& ids, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair, AutogradContext* ctx) {
+                           const Tensor& ids, double tau, int64_t grad_bytes, int64_t keep_bytes, int64_t pair, AutogradContext* ctx) {
     Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), idr = id_rows(ids);
     std::vector<Tensor> out = head_prob_stats(h, wc, idr, tau, pair, ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {
-      save_head(ctx, hidden, w, main, tau, chunk, pair);
+      save_head(ctx, hidden, w, main, tau, grad_bytes, pair);
       ctx->save_for_backward({h, wc, idr, out[2], out[3], out[4]});
     }
     return {out[0].view(ids.sizes()), out[1].view(ids.sizes())};
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const Tensor& wc,
-                               const c10::optional<Tensor>& main, const Tensor& ids, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
-    return run(hidden, w, wc, main, ids, tau, chunk, keep_bytes, pair, ctx);
+                               const c10::optional<Tensor>& main, const Tensor& ids, double tau, int64_t grad_bytes, int64_t keep_bytes, int64_t pair) {
+    return run(hidden, w, wc, main, ids, tau, grad_bytes, keep_bytes, pair, ctx);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     if (!g[0].defined() && !g[1].defined()) return variable_list(9);
@@ -827,24 +831,24 @@ struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
 };
 
 variable_list head_token_logprobs(const Tensor& hidden, const Tensor& w, const Tensor& wc, const c10::optional<Tensor>& main,
-                                  const Tensor& ids, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
+                                  const Tensor& ids, double tau, int64_t grad_bytes, int64_t keep_bytes, int64_t pair) {
   c10::cuda::CUDAGuard guard(hidden.device());
-  if (wants_grad(hidden) || wants_grad(w)) return HeadTokenLogprobs::apply(hidden, w, wc, main, ids, tau, chunk, keep_bytes, pair);
+  if (wants_grad(hidden) || wants_grad(w)) return HeadTokenLogprobs::apply(hidden, w, wc, main, ids, tau, grad_bytes, keep_bytes, pair);
   at::NoGradGuard no_grad;
-  return HeadTokenLogprobs::run(hidden, w, wc, main, ids, tau, chunk, keep_bytes, pair, nullptr);
+  return HeadTokenLogprobs::run(hidden, w, wc, main, ids, tau, grad_bytes, keep_bytes, pair, nullptr);
 }
 
 struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
   static variable_list run(const Tensor& hidden, const Tensor& w, const Tensor& wc_in, const c10::optional<Tensor>& main,
                            const Tensor& targets, const c10::optional<Tensor>& mask, const Tensor& t_ids, const Tensor& t_logits,
-                           double tau, int64_t chunk, int64_t keep_bytes, int64_t pair, AutogradContext* ctx) {
+                           double tau, int64_t grad_bytes, int64_t keep_bytes, int64_t pair, AutogradContext* ctx) {
     Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), tgt = id_rows(targets);
     const std::pair<Tensor, Tensor> raw = teacher_rows(t_ids, t_logits);
     const std::vector<Tensor> t = teacher_prepare(raw.first, raw.second, wc.size(0), tau);
     std::vector<Tensor> out = head_distill_stats(h, wc, tgt, mask_rows(mask), t[0], t[1], t[2], tau, pair,
                                                  ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {
-      save_head(ctx, hidden, w, main, tau, chunk, pair);
+      save_head(ctx, hidden, w, main, tau, grad_bytes, pair);
       ctx->save_for_backward({h, wc, tgt, t[0], t[1], out[6], out[7], out[8], out[9], out[10], out[11]});
       ctx->mark_non_differentiable({out[1], out[3], out[5]});
     }
@@ -852,8 +856,8 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, const Tensor& wc,
                                const c10::optional<Tensor>& main, const Tensor& targets, const c10::optional<Tensor>& mask,
-                               const Tensor& t_ids, const Tensor& t_logits, double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
-    return run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, keep_bytes, pair, ctx);
+                               const Tensor& t_ids, const Tensor& t_logits, double tau, int64_t grad_bytes, int64_t keep_bytes, int64_t pair) {
+    return run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, grad_bytes, keep_bytes, pair, ctx);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     if (!g[0].defined() && !g[2].defined() && !g[4].defined()) return variable_list(12);
@@ -882,12 +886,12 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
 
 variable_list head_distill_loss(const Tensor& hidden, const Tensor& w, const Tensor& wc, const c10::optional<Tensor>& main,
                                 const Tensor& targets, const c10::optional<Tensor>& mask, const Tensor& t_ids, const Tensor& t_logits,
-                                double tau, int64_t chunk, int64_t keep_bytes, int64_t pair) {
+                                double tau, int64_t grad_bytes, int64_t keep_bytes, int64_t pair) {
   c10::cuda::CUDAGuard guard(hidden.device());
   if (wants_grad(hidden) || wants_grad(w))
-    return HeadDistillLoss::apply(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, keep_bytes, pair);
+    return HeadDistillLoss::apply(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, grad_bytes, keep_bytes, pair);
   at::NoGradGuard no_grad;
-  return HeadDistillLoss::run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, chunk, keep_bytes, pair, nullptr);
+  return HeadDistillLoss::run(hidden, w, wc, main, targets, mask, t_ids, t_logits, tau, grad_bytes, keep_bytes, pair, nullptr);
 }
 
 // Up to four y_i = act_i(A_i B_i^T) with the same number of rows in one launch (bf16 in, bf16 out).  Returns false, having

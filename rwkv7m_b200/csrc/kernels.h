@@ -119,9 +119,9 @@ struct RowStatsArgs {
   float* entropy;                        // [rows]
   const int* ids; float* logprob;        // [rows]: log-probability of one column each, 0 for an id outside [0, V)
   int top_k; int* top_ids; float* top_logprobs;   // [rows, top_k], largest first, equal logits by index
-  const float* mask;                     // [rows] or null: rows at zero are not read
-  // distillation: the teacher's alternatives [rows, K <= 256] as teacher_prepare takes them; its probabilities (for the
+  // distillation (not together with alternatives): rows whose mask is zero are not read; the teacher's alternatives [rows, K <= 256] as teacher_prepare takes them; its probabilities (for the
   // gradient, unwritten where the mask is zero) and the loss of every row
+  const float* mask;                     // [rows] or null
   int K; const int* t_ids; const void* t_logits; bool t_bf16; float* t_prob; float* row_loss;
 };
 int row_stats(const RowStatsArgs& a, cudaStream_t st);

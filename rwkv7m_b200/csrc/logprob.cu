@@ -240,7 +240,7 @@ __device__ bool row_top(TopShared<NT>& sh, const float (&runs)[kSub][NT], const 
   const bool has = tid < r.units;
   key >>= SH;
   if (!has) key = 0u;                             // a thread without units has none
-  // a bound that at least k thread maxima reach, the largest one or one that exactly k reach
+  // the largest bound that at least k thread maxima reach
   uint32_t bound = 0u;
   bool exact = false;
   for (int b = 31 - SH; b >= 0 && !exact; --b) {
@@ -248,6 +248,15 @@ __device__ bool row_top(TopShared<NT>& sh, const float (&runs)[kSub][NT], const 
     const int n = __syncthreads_count(key >= t);
     if (n >= k) bound = t;
     exact = n == k;
+  }
+  if (exact) {
+    // exactly the k largest, found before the last bit: the smallest of them is the tightest bound that they share
+    const uint32_t mn = __reduce_min_sync(0xffffffffu, key >= bound ? key : 0xffffffffu);
+    if ((tid & 31) == 0) sh.sel[tid >> 5] = (int)mn;
+    __syncthreads();
+    bound = 0xffffffffu;
+    for (int w = 0; w < NT / 32; ++w) bound = min(bound, (uint32_t)sh.sel[w]);
+    __syncthreads();
   }
   if (bound > 0u && bound <= (floor_key >> SH)) return false;
   if (tid == 0) { sh.nsel = 0; sh.n = 0; sh.ngrp = 0; }
@@ -364,28 +373,31 @@ template <bool TOP> struct Ahead<kFewRowsThreads, TOP> { static constexpr int kB
 
 // Forward: one CTA per row, its threads over the row's 16-byte units.  A thread copies its own units into its own places of
 // shared memory, several batches ahead, so that no thread waits for another and the copies in flight cost no registers.
-// Bound by memory: 4096 x 65536 bf16 take 90.9 us, 5.9 TB/s (a plain read of them 75.6 us), of which the row's start and end
-// leave the rest.  With two register buffers of four units instead of the ring it was 106 us; one CTA going from row to row
-// and reading ahead into the next one 113 us, for the registers that costs.
-template <typename T, bool TOP, int NT>
-__global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kernel(RowStatsArgs a) {
+// Bound by memory: 4096 x 65536 bf16 take 85.7 us, 6.27 TB/s (as fp32, 4096 x 32768, 82.4 us; a plain read 75.6 us).  With two
+// register buffers of four units instead of the ring it was 106 us; one CTA going from row to row and reading ahead into the
+// next one 113 us, for the registers that costs.
+// kDo says what else a row is for: nothing, its alternatives, or its distillation loss.
+enum RowDo { kOnlyStats, kAlternatives, kDistill };
+template <typename T, RowDo kDo, int NT>
+__global__ void __launch_bounds__(NT, Ahead<NT, kDo == kAlternatives>::kResident) row_stats_kernel(RowStatsArgs a) {
+  constexpr bool TOP = kDo == kAlternatives;
   constexpr int E = Row<T>::E;
   constexpr int W = NT / 32;
   constexpr int kBatch = Ahead<NT, TOP>::kBatch, kStages = Ahead<NT, TOP>::kStages;
   const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float c = kLog2e * a.inv_tau;
-  if (a.mask != nullptr && a.mask[row] == 0.f) {
+  if (kDo == kDistill && a.mask != nullptr && a.mask[row] == 0.f) {
     // a row that does not count is not read: whatever it holds stays out of the sums
     if (tid == 0) {
       a.stats[row] = make_float2(0.f, 0.f);
-      if (a.row_loss != nullptr) a.row_loss[row] = 0.f;
+      a.row_loss[row] = 0.f;
     }
     return;
   }
   __shared__ float sm_m[W];
   __shared__ float2 sm_s[W], sm_l[W];
   __shared__ float sm_ln;
-  __shared__ __align__(16) uint4 ring[kStages * kBatch][NT];
+  __shared__ __align__(128) uint4 ring[kStages * kBatch][NT];     // on whole lines: 48 bytes off cost 6 us of 90
   using Top = typename std::conditional<TOP, TopShared<NT>, int>::type;
   static_assert(sizeof(Top) <= sizeof(ring), "the alternatives are chosen when the ring has been read");
   Top& sh = *reinterpret_cast<Top*>(&ring[0][0]);
@@ -430,7 +442,15 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
   };
 #pragma unroll
   for (int j = 0; j < kStages; ++j) issue(j, j);
-  if (a.row_loss != nullptr) {                        // while the first units are on their way
+  // what the row's end needs of single columns is asked for now: there, two loads in a row would be the CTA's whole work
+  int id = -1;
+  float z_id = 0.f;
+  if (tid == 0 && a.logprob != nullptr) {
+    id = a.ids[row];
+    if (id >= 0 && id < a.V) z_id = to_float(r.x[id]);
+  }
+  float z_t[kMine];
+  if constexpr (kDo == kDistill) {                    // while the first units are on their way
     float x[kMine], m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
@@ -456,6 +476,7 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       t_p[i] *= inv;
+      z_t[i] = t_p[i] > 0.f ? to_float(r.x[t_col[i]]) : 0.f;
       if (tid + i * NT < a.K) a.t_prob[(size_t)row * a.K + tid + i * NT] = t_p[i];
     }
     t_plogp = t.x > 0.f ? kLn2 * (t.y * inv - log2_row(t.x)) : INFINITY;       // sum p ln p; infinite without alternatives
@@ -478,8 +499,9 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
     take_fast<T, TOP>(st, raw, u, c, slack);
   };
   if (b0 == 1 && tid == 0) ragged(0);
-  int stage = 0, in_run = 0, which = 0;
-  for (int j = 0; j < nb; ++j) {
+  int stage = 0, in_run = 0, which = 0, j = 0;
+  // one batch; `inside`: it and the one requested in its place are whole units for every thread
+  auto step = [&](auto inside) {
     cp_async_wait<kStages - 1>();
     uint4 raw[kBatch];
 #pragma unroll
@@ -487,16 +509,28 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int u = (j * kBatch + i) * NT + tid;
-      if (u >= b0 && u < b1) take_fast<T, TOP>(st, raw[i], u, c, slack);
+      if (inside || (u >= b0 && u < b1)) take_fast<T, TOP>(st, raw[i], u, c, slack);
     }
-    issue(j + kStages, stage);
+    if (inside) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        cp_async16(mine + (uint32_t)((stage * kBatch + i) * NT * 16), base + ((j + kStages) * kBatch + i) * NT);
+      cp_async_commit();
+    } else {
+      issue(j + kStages, stage);
+    }
     stage = stage + 1 == kStages ? 0 : stage + 1;
-    if (TOP && (++in_run == run || j + 1 == nb)) {
+    ++j;
+    if (TOP && (++in_run == run || j == nb)) {
       runs[which++][tid] = st.run_m;
       st.run_m = -INFINITY;
       in_run = 0;
     }
-  }
+  };
+  const int inner = b1 / (kBatch * NT) - kStages;     // batches with kStages full ones behind them
+  if (b0 == 1 && inner > 0) step(std::false_type());
+  while (j < inner) step(std::true_type());
+  while (j < nb) step(std::false_type());
   cp_async_wait<0>();
   if (b1 < r.units && r.units - 1 >= b0 && tid == (r.units - 1) % NT) {
     ragged(r.units - 1);
@@ -534,19 +568,16 @@ __global__ void __launch_bounds__(NT, Ahead<NT, TOP>::kResident) row_stats_kerne
     const float ln_s = tot.x > 0.f ? l2s * kLn2 : __int_as_float(0x7fffffff);
     a.stats[row] = make_float2(m, l2s);
     if (a.entropy != nullptr) a.entropy[row] = tot.x > 0.f ? ln_s - kLn2 * (tot.y / tot.x) : ln_s;
-    if (a.logprob != nullptr) {
-      const int id = a.ids[row];
-      // an id outside the vocabulary is no token: nothing to score
-      a.logprob[row] = (id >= 0 && id < a.V) ? (to_float(r.x[id]) - m) * a.inv_tau - ln_s : 0.f;
-    }
+    // an id outside the vocabulary is no token: nothing to score
+    if (a.logprob != nullptr) a.logprob[row] = id >= 0 && id < a.V ? (z_id - m) * a.inv_tau - ln_s : 0.f;
     sm_ln = ln_s;
   }
-  if (a.row_loss != nullptr) {
-    // distillation: mask tau^2 (sum p ln p - sum p ln q) over the teacher's alternatives
+  if constexpr (kDo == kDistill) {
+    // mask tau^2 (sum p ln p - sum p ln q) over the teacher's alternatives
     float acc = 0.f, psum = 0.f;
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
-      if (t_p[i] > 0.f) { acc += t_p[i] * ((to_float(r.x[t_col[i]]) - m) * a.inv_tau); psum += t_p[i]; }
+      if (t_p[i] > 0.f) { acc += t_p[i] * ((z_t[i] - m) * a.inv_tau); psum += t_p[i]; }
     const float2 t = block_sum2(sm_l, acc, psum);
     if (tid == 0)
       a.row_loss[row] = t_plogp < INFINITY ? (a.mask != nullptr ? a.mask[row] : 1.f) * a.tau * a.tau * (t_plogp - (t.x - t.y * sm_ln)) : 0.f;
@@ -986,16 +1017,13 @@ int launch_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t
 
 namespace {
 
-template <typename T, bool TOP, int NT>
-void launch_row_stats_threads(const RowStatsArgs& a, cudaStream_t st) { row_stats_kernel<T, TOP, NT><<<a.rows, NT, 0, st>>>(a); }
-
-// No more rows than SMs: a row is a matter of latency and takes the larger CTA (one bf16 row of 65536: 8.3 us with 512
-// threads, 12.4 with 128).  Many rows: small CTAs, whose starts and ends fall apart (4096 such rows: 90.4 us with 128, 97.6
-// with 256, 117 with 512; with 20 alternatives 119, 133 and 188 us).
-template <typename T, bool TOP>
+// No more rows than SMs: a row is a matter of latency and takes the larger CTA (one bf16 row of 65536: 7.1 us with 512
+// threads, 12.4 with 128).  Many rows: small CTAs, whose starts and ends fall apart (4096 such rows: 90 us with 128, 98 with
+// 256, 117 with 512; with 20 alternatives 119, 133 and 188 us, at the same state of the kernel).
+template <typename T, RowDo kDo>
 int launch_row_stats(const RowStatsArgs& a, cudaStream_t st) {
-  if (a.rows <= 148) launch_row_stats_threads<T, TOP, kFewRowsThreads>(a, st);
-  else launch_row_stats_threads<T, TOP, kManyRowsThreads>(a, st);
+  if (a.rows <= 148) row_stats_kernel<T, kDo, kFewRowsThreads><<<a.rows, kFewRowsThreads, 0, st>>>(a);
+  else row_stats_kernel<T, kDo, kManyRowsThreads><<<a.rows, kManyRowsThreads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
@@ -1003,8 +1031,9 @@ int launch_row_stats(const RowStatsArgs& a, cudaStream_t st) {
 
 int row_stats(const RowStatsArgs& a, cudaStream_t st) {
   if (a.rows <= 0) return 0;
-  if (a.top_k > 0) return a.is_bf16 ? launch_row_stats<bf16, true>(a, st) : launch_row_stats<float, true>(a, st);
-  return a.is_bf16 ? launch_row_stats<bf16, false>(a, st) : launch_row_stats<float, false>(a, st);
+  if (a.top_k > 0) return a.is_bf16 ? launch_row_stats<bf16, kAlternatives>(a, st) : launch_row_stats<float, kAlternatives>(a, st);
+  if (a.row_loss != nullptr) return a.is_bf16 ? launch_row_stats<bf16, kDistill>(a, st) : launch_row_stats<float, kDistill>(a, st);
+  return a.is_bf16 ? launch_row_stats<bf16, kOnlyStats>(a, st) : launch_row_stats<float, kOnlyStats>(a, st);
 }
 
 int row_grad(const RowGradArgs& a, cudaStream_t st) {

@@ -373,8 +373,9 @@ def _check_head(name, hidden, head_w):
 
 def head_token_logprobs(hidden, head_w, ids, *, temperature=1.0):
     """``(logprob, entropy)`` of :func:`token_logprobs` for the logits ``hidden`` [..., C] @ ``head_w`` [V, C].T, which are not
-    kept: forward reduces them where the product leaves them, in fp32, backward recomputes them.  ``hidden`` is what the head
-    reads (behind the final layer norm).  Differentiable in both."""
+    returned: forward reduces them where the product leaves them, in fp32.  ``hidden`` is what the head reads (behind the
+    final layer norm) and has to be finite at every position, scored or not.  Differentiable in both; for the backward pass
+    the GPU keeps the fp32 logits up to ``RWKV7M_B200_HEAD_KEEP_BYTES`` (8 GiB) and computes larger ones again."""
     name = "head_token_logprobs"
     _check_head(name, hidden, head_w)
     _check_ids(name, ids, hidden.shape[:-1], hidden.device)
@@ -386,12 +387,13 @@ def head_token_logprobs(hidden, head_w, ids, *, temperature=1.0):
 
 def head_distill_loss(hidden, head_w, targets, mask, teacher_ids, teacher_logits, *, temperature=1.0):
     """The loss pieces of :func:`head_loss` and of :func:`distill_loss` in one pass over the head: ``(ce_total, ce_count,
-    l2_total, l2_count, kd_total, kd_count)`` for the logits ``hidden`` [..., C] @ ``head_w`` [V, C].T, which are not kept.
+    l2_total, l2_count, kd_total, kd_count)`` for the logits ``hidden`` [..., C] @ ``head_w`` [V, C].T, which are not returned
+    (and kept for the backward pass as in :func:`head_token_logprobs`).
 
     Cross-entropy (at temperature 1) runs over positions with mask != 0 and a target inside the vocabulary, L2Wrap over
     every position, distillation (at ``temperature``) over positions with mask != 0 and a teacher that is not empty;
-    ``kd_count`` is the sum of the mask.  ``hidden`` is what the head reads (behind the final layer norm).  Differentiable
-    in ``hidden`` and ``head_w``."""
+    ``kd_count`` is the sum of the mask.  ``hidden`` is what the head reads (behind the final layer norm) and has to be finite
+    at every position, counted or not.  Differentiable in ``hidden`` and ``head_w``."""
     name = "head_distill_loss"
     _check_head(name, hidden, head_w)
     lead = hidden.shape[:-1]

@@ -1090,8 +1090,9 @@ def distill_loss(logits, teacher_ids, teacher_logits, mask, tau):
     return _C.distill_loss(logits, teacher_ids, teacher_logits, mask, tau)
 
 
-# Rows of the [rows, V] bf16 gradient of the logits that a backward pass through the head holds at a time.
-HEAD_GRAD_ROWS = 16384
+# Size of the [rows, V] bf16 gradient of the logits that a backward pass through the head holds at a time (16384 rows of a
+# 65536-token vocabulary).
+HEAD_GRAD_BYTES = 2 << 30
 # A forward pass through the head keeps its fp32 logits for the backward pass while they fit into this many bytes; beyond, they
 # are computed a second time.
 HEAD_KEEP_BYTES = int(os.environ.get("RWKV7M_B200_HEAD_KEEP_BYTES", str(8 << 30)))
@@ -1119,7 +1120,7 @@ def head_token_logprobs(hidden, head_w, ids, tau):
     products."""
     if _head_kernels_apply(hidden):
         _count(2)
-        return tuple(_C.head_token_logprobs(*_head_operands(hidden, head_w), ids, tau, HEAD_GRAD_ROWS, HEAD_KEEP_BYTES,
+        return tuple(_C.head_token_logprobs(*_head_operands(hidden, head_w), ids, tau, HEAD_GRAD_BYTES, HEAD_KEEP_BYTES,
                                                     int(GEMM_PAIR)))
     return tuple(token_logprobs(_head_logits(hidden, head_w), ids, 0, tau)[:2])
 
@@ -1130,7 +1131,7 @@ def head_distill_loss(hidden, head_w, targets, mask, teacher_ids, teacher_logits
     if _head_kernels_apply(hidden):
         _count(4)
         return tuple(_C.head_distill_loss(*_head_operands(hidden, head_w), targets, mask, teacher_ids, teacher_logits, tau,
-                                          HEAD_GRAD_ROWS, HEAD_KEEP_BYTES, int(GEMM_PAIR)))
+                                          HEAD_GRAD_BYTES, HEAD_KEEP_BYTES, int(GEMM_PAIR)))
     logits = _head_logits(hidden, head_w)
     kd = distill_loss(logits, teacher_ids, teacher_logits, mask, tau)
     return R.distill_components(logits, targets, mask, teacher_ids, teacher_logits, tau, kd=kd)

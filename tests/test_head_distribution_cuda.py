@@ -216,8 +216,10 @@ def test_several_chunks_and_main_gradient(monkeypatch):
         lp, ent = ops.head_token_logprobs(h, weight, ids)
         return torch.autograd.grad((lp, ent), (h, weight), (up, up), allow_unused=True)
 
+    h, w, ids = _operands(600, 1003, 256)
+    up = torch.ones(600, device="cuda") / 600
     one = grads(w)
-    monkeypatch.setattr(kk, "HEAD_GRAD_ROWS", 64)
+    monkeypatch.setattr(kk, "HEAD_GRAD_BYTES", 1)         # 256 rows at a time
     many = grads(w)
     # the same roundings of dz; dW is added up in another order in fp32 and rounded once either way
     assert torch.equal(one[0], many[0])

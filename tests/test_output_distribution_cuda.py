@@ -319,6 +319,61 @@ def test_same_result_on_every_run():
         assert all(torch.equal(a, b) for a, b in zip(first, again))
 
 
+def test_wide_ids_do_not_wrap():
+    z = _logits(3, 100, "fp32")
+    wide = torch.tensor([2 ** 32 + 7, -2 ** 32 + 7, 2 ** 40], device="cuda")
+    assert ops.token_logprobs(z, wide).logprob.tolist() == [0.0, 0.0, 0.0]
+    t = torch.zeros(3, 2, device="cuda")
+    ids = torch.stack((wide, torch.tensor([3, 4, 5], device="cuda")), dim=1)
+    only = ops.distill_loss(z, ids[:, 1:], t[:, 1:])[0]
+    assert abs(float(ops.distill_loss(z, ids, t)[0]) - float(only)) <= 4 * U * abs(float(only))
+
+
+def test_one_row_and_scalars():
+    z = _logits(1, 777, "bf16")[0]
+    out = ops.token_logprobs(z, torch.tensor(5, device="cuda"), top_k=2)
+    want = R.token_logprobs(z.double(), torch.tensor(5, device="cuda"), 2)
+    assert out.logprob.shape == () and out.top_ids.shape == (2,) and torch.equal(out.top_ids, want[2])
+    assert abs(float(out.logprob) - float(want[0])) <= 2000 * U
+
+
+def test_positive_and_negative_maxima():
+    # exactly k thread maxima are positive: the first bit of the search already separates them
+    g = torch.Generator().manual_seed(11)
+    z = -torch.rand(4, 65536, generator=g) - 0.1
+    for r in range(4):
+        z[r, torch.randperm(65536, generator=g)[: 12 + r]] *= -1
+    for dtype in (torch.float32, torch.bfloat16):
+        x = z.to(dtype).cuda()
+        for k in (12, 13, 14, 15, 40):
+            _check_forward(x, torch.zeros(4, dtype=torch.long, device="cuda"), k, 1.0)
+
+
+def test_a_second_derivative_is_refused():
+    z = _logits(2, 30, "fp32").requires_grad_()
+    g, = torch.autograd.grad(ops.token_logprobs(z, torch.zeros(2, dtype=torch.int32, device="cuda")).logprob.sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.square().sum(), z)
+
+
+def test_two_streams_at_once():
+    z = [_logits(300, 20000, "bf16", seed=s).requires_grad_() for s in range(2)]
+    ids = torch.arange(300, device="cuda")
+    want = [ops.token_logprobs(x, ids, top_k=7) for x in z]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [None, None]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = ops.token_logprobs(z[i], ids, top_k=7)
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_refusals_on_a_gpu():
     z = _logits(2, 10, "fp32")
     ids = torch.zeros(2, dtype=torch.int32, device="cuda")
