@@ -382,18 +382,23 @@ void check_head(const Tensor& H, const Tensor& W, const char* name) {
               name, ": bf16 row-major hidden states [M, C] and weight [V, C]");
 }
 
-// The logits of a forward pass kept for its backward pass (undefined = recompute them there).
-Tensor keep_logits(const Tensor& H, const Tensor& W, bool keep) {
-  return keep ? torch::empty({H.size(0), (W.size(0) + 7) / 8 * 8}, H.options().dtype(at::kFloat)) : Tensor();
+// The logits of a forward pass kept for its backward pass, {distances, largest of 64} (see GemmVocab); undefined = they are
+// computed again there.
+struct Kept { Tensor z, top; };
+Kept keep_logits(const Tensor& H, const Tensor& W, bool keep) {
+  if (!keep) return {};
+  return {torch::empty({H.size(0), (W.size(0) + 7) / 8 * 8}, H.options().dtype(at::kHalf)),
+          torch::empty({H.size(0), (W.size(0) + 63) / 64}, H.options().dtype(at::kFloat))};
 }
-void set_kept(rk::GemmArgs& p, const Tensor& z, int64_t row) {
-  if (!z.defined()) return;
-  p.vocab.z = z.data_ptr<float>() + row * z.stride(0);
-  p.vocab.ldz = (int)z.stride(0);
+void set_kept(rk::GemmArgs& p, const Kept& k, int64_t row) {
+  if (!k.z.defined()) return;
+  p.vocab.z = static_cast<char*>(k.z.data_ptr()) + row * k.z.stride(0) * 2;
+  p.vocab.ldz = (int)k.z.stride(0);
+  p.vocab.z_top = k.top.data_ptr<float>() + row * k.top.stride(0);
 }
-const float* check_kept(const Tensor& z, const Tensor& H, const Tensor& W) {
-  check_rows(z, H, at::kFloat, {H.size(0), (W.size(0) + 7) / 8 * 8}, "kept logits");
-  return z.data_ptr<float>();
+void check_kept(const Kept& k, const Tensor& H, const Tensor& W) {
+  check_rows(k.z, H, at::kHalf, {H.size(0), (W.size(0) + 7) / 8 * 8}, "kept logits");
+  check_rows(k.top, H, at::kFloat, {H.size(0), (W.size(0) + 63) / 64}, "kept maxima");
 }
 
 // -> logprob, entropy [M], and for the backward pass stat [M, 4], the targets' z [M] and the kept logits
@@ -404,7 +409,8 @@ std::vector<Tensor> head_prob_stats(const Tensor& H, const Tensor& W, const Tens
   check_rows(ids, H, at::kInt, {M}, "ids");
   auto f32 = H.options().dtype(at::kFloat);
   Tensor lp = torch::empty({M}, f32), ent = torch::empty({M}, f32), stat = torch::empty({M, 4}, f32), tz = torch::empty({M}, f32);
-  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32), kept = keep_logits(H, W, keep);
+  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32);
+  const Kept kept = keep_logits(H, W, keep);
   for (int64_t r = 0; r < M; r += kHeadStatsRows) {
     const int64_t n = std::min(kHeadStatsRows, M - r);
     rk::GemmArgs p = head_gemm(H, W, r, n, rk::kEpiProbStats, pair, tau);
@@ -420,7 +426,7 @@ std::vector<Tensor> head_prob_stats(const Tensor& H, const Tensor& W, const Tens
                                       stream()) == 0,
                 "head_token_logprobs: combine launch failed");
   }
-  return {lp, ent, stat, tz, kept};
+  return {lp, ent, stat, tz, kept.z, kept.top};
 }
 
 void check_dz(const Tensor& dz, const Tensor& H, const Tensor& W) {
@@ -432,7 +438,7 @@ void check_dz(const Tensor& dz, const Tensor& H, const Tensor& W) {
 
 // Gradient of the rows' log-probabilities and entropies with respect to z, into dz (bf16 [M, V], padded row pitch).
 void head_prob_grad(const Tensor& H, const Tensor& W, const Tensor& ids, const Tensor& stat, const Tensor& tz,
-                    const Tensor& kept, const c10::optional<Tensor>& g_lp, const c10::optional<Tensor>& g_ent, double tau, Tensor dz,
+                    const Kept& kept, const c10::optional<Tensor>& g_lp, const c10::optional<Tensor>& g_ent, double tau, Tensor dz,
                     int64_t pair) {
   check_head(H, W, "head_token_logprobs");
   c10::cuda::CUDAGuard guard(H.device());
@@ -450,8 +456,9 @@ void head_prob_grad(const Tensor& H, const Tensor& W, const Tensor& ids, const T
   rk::HeadFix f{};
   f.dz = p.D; f.ld = dz.stride(0); f.rows = (int)M; f.V = (int)V; f.tau = (float)tau;
   f.target = p.vocab.target; f.target_z = tz.data_ptr<float>(); f.stat = p.vocab.stat; f.g0 = p.vocab.g0; f.g1 = p.vocab.g1;
-  if (kept.defined()) {
-    TORCH_CHECK(rk::head_prob_grad_kept(f, check_kept(kept, H, W), kept.stride(0), stream()) == 0,
+  if (kept.z.defined()) {
+    check_kept(kept, H, W);
+    TORCH_CHECK(rk::head_prob_grad_kept(f, kept.z.data_ptr(), kept.z.stride(0), kept.top.data_ptr<float>(), stream()) == 0,
                 "head_token_logprobs backward: launch failed");
     return;
   }
@@ -476,7 +483,8 @@ std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const T
   auto f32 = H.options().dtype(at::kFloat);
   Tensor stat = torch::empty({M, 4}, f32), weight = torch::empty({M, 2}, f32), am = torch::empty({M}, f32.dtype(at::kInt));
   Tensor tz = torch::empty({M}, f32), cz = torch::empty({M, K}, f32), rows = torch::empty({4, M}, f32);
-  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32), kept = keep_logits(H, W, keep);
+  Tensor buf = torch::empty({std::min(M, kHeadStatsRows), tiles, 4}, f32);
+  const Kept kept = keep_logits(H, W, keep);
   float* rp = rows.data_ptr<float>();
   for (int64_t r = 0; r < M; r += kHeadStatsRows) {
     const int64_t n = std::min(kHeadStatsRows, M - r);
@@ -512,14 +520,14 @@ std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const T
     t.in[i] = in[i]; t.out[i] = out[i].data_ptr<float>();
   }
   TORCH_CHECK(rk::row_totals(t, stream()) == 0, "head_distill_loss: totals launch failed");
-  for (const Tensor& x : {stat, weight, am, tz, cz, kept}) out.push_back(x);
+  for (const Tensor& x : {stat, weight, am, tz, cz, kept.z, kept.top}) out.push_back(x);
   return out;
 }
 
 // Gradient of g_ce ce_total + g_l2 l2_total + g_kd kd_total with respect to z, in units of `unit` (fp32 [1], written as well),
 // into dz (bf16 [M, V], padded row pitch).
 void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, const std::vector<Tensor>& saved, const Tensor& t_ids,
-                       const Tensor& t_prob, const Tensor& kept, const c10::optional<Tensor>& g_ce, const c10::optional<Tensor>& g_l2,
+                       const Tensor& t_prob, const Kept& kept, const c10::optional<Tensor>& g_ce, const c10::optional<Tensor>& g_l2,
                        const c10::optional<Tensor>& g_kd, double tau, Tensor dz, Tensor unit, int64_t pair) {
   check_head(H, W, "head_distill_loss");
   c10::cuda::CUDAGuard guard(H.device());
@@ -544,8 +552,9 @@ void head_distill_grad(const Tensor& H, const Tensor& W, const Tensor& targets, 
   f.g_l2 = rows_ptr(g_l2, H, 1, "g_l2");
   f.t_ids = t_ids.data_ptr<int>(); f.t_prob = t_prob.data_ptr<float>();
   f.unit = check_rows(unit, H, at::kFloat, {1}, "unit").data_ptr<float>();
-  if (kept.defined()) {
-    TORCH_CHECK(rk::head_distill_grad_kept(f, check_kept(kept, H, W), kept.stride(0), stream()) == 0,
+  if (kept.z.defined()) {
+    check_kept(kept, H, W);
+    TORCH_CHECK(rk::head_distill_grad_kept(f, kept.z.data_ptr(), kept.z.stride(0), kept.top.data_ptr<float>(), stream()) == 0,
                 "head_distill_loss backward: launch failed");
     return;
   }
@@ -786,8 +795,10 @@ std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, c
   return r;
 }
 // Logits are kept between the passes while they fit into `keep_bytes`.
-bool keeps(const Tensor& h, const Tensor& wc, int64_t keep_bytes) { return h.size(0) * ((wc.size(0) + 7) / 8 * 8) * 4 <= keep_bytes; }
-Tensor part(const Tensor& t, int64_t s, int64_t n) { return t.defined() ? t.narrow(0, s, n) : t; }
+bool keeps(const Tensor& h, const Tensor& wc, int64_t keep_bytes) { return h.size(0) * ((wc.size(0) + 7) / 8 * 8) * 2 <= keep_bytes; }
+Kept part(const Tensor& z, const Tensor& top, int64_t s, int64_t n) {
+  return z.defined() ? Kept{z.narrow(0, s, n), top.narrow(0, s, n)} : Kept{};
+}
 c10::optional<Tensor> part(const c10::optional<Tensor>& t, int64_t s, int64_t n) {
   return t.has_value() ? c10::optional<Tensor>(t->narrow(0, s, n)) : c10::nullopt;
 }
@@ -800,7 +811,7 @@ struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
     std::vector<Tensor> out = head_prob_stats(h, wc, idr, tau, pair, ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {
       save_head(ctx, hidden, w, main, tau, grad_bytes, pair);
-      ctx->save_for_backward({h, wc, idr, out[2], out[3], out[4]});
+      ctx->save_for_backward({h, wc, idr, out[2], out[3], out[4], out[5]});
     }
     return {out[0].view(ids.sizes()), out[1].view(ids.sizes())};
   }
@@ -819,7 +830,7 @@ struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
       const double tau = ctx->saved_data["tau"].toDouble();
       const int64_t pair = ctx->saved_data["pair"].toInt();
       r = head_backward(ctx, s[0], s[1], Tensor(), [&](int64_t b, int64_t n, const Tensor& dz) {
-        head_prob_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[5], b, n), part(g_lp, b, n),
+        head_prob_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[5], s[6], b, n), part(g_lp, b, n),
                        part(g_ent, b, n), tau, dz, pair);
       });
     }
@@ -849,7 +860,7 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
                                                  ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {
       save_head(ctx, hidden, w, main, tau, grad_bytes, pair);
-      ctx->save_for_backward({h, wc, tgt, t[0], t[1], out[6], out[7], out[8], out[9], out[10], out[11]});
+      ctx->save_for_backward({h, wc, tgt, t[0], t[1], out[6], out[7], out[8], out[9], out[10], out[11], out[12]});
       ctx->mark_non_differentiable({out[1], out[3], out[5]});
     }
     return {out[0], out[1], out[2], out[3], out[4], out[5]};
@@ -873,7 +884,7 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
       r = head_backward(ctx, s[0], s[1], unit, [&](int64_t b, int64_t n, const Tensor& dz) {
         std::vector<Tensor> rows;
         for (int i = 5; i < 10; ++i) rows.push_back(s[i].narrow(0, b, n));
-        head_distill_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), rows, s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[10], b, n), g_ce, g_l2,
+        head_distill_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), rows, s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[10], s[11], b, n), g_ce, g_l2,
                           g_kd, tau, dz, unit, pair);
       });
     }

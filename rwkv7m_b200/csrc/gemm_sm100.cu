@@ -11,6 +11,7 @@
 // dW = dy^T x without any transposition pass.  Every wait is bounded: when a
 // limit runs out the CTA records an error code, drains and frees TMEM.
 #include <cuda.h>
+#include <cuda_fp16.h>
 
 #include <cstdio>
 #include <cstdlib>
@@ -265,14 +266,19 @@ struct VocabRow {
   int am, k, next, tgt;
 };
 
+// columns past the last one take no part
+__device__ __forceinline__ void vocab_mask_columns(uint32_t (&v)[32], int col0, int N) {
+  if (col0 + 32 <= N) return;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) if (col0 + j >= N) v[j] = 0xff800000u;
+}
+
+// `cm`: the largest of the 32 logits
 template <int EPI>
-__device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, uint32_t (&v)[32], int col0, int N, size_t row, const GemmVocab& g) {
+__device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, const uint32_t (&v)[32], float cm, int col0, int N, size_t row,
+                                                  const GemmVocab& g) {
   if (col0 >= N) return;
   const bool ragged = col0 + 32 > N;
-  if (ragged) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) if (col0 + j >= N) v[j] = 0xff800000u;
-  }
   if (st.tgt >= col0 && st.tgt < col0 + 32) g.target_z[row] = pick32(v, st.tgt - col0);
   if (EPI == kEpiDistillStats) {
     while (st.next < col0 + 32) {          // the teacher's alternatives come in the order of the columns
@@ -281,10 +287,6 @@ __device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, uint32_t (&v)[32
       st.next = st.k < g.listed ? g.cols[row * g.listed + st.k] : 0x7fffffff;
     }
   }
-  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(v[j]));
-  const float cm = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
   if (cm > st.m) {
     if (st.m != -INFINITY) {
       const float d = (st.m - cm) * g.c, f = ex2(d);
@@ -301,6 +303,7 @@ __device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, uint32_t (&v)[32
     }
   }
   const float mc = st.m * g.c, m1 = st.m * 1.4426950408889634f;
+  const bool one = EPI == kEpiDistillStats && g.tau == 1.f;     // both temperatures are the same
   float a[2] = {0.f, 0.f}, b[2] = {0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
@@ -310,10 +313,11 @@ __device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, uint32_t (&v)[32
     const float e = ex2(t);
     a[j & 1] += e;
     if (EPI == kEpiProbStats) b[j & 1] = fmaf(e, t, b[j & 1]);
-    else b[j & 1] += ex2(fmaf(z, 1.4426950408889634f, -m1));
+    else if (!one) b[j & 1] += ex2(fmaf(z, 1.4426950408889634f, -m1));
   }
   st.s1 += a[0] + a[1];
-  st.s2 += b[0] + b[1];
+  if (EPI == kEpiDistillStats && one) st.s2 = st.s1;
+  else st.s2 += b[0] + b[1];
 }
 
 // A row's factors of the gradient epilogues: dz = q (A + B log2 q) with log2 q = z c + b, or a1 2^(z log2e + b1) + a 2^(z c + b).
@@ -364,21 +368,38 @@ constexpr int kOutStageBytes = 128 * 128;   // 128 rows x 64 bf16
 
 __device__ __forceinline__ void epilogue_named_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// A chunk of 32 fp32 columns of this thread's row into a 16 KB staging buffer (128 rows x 128 bytes, 128-byte swizzle).
-__device__ __forceinline__ void stage_f32(const uint32_t (&v)[32], uint8_t* buf, int tile_row) {
+// 64 logits of this thread's row as fp16 distances below their largest, into a 16 KB staging buffer (128 rows x 128 bytes,
+// 128-byte swizzle).  What matters in a row is close to its maximum: a distance d carries an error of 2^-12 |d|, so q = 2^d
+// is off by less than the bf16 rounding of its gradient wherever q is more than a few percent of the largest.
+__device__ __forceinline__ void stage_distances(const uint32_t (&v0)[32], const uint32_t (&v1)[32], float top, uint8_t* buf, int tile_row) {
+  uint32_t pk[32];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const __half2 a = __floats2half2_rn(__uint_as_float(v0[2 * j]) - top, __uint_as_float(v0[2 * j + 1]) - top);
+    const __half2 b = __floats2half2_rn(__uint_as_float(v1[2 * j]) - top, __uint_as_float(v1[2 * j + 1]) - top);
+    pk[j] = *reinterpret_cast<const uint32_t*>(&a);
+    pk[16 + j] = *reinterpret_cast<const uint32_t*>(&b);
+  }
   uint8_t* dst = buf + tile_row * 128;
   const int sw = tile_row & 7;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<uint4*>(dst + ((j ^ sw) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    *reinterpret_cast<uint4*>(dst + ((j ^ sw) << 4)) = make_uint4(pk[4 * j], pk[4 * j + 1], pk[4 * j + 2], pk[4 * j + 3]);
   fence_proxy_async_smem();
 }
 
+__device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
+  float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(v[j]));
+  return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+}
+
 // Statistics of this thread's row over the 256 columns of a tile, from the accumulator at taddr.  With `tm` not null the
-// logits are stored as well, boxes of 128 rows x 32 columns through the staging buffers, while their statistics are taken.
+// logits are kept as well, 64 columns at a time: the largest in fp32, the distances below it through the staging buffers.
 template <int EPI>
 __device__ __forceinline__ void vocab_stats_tile(uint32_t taddr, int m0, int tile_row, int n0, int N, int M, float4* __restrict__ out,
-                                                 const GemmVocab& g, const CUtensorMap* tm, uint8_t* out_stage, bool issuer) {
+                                                 const GemmVocab& g, const CUtensorMap* tm, uint8_t* out_stage, int& obuf, bool issuer) {
   const int row = m0 + tile_row;
   const bool live = row < M;
   VocabRow st{-INFINITY, 0.f, 0.f, 0, 0, 0x7fffffff, -1};
@@ -401,25 +422,22 @@ __device__ __forceinline__ void vocab_stats_tile(uint32_t taddr, int m0, int til
     tmem_ld_32x32(taddr + c * 32, v0);
     tmem_ld_32x32(taddr + c * 32 + 32, v1);
     tmem_ld_wait();
-    if (tm != nullptr && m0 < M) {           // the same for all 128 threads
-      const int c0 = n0 + c * 32;
-      if (c0 < N) {
-        stage_f32(v0, out_stage, tile_row);
-        if (c0 + 32 < N) stage_f32(v1, out_stage + kOutStageBytes, tile_row);
-        epilogue_named_barrier();
-        if (issuer) {
-          tma_store_2d(tm, out_stage, c0, m0);
-          if (c0 + 32 < N) tma_store_2d(tm, out_stage + kOutStageBytes, c0 + 32, m0);
-          tma_store_commit();
-        }
-      }
-    }
-    vocab_stats_chunk<EPI>(st, v0, n0 + c * 32, N, (size_t)row, g);
-    vocab_stats_chunk<EPI>(st, v1, n0 + c * 32 + 32, N, (size_t)row, g);
-    if (tm != nullptr && m0 < M) {           // both buffers are free again before the next round writes them
-      if (issuer) tma_store_wait_read<0>();
+    const int c0 = n0 + c * 32;
+    vocab_mask_columns(v0, c0, N);
+    vocab_mask_columns(v1, c0 + 32, N);
+    const float m0c = max32(v0), m1c = max32(v1);
+    if (tm != nullptr && m0 < M && c0 < N) {           // the same for all 128 threads
+      uint8_t* buf = out_stage + obuf * kOutStageBytes;
+      const float top = fmaxf(m0c, m1c);
+      stage_distances(v0, v1, top, buf, tile_row);
+      if (live) g.z_top[(size_t)row * ((N + 63) / 64) + c0 / 64] = top;
+      if (issuer) tma_store_wait_read<0>();           // the other buffer, before the next round writes it
       epilogue_named_barrier();
+      if (issuer) { tma_store_2d(tm, buf, c0, m0); tma_store_commit(); }
+      obuf ^= 1;                                      // over the tiles too: a ragged tile may end on either buffer
     }
+    vocab_stats_chunk<EPI>(st, v0, m0c, c0, N, (size_t)row, g);
+    vocab_stats_chunk<EPI>(st, v1, m1c, c0 + 32, N, (size_t)row, g);
   }
   if (live)
     *out = EPI == kEpiProbStats ? make_float4(st.m, st.s1, st.s2, 0.f) : make_float4(st.m, st.s2, st.s1, __int_as_float(st.am));
@@ -637,7 +655,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
       } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
         vocab_stats_tile<EPI>(t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
-                              tma_out != 0 ? &tmD : nullptr, out_stage, issuer);
+                              tma_out != 0 ? &tmD : nullptr, out_stage, obuf, issuer);
       } else if constexpr (BN >= 64) {
         VocabCoef coef;
         if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
@@ -1063,7 +1081,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
       } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
         vocab_stats_tile<EPI>(t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
-                              tma_out != 0 ? &tmD : nullptr, out_stage, issuer);
+                              tma_out != 0 ? &tmD : nullptr, out_stage, obuf, issuer);
       } else {
       VocabCoef coef;
       if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
@@ -1140,30 +1158,29 @@ EncodeTiledFn encode_fn() {
 }
 
 struct MapKey {
-  const void* ptr; int rows, cols, ld, box_rows; bool f32;
+  const void* ptr; int rows, cols, ld, box_rows;
   bool operator==(const MapKey& o) const {
-    return ptr == o.ptr && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows && f32 == o.f32;
+    return ptr == o.ptr && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows;
   }
 };
 struct MapKeyHash {
   size_t operator()(const MapKey& k) const {
     size_t h = reinterpret_cast<size_t>(k.ptr);
     h ^= (size_t)k.rows * 0x9E3779B97F4A7C15ull + (size_t)k.cols * 0xC2B2AE3D27D4EB4Full;
-    h ^= ((size_t)k.ld << 20) ^ (size_t)k.box_rows ^ ((size_t)k.f32 << 40);
+    h ^= ((size_t)k.ld << 20) ^ (size_t)k.box_rows;
     return h;
   }
 };
 
-// Row-major bf16 (or fp32) matrix [rows, cols] with leading dimension ld; box = 128 bytes of columns x box_rows rows, 128B
-// swizzle.
+// Row-major matrix [rows, cols] of 16-bit elements with leading dimension ld; box = 64 columns x box_rows rows, 128B swizzle.
 // The cache stores the 128 descriptor bytes as a plain byte array: CUtensorMap is 64-byte aligned and
 // node-based containers do not honour that alignment under every host compiler configuration.
 struct MapBytes { unsigned char raw[sizeof(CUtensorMap)]; };
 
-bool make_map(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int box_rows, bool f32 = false) {
+bool make_map(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int box_rows) {
   static std::unordered_map<MapKey, MapBytes, MapKeyHash> cache;
   static std::mutex mu;
-  MapKey key{ptr, rows, cols, ld, box_rows, f32};
+  MapKey key{ptr, rows, cols, ld, box_rows};
   {
     std::lock_guard<std::mutex> g(mu);
     auto it = cache.find(key);
@@ -1182,10 +1199,10 @@ bool make_map(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int
     context_bound = true;
   }
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)ld * (f32 ? 4 : 2)};
-  cuuint32_t box[2] = {f32 ? 32u : 64u, (cuuint32_t)box_rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1u, 1u};
-  CUresult r = fn(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return false;
@@ -1270,7 +1287,7 @@ int launch(const GemmArgs& p, cudaStream_t st) {
       (!kTwoInput || (p.N % 64 == 0 && (reinterpret_cast<uintptr_t>(p.aux) & 15) == 0 && p.ldaux % 8 == 0)))
     tma_out = make_map(&td, p.D, p.M, p.N, p.ldd, BM) ? 1 : 0;
   if ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && p.vocab.z != nullptr) {
-    if (!make_map(&td, p.vocab.z, p.M, p.N, p.vocab.ldz, BM, true)) return 2;
+    if (!make_map(&td, p.vocab.z, p.M, p.N, p.vocab.ldz, BM)) return 2;
     tma_out = 1;
   }
   if (kVocabGrad && tma_out == 0) return 2;
@@ -1376,7 +1393,7 @@ int launch_pair(const GemmArgs& p, cudaStream_t st) {
       (!kTwoInput || (p.N % 64 == 0 && (reinterpret_cast<uintptr_t>(p.aux) & 15) == 0 && p.ldaux % 8 == 0)))
     tma_out = make_map(&td, p.D, p.M, p.N, p.ldd, BM) ? 1 : 0;
   if ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && p.vocab.z != nullptr) {
-    if (!make_map(&td, p.vocab.z, p.M, p.N, p.vocab.ldz, BM, true)) return 2;
+    if (!make_map(&td, p.vocab.z, p.M, p.N, p.vocab.ldz, BM)) return 2;
     tma_out = 1;
   }
   if (kVocabGrad && tma_out == 0) return 2;
@@ -1730,7 +1747,7 @@ int gemm_bf16(const GemmArgs& p, cudaStream_t st) {
   if (p.epilogue == kEpiProbStats || p.epilogue == kEpiDistillStats || p.epilogue == kEpiProbGrad || p.epilogue == kEpiDistillGrad) {
     const bool stats = p.epilogue == kEpiProbStats || p.epilogue == kEpiDistillStats;
     if (p.layout != kGemmTN || (stats ? (p.ldd & 3) || p.ldd < 4 * ((p.N + 255) / 256) : (p.ldd & 7) || p.ldd < p.N)) return 6;
-    if (stats && p.vocab.z != nullptr && ((reinterpret_cast<uintptr_t>(p.vocab.z) & 15) || (p.vocab.ldz & 3) || p.vocab.ldz < p.N)) return 6;
+    if (stats && p.vocab.z != nullptr && ((reinterpret_cast<uintptr_t>(p.vocab.z) & 15) || (p.vocab.ldz & 7) || p.vocab.ldz < p.N || p.vocab.z_top == nullptr)) return 6;
     if (p.error_flag == nullptr) return 7;
     return launch_vocab(p, st);
   }

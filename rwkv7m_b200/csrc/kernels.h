@@ -177,9 +177,9 @@ struct HeadFix {
   const int* t_ids; const float* t_prob; const float* cols_z;
 };
 int head_prob_fix(const HeadFix& a, cudaStream_t st);
-// The whole gradient from kept logits z (fp32, row pitch ldz a multiple of 4 floats): dense part and listed columns.
-int head_prob_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st);
-int head_distill_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st);
+// The whole gradient from kept logits (GemmVocab::z, z_top): dense part and listed columns.
+int head_prob_grad_kept(const HeadFix& a, const void* z, int64_t ldz, const float* z_top, cudaStream_t st);
+int head_distill_grad_kept(const HeadFix& a, const void* z, int64_t ldz, const float* z_top, cudaStream_t st);
 int head_distill_fix(const HeadFix& a, cudaStream_t st);
 
 // ---- data-parallel optimizer step over symmetric memory -------------------------------
@@ -302,7 +302,8 @@ enum GemmEpilogue {
 struct GemmVocab {
   float c;                 // log2(e) / tau: t = (z - max) c
   float inv_tau, tau;
-  float* z; int ldz;       // statistics: the logits themselves as well, fp32 with a row pitch that is a multiple of 4; or null
+  void* z; int ldz;        // statistics, or null: the logits are kept as well, fp16 distances [M, N] below the largest of every
+  float* z_top;            // 64 columns (row pitch ldz a multiple of 8), and those [M, ceil(N / 64)]
   int listed;              // columns per row in `cols` (kEpiDistillStats)
   const int* target;       // [M]: the column whose z goes to target_z (statistics)
   float* target_z;

@@ -14,6 +14,8 @@
 #include <climits>
 #include <type_traits>
 
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -937,65 +939,76 @@ __global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
   distill_listed(a, k, row, 0, a.V, threadIdx.x & 31, 32);
 }
 
-// Gradient from kept logits: fp32 in, bf16 out.  A thread takes 8 columns at a time (32 bytes in, 16 out), a CTA `iters`
-// blocks of 4096 columns, the next block's logits in flight while one is written.  Rows from the last to the first, as above.
+// Gradient from kept logits: fp16 distances in, bf16 out.  A thread takes 8 columns at a time (16 bytes in, 16 out), a CTA
+// `iters` blocks of 8192 columns, the next block's in flight while one is written.  Rows from the last to the first, as above.
 template <bool DISTILL>
-__global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const float* __restrict__ z, int64_t ldz, int iters) {
-  constexpr int kBlock = 256 * 8 * 2;
+__global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const __half* __restrict__ z, int64_t ldz,
+                                                                const float* __restrict__ z_top, int iters) {
+  constexpr int kEach = 4, kBlock = 256 * 8 * kEach;
   const int row = a.rows - 1 - (int)blockIdx.y, tid = threadIdx.x;
   const int c0 = blockIdx.x * kBlock * iters, c1 = min(a.V, c0 + kBlock * iters);
   if (c0 >= c1) return;
-  const float* x = z + (size_t)row * ldz;
+  const __half* x = z + (size_t)row * ldz;
+  const float* tops = z_top + (size_t)row * ((a.V + 63) / 64);
   bf16* out = reinterpret_cast<bf16*>(a.dz) + (size_t)row * a.ld;
   // both pitches cover whole groups of 8 columns, so the last group of a row is read and written whole
-  auto fetch = [&](float4 (&buf)[4], int c) {
+  auto fetch = [&](uint4 (&buf)[kEach], float (&top)[kEach], int c) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kEach; ++i) {
       const int col = c + (tid + i * 256) * 8;
       if (col < c1) {
-        buf[2 * i] = __ldg(reinterpret_cast<const float4*>(x + col));
-        buf[2 * i + 1] = __ldg(reinterpret_cast<const float4*>(x + col + 4));
+        buf[i] = __ldg(reinterpret_cast<const uint4*>(x + col));
+        top[i] = __ldg(tops + col / 64);
       }
     }
   };
-  float4 cur[4];
-  fetch(cur, c0);
+  uint4 cur[kEach];
+  float top[kEach];
+  fetch(cur, top, c0);
   float gl;
   bool live;
   const HeadCoef k = head_coef<DISTILL>(a, row, gl, live);
   if (DISTILL && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *a.unit = k.unit;
-  const f2 nm = pack2(-k.m, -k.m), cc = pack2(k.c, k.c), nl = pack2(-k.l2st, -k.l2st), A2 = pack2(k.A, k.A), B2 = pack2(k.B, k.B);
-  const f2 c1v = pack2(kLog2e, kLog2e), nl1 = pack2(-k.l2s1, -k.l2s1), gk = pack2(k.g_kd, k.g_kd), gc = pack2(k.g_ce, k.g_ce);
-  auto value2 = [&](float z0, float z1) {
-    const f2 d = add2(pack2(z0, z1), nm), l = fma2(d, cc, nl);
+  const f2 cc = pack2(k.c, k.c), nl = pack2(-k.l2st, -k.l2st), A2 = pack2(k.A, k.A), B2 = pack2(k.B, k.B);
+  const bool one = DISTILL && a.tau == 1.f;           // both softmaxes are the same
+  const float g_kd = one ? k.g_kd + k.g_ce : k.g_kd;
+  const f2 c1v = pack2(kLog2e, kLog2e), nl1 = pack2(-k.l2s1, -k.l2s1), gk = pack2(g_kd, g_kd), gc = pack2(k.g_ce, k.g_ce);
+  auto value2 = [&](uint32_t h, f2 below) {           // below: the group's largest logit minus the row's
+    const float2 zf = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    const f2 d = add2(pack2(zf.x, zf.y), below), l = fma2(d, cc, nl);
     float l0, l1, r0, r1;
     unpack2(l, l0, l1);
     const f2 q = pack2(exp2_fast(l0), exp2_fast(l1));
-    if (DISTILL) {
+    if (DISTILL && one) {
+      unpack2(mul2(q, gk), r0, r1);
+    } else if (DISTILL) {
       float e0, e1;
       unpack2(fma2(d, c1v, nl1), e0, e1);
       unpack2(fma2(gk, q, mul2(gc, pack2(exp2_fast(e0), exp2_fast(e1)))), r0, r1);
     } else {
       unpack2(mul2(q, fma2(B2, l, A2)), r0, r1);
     }
-    const __nv_bfloat162 h = __floats2bfloat162_rn(r0, r1);
-    return *reinterpret_cast<const uint32_t*>(&h);
+    const __nv_bfloat162 o = __floats2bfloat162_rn(r0, r1);
+    return *reinterpret_cast<const uint32_t*>(&o);
   };
   for (int c = c0; c < c1; c += kBlock) {
-    float4 nxt[4];
-    if (c + kBlock < c1) fetch(nxt, c + kBlock);
+    uint4 nxt[kEach];
+    float ntop[kEach];
+    if (c + kBlock < c1) fetch(nxt, ntop, c + kBlock);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kEach; ++i) {
       const int col = c + (tid + i * 256) * 8;
       if (col < c1) {
-        const float4 p = cur[2 * i], q = cur[2 * i + 1];
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (live) w = make_uint4(value2(p.x, p.y), value2(p.z, p.w), value2(q.x, q.y), value2(q.z, q.w));
+        if (live) {
+          const f2 below = pack2(top[i] - k.m, top[i] - k.m);
+          w = make_uint4(value2(cur[i].x, below), value2(cur[i].y, below), value2(cur[i].z, below), value2(cur[i].w, below));
+        }
         *reinterpret_cast<uint4*>(out + col) = w;
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) cur[i] = nxt[i];
+    for (int i = 0; i < kEach; ++i) { cur[i] = nxt[i]; top[i] = ntop[i]; }
   }
   __syncthreads();
   if (DISTILL) distill_listed(a, k, row, c0, c1, tid, 256);
@@ -1003,13 +1016,13 @@ __global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const
 }
 
 template <bool DISTILL>
-int launch_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st) {
+int launch_grad_kept(const HeadFix& a, const void* z, int64_t ldz, const float* z_top, cudaStream_t st) {
   if (a.rows <= 0) return 0;
   if (a.rows > 65535 || (ldz & 7) || (a.ld & 7) || ldz < (a.V + 7) / 8 * 8 || a.ld < (a.V + 7) / 8 * 8) return 6;
-  const int blocks = (a.V + 4095) / 4096;
+  const int blocks = (a.V + 8191) / 8192;
   int iters = 1;
   while (iters < 4 && iters < blocks && (int64_t)a.rows * blocks >= 8ll * iters * 4 * 148) iters *= 2;
-  head_grad_kept_kernel<DISTILL><<<dim3((blocks + iters - 1) / iters, a.rows), 256, 0, st>>>(a, z, ldz, iters);
+  head_grad_kept_kernel<DISTILL><<<dim3((blocks + iters - 1) / iters, a.rows), 256, 0, st>>>(a, static_cast<const __half*>(z), ldz, z_top, iters);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
@@ -1112,12 +1125,12 @@ int head_distill_fix(const HeadFix& a, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
-int head_prob_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st) {
-  return launch_grad_kept<false>(a, z, ldz, st);
+int head_prob_grad_kept(const HeadFix& a, const void* z, int64_t ldz, const float* z_top, cudaStream_t st) {
+  return launch_grad_kept<false>(a, z, ldz, z_top, st);
 }
 
-int head_distill_grad_kept(const HeadFix& a, const float* z, int64_t ldz, cudaStream_t st) {
-  return launch_grad_kept<true>(a, z, ldz, st);
+int head_distill_grad_kept(const HeadFix& a, const void* z, int64_t ldz, const float* z_top, cudaStream_t st) {
+  return launch_grad_kept<true>(a, z, ldz, z_top, st);
 }
 
 }  // namespace rk

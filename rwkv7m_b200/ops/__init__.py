@@ -375,7 +375,7 @@ def head_token_logprobs(hidden, head_w, ids, *, temperature=1.0):
     """``(logprob, entropy)`` of :func:`token_logprobs` for the logits ``hidden`` [..., C] @ ``head_w`` [V, C].T, which are not
     returned: forward reduces them where the product leaves them, in fp32.  ``hidden`` is what the head reads (behind the
     final layer norm) and has to be finite at every position, scored or not.  Differentiable in both; for the backward pass
-    the GPU keeps the fp32 logits up to ``RWKV7M_B200_HEAD_KEEP_BYTES`` (8 GiB) and computes larger ones again."""
+    the GPU keeps the logits in 16 bits up to ``RWKV7M_B200_HEAD_KEEP_BYTES`` (4 GiB) and computes larger ones again."""
     name = "head_token_logprobs"
     _check_head(name, hidden, head_w)
     _check_ids(name, ids, hidden.shape[:-1], hidden.device)

@@ -1093,9 +1093,9 @@ def distill_loss(logits, teacher_ids, teacher_logits, mask, tau):
 # Size of the [rows, V] bf16 gradient of the logits that a backward pass through the head holds at a time (16384 rows of a
 # 65536-token vocabulary).
 HEAD_GRAD_BYTES = 2 << 30
-# A forward pass through the head keeps its fp32 logits for the backward pass while they fit into this many bytes; beyond, they
-# are computed a second time.
-HEAD_KEEP_BYTES = int(os.environ.get("RWKV7M_B200_HEAD_KEEP_BYTES", str(8 << 30)))
+# A forward pass through the head keeps its logits for the backward pass (16 bits each, as distances below the largest of 64)
+# while they fit into this many bytes; beyond, they are computed a second time.
+HEAD_KEEP_BYTES = int(os.environ.get("RWKV7M_B200_HEAD_KEEP_BYTES", str(4 << 30)))
 
 
 def _head_kernels_apply(hidden):
