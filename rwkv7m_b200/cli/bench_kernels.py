@@ -267,9 +267,65 @@ def bench_lora_group(M, C, iters=10, ranks=(128, 128, 224, 64), acts=(1, 0, 2, 0
     return [row]
 
 
+def bench_distribution(rows, M, C, V, K=32, iters=10):
+    """The operators on the distribution over the vocabulary: from logits [rows, V], and through the head at [M, C] x [V, C]."""
+    from rwkv7m_b200 import ops
+
+    dev = "cuda"
+    logits = (torch.randn(rows, V, device=dev) * 3).bfloat16().requires_grad_(True)
+    ids = torch.randint(0, V, (rows,), device=dev, dtype=torch.int32)
+    up = torch.randn(rows, device=dev) / rows
+    flush = torch.empty(256 * 1024 * 1024, dtype=torch.uint8, device=dev)
+
+    def teacher(n):
+        return (torch.randint(0, V, (n, K), device=dev, dtype=torch.int32), (torch.randn(n, K, device=dev) * 3).bfloat16())
+
+    t_ids, t_logits = teacher(rows)
+    hidden = torch.randn(M, C, device=dev).bfloat16().requires_grad_(True)
+    head = (torch.randn(V, C, device=dev) * (2.0 / C ** 0.5)).bfloat16().requires_grad_(True)
+    targets = torch.randint(0, V, (M,), device=dev, dtype=torch.int32)
+    h_ids, h_logits = teacher(M)
+    h_up = torch.randn(M, device=dev) / M
+
+    def scores(top_k):
+        with torch.no_grad():
+            ops.token_logprobs(logits, ids, top_k=top_k)
+
+    def scores_grad():
+        out = ops.token_logprobs(logits, ids)
+        torch.autograd.grad((out.logprob, out.entropy), logits, (up, up))
+
+    def distill():
+        kd, count = ops.distill_loss(logits, t_ids, t_logits, temperature=2.0)
+        torch.autograd.grad(kd / count, logits)
+
+    def head_scores():
+        with torch.no_grad():
+            ops.head_token_logprobs(hidden, head, targets)
+
+    def head_scores_grad():
+        torch.autograd.grad(ops.head_token_logprobs(hidden, head, targets), (hidden, head), (h_up, h_up))
+
+    def head_distill():
+        ce, n, l2, ln, kd, kn = ops.head_distill_loss(hidden, head, targets, None, h_ids, h_logits, temperature=2.0)
+        torch.autograd.grad(0.5 * ce / n + 0.5 * kd / kn + l2 / ln, (hidden, head))
+
+    once, product = 2.0 * rows * V, 2.0 * M * V * C
+    out = []
+    for name, fn, nbytes in (("token_logprobs fwd", lambda: scores(0), once), ("token_logprobs fwd, 20 alternatives", lambda: scores(20), once),
+                             ("token_logprobs fwd+bwd", scores_grad, 3 * once), ("distill_loss fwd+bwd", distill, 3 * once)):
+        ms = _time(fn, iters, flush=flush)["median_ms"]
+        out.append({"kernel": name, "rows": rows, "V": V, "ms": ms, "gbs": nbytes / ms / 1e6})
+    for name, fn, flops in (("head_token_logprobs fwd", head_scores, product), ("head_token_logprobs fwd+bwd", head_scores_grad, 3 * product),
+                            ("head_distill_loss fwd+bwd", head_distill, 3 * product)):
+        ms = _time(fn, iters, flush=flush)["median_ms"]
+        out.append({"kernel": name, "M": M, "C": C, "V": V, "ms": ms, "tflops": flops / ms / 1e9})
+    return out
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("--what", default="wkv,gemm", help="comma list of wkv, gemm, fused, optim, loss, screening, lora")
+    ap.add_argument("--what", default="wkv,gemm", help="comma list of wkv, gemm, fused, optim, loss, screening, lora, distribution")
     ap.add_argument("--gemm-shape", default=None, help="M,N,K of a single GEMM case")
     ap.add_argument("--wkv-shape", default=None, help="T,B,H,N of a single WKV case")
     ap.add_argument("--wkv-impl", choices=["chunked", "sequential"], default=None)
@@ -307,6 +363,9 @@ def main(argv=None):
         results += bench_screening(8, steps, iters=min(args.iters, 3), preset=args.screen_preset)
     if "lora" in args.what:
         results += bench_lora_group(4096 if args.small else 32768, 2048, iters=args.iters)
+    if "distribution" in args.what:
+        shape = (2048, 2048, 1024) if args.small else (4096, 16384, 2048)
+        results += bench_distribution(*shape, 65536, iters=args.iters)
     if "optim" in args.what:
         results += bench_optimizer((64 if args.small else 512) * 1024 * 1024, iters=args.iters)
     for r in results:

@@ -941,6 +941,8 @@ __global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
 
 // Gradient from kept logits: fp16 distances in, bf16 out.  A thread takes 8 columns at a time (16 bytes in, 16 out), a CTA
 // `iters` blocks of 8192 columns, the next block's in flight while one is written.  Rows from the last to the first, as above.
+// Bound by memory and, with two temperatures, by two exponentials an element: 16384 x 65536 take 858 us, 5.0 TB/s; 4093 x
+// 65536 with one 164 us, 6.5 TB/s.
 template <bool DISTILL>
 __global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const __half* __restrict__ z, int64_t ldz,
                                                                 const float* __restrict__ z_top, int iters) {
@@ -1020,8 +1022,9 @@ int launch_grad_kept(const HeadFix& a, const void* z, int64_t ldz, const float* 
   if (a.rows <= 0) return 0;
   if (a.rows > 65535 || (ldz & 7) || (a.ld & 7) || ldz < (a.V + 7) / 8 * 8 || a.ld < (a.V + 7) / 8 * 8) return 6;
   const int blocks = (a.V + 8191) / 8192;
+  // as in row_grad; 16384 x 65536: 1331 us with one block per CTA, 1057 with two, 894 with four, 858 with eight
   int iters = 1;
-  while (iters < 4 && iters < blocks && (int64_t)a.rows * blocks >= 8ll * iters * 4 * 148) iters *= 2;
+  while (iters < 8 && iters < blocks && (int64_t)a.rows * blocks >= 2ll * iters * 4 * 148) iters *= 2;
   head_grad_kept_kernel<DISTILL><<<dim3((blocks + iters - 1) / iters, a.rows), 256, 0, st>>>(a, static_cast<const __half*>(z), ldz, z_top, iters);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
@@ -1054,10 +1057,10 @@ int row_grad(const RowGradArgs& a, cudaStream_t st) {
   const int E = a.is_bf16 ? 8 : 4;
   const int units = (a.V + 2 * E - 2) / E;            // the most a row can touch, whatever its alignment
   const int blocks = (units + kThreads * kUnroll - 1) / (kThreads * kUnroll);
-  // up to four blocks per CTA, as long as that leaves a few waves of CTAs (4096 bf16 rows of 65536: 226 us with one, 179
-  // with two, 163 with four, 164 with eight)
+  // up to four blocks per CTA while that leaves a wave of CTAs (4096 bf16 rows of 65536: 230 us with one, 180 with two, 163 with
+  // four, 164 with eight; 256 rows: 12.8, 11.6, 11.6, 19.4; 16 rows: 3.7, 4.7, 6.7, 11.2)
   int iters = 1;
-  while (iters < 4 && iters < blocks && (int64_t)a.rows * blocks >= 8ll * iters * 4 * 148) iters *= 2;
+  while (iters < 4 && iters < blocks && (int64_t)a.rows * blocks >= 2ll * iters * 4 * 148) iters *= 2;
   const int parts = (blocks + iters - 1) / iters;
   // the grid's second axis ends at 65535 rows
   for (int r0 = (a.rows - 1) / 65535 * 65535; r0 >= 0; r0 -= 65535) {
