@@ -796,11 +796,11 @@ std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, c
 }
 // Logits are kept between the passes while they fit into `keep_bytes`.
 bool keeps(const Tensor& h, const Tensor& wc, int64_t keep_bytes) { return h.size(0) * ((wc.size(0) + 7) / 8 * 8) * 2 <= keep_bytes; }
-Kept part(const Tensor& z, const Tensor& top, int64_t s, int64_t n) {
-  return z.defined() ? Kept{z.narrow(0, s, n), top.narrow(0, s, n)} : Kept{};
-}
+// Rows [s, s + n) of what a pass saved
+Tensor part(const Tensor& t, int64_t s, int64_t n) { return n == t.size(0) ? t : t.narrow(0, s, n); }
+Kept part(const Tensor& z, const Tensor& top, int64_t s, int64_t n) { return z.defined() ? Kept{part(z, s, n), part(top, s, n)} : Kept{}; }
 c10::optional<Tensor> part(const c10::optional<Tensor>& t, int64_t s, int64_t n) {
-  return t.has_value() ? c10::optional<Tensor>(t->narrow(0, s, n)) : c10::nullopt;
+  return t.has_value() ? c10::optional<Tensor>(part(*t, s, n)) : c10::nullopt;
 }
 
 // `wc` is the bf16 weight that the products read (w itself, or the copy kept beside it), `main` a bound fp32 main gradient.
@@ -830,7 +830,7 @@ struct HeadTokenLogprobs : torch::autograd::Function<HeadTokenLogprobs> {
       const double tau = ctx->saved_data["tau"].toDouble();
       const int64_t pair = ctx->saved_data["pair"].toInt();
       r = head_backward(ctx, s[0], s[1], Tensor(), [&](int64_t b, int64_t n, const Tensor& dz) {
-        head_prob_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[5], s[6], b, n), part(g_lp, b, n),
+        head_prob_grad(part(s[0], b, n), s[1], part(s[2], b, n), part(s[3], b, n), part(s[4], b, n), part(s[5], s[6], b, n), part(g_lp, b, n),
                        part(g_ent, b, n), tau, dz, pair);
       });
     }
@@ -883,9 +883,9 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
       Tensor unit = torch::empty({1}, s[0].options().dtype(at::kFloat));
       r = head_backward(ctx, s[0], s[1], unit, [&](int64_t b, int64_t n, const Tensor& dz) {
         std::vector<Tensor> rows;
-        for (int i = 5; i < 10; ++i) rows.push_back(s[i].narrow(0, b, n));
-        head_distill_grad(s[0].narrow(0, b, n), s[1], s[2].narrow(0, b, n), rows, s[3].narrow(0, b, n), s[4].narrow(0, b, n), part(s[10], s[11], b, n), g_ce, g_l2,
-                          g_kd, tau, dz, unit, pair);
+        for (int i = 5; i < 10; ++i) rows.push_back(part(s[i], b, n));
+        head_distill_grad(part(s[0], b, n), s[1], part(s[2], b, n), rows, part(s[3], b, n), part(s[4], b, n), part(s[10], s[11], b, n),
+                          g_ce, g_l2, g_kd, tau, dz, unit, pair);
       });
     }
     variable_list grads(12);
