@@ -369,8 +369,8 @@ constexpr int kOutStageBytes = 128 * 128;   // 128 rows x 64 bf16
 __device__ __forceinline__ void epilogue_named_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // 64 logits of this thread's row as fp16 distances below their largest, into a 16 KB staging buffer (128 rows x 128 bytes,
-// 128-byte swizzle).  What matters in a row is close to its maximum: a distance d carries an error of 2^-12 |d|, so q = 2^d
-// is off by less than the bf16 rounding of its gradient wherever q is more than a few percent of the largest.
+// 128-byte swizzle).  What matters in a row is close to its maximum: a distance d is off by at most 2^-11 |d|, and with it its
+// softmax term relatively, which is less than the 2^-8 of its gradient's rounding to bf16 for every d above -8 tau.
 __device__ __forceinline__ void stage_distances(const uint32_t (&v0)[32], const uint32_t (&v1)[32], float top, uint8_t* buf, int tile_row) {
   uint32_t pk[32];
 #pragma unroll

@@ -976,7 +976,8 @@ __global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const
   const float g_kd = one ? k.g_kd + k.g_ce : k.g_kd;
   const f2 c1v = pack2(kLog2e, kLog2e), nl1 = pack2(-k.l2s1, -k.l2s1), gk = pack2(g_kd, g_kd), gc = pack2(k.g_ce, k.g_ce);
   auto value2 = [&](uint32_t h, f2 below) {           // below: the group's largest logit minus the row's
-    const float2 zf = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    // a distance past fp16's range counts as its end: the exponential is zero there, and 0 * l has to stay finite
+    const float2 zf = __half22float2(__hmax2_nan(*reinterpret_cast<const __half2*>(&h), __floats2half2_rn(-65504.f, -65504.f)));
     const f2 d = add2(pack2(zf.x, zf.y), below), l = fma2(d, cc, nl);
     float l0, l1, r0, r1;
     unpack2(l, l0, l1);

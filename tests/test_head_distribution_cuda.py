@@ -224,6 +224,26 @@ def test_losses_of_one_kind_and_large_differences():
         _check_grads(got, want, torch.maximum(dz.abs(), mass * (4 * tol + 3000 * U)), tol, h, w, _kept_error(zd, mass, 1.0))
 
 
+def test_logits_far_apart():
+    """Distances between logits beyond 65504: probabilities of exactly 0 and 1, and gradients without a NaN."""
+    h, w, ids = _operands(20, 600, 64, seed=8)
+    big = (h.detach() * 65536).requires_grad_()
+    lp, ent = ops.head_token_logprobs(big, w, ids)
+    g = torch.autograd.grad((lp, ent), (big, w), (torch.ones_like(lp), torch.ones_like(lp)))
+    zmax = (big.detach().float() @ w.detach().float().T).abs().max()
+    assert float(zmax) > 2 * 65504
+    assert torch.isfinite(lp).all() and torch.isfinite(ent).all() and all(torch.isfinite(x).all() for x in g)
+    top = (big.detach().double() @ w.detach().double().T).argmax(-1)
+    sure = ops.head_token_logprobs(big, w, top)[0]
+    # the runner-up is far behind in nearly every row, so S is the maximum's own term: 2^(m c - fl(m c)), whose exponent is off by
+    # half a step of m c, 2^-24 |m| in natural units (m here is near 5e5, where fp32 logits themselves are 2^-5 apart)
+    assert float((sure >= -2 * U * float(zmax)).float().mean()) > 0.8
+    t_ids, t = _teacher(20, 600, 5, 1)
+    out = ops.head_distill_loss(big, w, ids, None, t_ids, t, temperature=2.0)
+    g = torch.autograd.grad(out[0] + out[4], (big, w))
+    assert all(torch.isfinite(x).all() for x in g)
+
+
 def test_several_chunks_and_main_gradient(monkeypatch):
     kk = _K()
     h, w, ids = _operands(150, 1003, 256)
