@@ -37,6 +37,13 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+using f2 = unsigned long long;     // two fp32 numbers for the packed instructions of sm_100
+__device__ __forceinline__ f2 pack2(float x, float y) { f2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y)); return r; }
+__device__ __forceinline__ void unpack2(f2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) { f2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
 // Unit in which a head's logit gradients are written as bf16: the larger of the two losses' upstream gradients.  The one-hot
 // terms that dominate every row then have few digits (1, or a ratio of the two), where g / count would round the same way in
 // every row, by up to 2^-8; the products put the unit back in fp32.

@@ -302,34 +302,48 @@ __device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, const uint32_t (
       st.am = col0 + ci;
     }
   }
-  const float mc = st.m * g.c, m1 = st.m * 1.4426950408889634f;
   const bool one = EPI == kEpiDistillStats && g.tau == 1.f;     // both temperatures are the same
-  float a[2] = {0.f, 0.f}, b[2] = {0.f, 0.f};
+  // z - m first: exact near the maximum, where the terms that count are
+  const f2 nm = pack2(-st.m, -st.m), cc = pack2(g.c, g.c), c1 = pack2(1.4426950408889634f, 1.4426950408889634f);
+  f2 a = 0ull, b = 0ull;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float z = __uint_as_float(v[j]);
-    float t = fmaf(z, g.c, -mc);
-    if (EPI == kEpiProbStats && ragged) t = fmaxf(t, -16384.f);       // 0 * t stays finite past the last column
-    const float e = ex2(t);
-    a[j & 1] += e;
-    if (EPI == kEpiProbStats) b[j & 1] = fmaf(e, t, b[j & 1]);
-    else if (!one) b[j & 1] += ex2(fmaf(z, 1.4426950408889634f, -m1));
+  for (int j = 0; j < 32; j += 2) {
+    const f2 d = add2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), nm);
+    f2 t = mul2(d, cc);
+    float x, y;
+    unpack2(t, x, y);
+    if (EPI == kEpiProbStats && ragged) {             // 0 * t stays finite past the last column
+      x = fmaxf(x, -16384.f);
+      y = fmaxf(y, -16384.f);
+      t = pack2(x, y);
+    }
+    const f2 e = pack2(ex2(x), ex2(y));
+    a = add2(a, e);
+    if (EPI == kEpiProbStats) b = fma2(e, t, b);
+    else if (!one) {
+      unpack2(mul2(d, c1), x, y);
+      b = add2(b, pack2(ex2(x), ex2(y)));
+    }
   }
-  st.s1 += a[0] + a[1];
+  float x, y;
+  unpack2(a, x, y);
+  st.s1 += x + y;
   if (EPI == kEpiDistillStats && one) st.s2 = st.s1;
-  else st.s2 += b[0] + b[1];
+  else { unpack2(b, x, y); st.s2 += x + y; }
 }
 
-// A row's factors of the gradient epilogues: dz = q (A + B log2 q) with log2 q = z c + b, or a1 2^(z log2e + b1) + a 2^(z c + b).
-// A row that nothing flows into has live = false and gets zeros, whatever its z.
-struct VocabCoef { float b, A, B, b1; bool live; };
+// A row's factors of the gradient epilogues: dz = q (A + B log2 q) with log2 q = (z - m) c - l, or with a second softmax
+// A q + B 2^((z - m) log2e - l1).  A row that nothing flows into has live = false and gets zeros, whatever its z.
+struct VocabCoef { float m, l, l1, A, B; bool live; };
 
 template <int EPI>
 __device__ __forceinline__ VocabCoef vocab_coef(int row, int M, int N, const GemmVocab& g) {
-  VocabCoef k{0.f, 0.f, 0.f, 0.f, false};
+  VocabCoef k{0.f, 0.f, 0.f, 0.f, 0.f, false};
   if (row >= M) return k;
   const float4 s = g.stat[row];
-  k.b = -fmaf(s.x, g.c, s.z);
+  k.m = s.x;
+  k.l1 = s.y;
+  k.l = s.z;
   if (EPI == kEpiProbGrad) {
     const int id = g.target[row];
     const float gl = g.g0 != nullptr && id >= 0 && id < N ? g.g0[row] : 0.f, gh = g.g1 != nullptr ? g.g1[row] : 0.f;
@@ -338,7 +352,6 @@ __device__ __forceinline__ VocabCoef vocab_coef(int row, int M, int N, const Gem
     k.live = gl != 0.f || gh != 0.f;
   } else {
     const float2 w = g.weight[row];
-    k.b1 = -fmaf(s.x, 1.4426950408889634f, s.y);
     const float unit = head_unit(g.g0, g.g1, g.tau);
     k.B = g.g0 != nullptr ? __fdiv_rn(g.g0[0], unit) * w.x : 0.f;             // cross-entropy
     k.A = g.g1 != nullptr ? __fdiv_rn(g.g1[0] * g.tau, unit) * w.y : 0.f;     // distillation: tau^2 / tau
@@ -349,13 +362,23 @@ __device__ __forceinline__ VocabCoef vocab_coef(int row, int M, int N, const Gem
 
 template <int EPI>
 __device__ __forceinline__ void vocab_grad_chunk(uint32_t (&v)[32], const VocabCoef& k, float c) {
+  const f2 nm = pack2(-k.m, -k.m), cc = pack2(c, c), nl = pack2(-k.l, -k.l), A = pack2(k.A, k.A), B = pack2(k.B, k.B);
+  const f2 c1 = pack2(1.4426950408889634f, 1.4426950408889634f), nl1 = pack2(-k.l1, -k.l1);
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float z = __uint_as_float(v[j]), l = fmaf(z, c, k.b);
-    float d;
-    if (EPI == kEpiProbGrad) d = ex2(l) * fmaf(k.B, l, k.A);
-    else d = fmaf(k.A, ex2(l), k.B * ex2(fmaf(z, 1.4426950408889634f, k.b1)));
-    v[j] = k.live ? __float_as_uint(d) : 0u;
+  for (int j = 0; j < 32; j += 2) {
+    const f2 d = add2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), nm), l = fma2(d, cc, nl);
+    float x, y;
+    unpack2(l, x, y);
+    const f2 q = pack2(ex2(x), ex2(y));
+    f2 r;
+    if (EPI == kEpiProbGrad) r = mul2(q, fma2(B, l, A));
+    else {
+      unpack2(fma2(d, c1, nl1), x, y);
+      r = fma2(A, q, mul2(B, pack2(ex2(x), ex2(y))));
+    }
+    unpack2(r, x, y);
+    v[j] = k.live ? __float_as_uint(x) : 0u;
+    v[j + 1] = k.live ? __float_as_uint(y) : 0u;
   }
 }
 
