@@ -304,6 +304,7 @@ struct GemmVocab {
   float inv_tau, tau;
   void* z; int ldz;        // statistics, or null: the logits are kept as well, fp16 distances [M, N] below the largest of every
   float* z_top;            // 64 columns (row pitch ldz a multiple of 8), and those [M, ceil(N / 64)]
+  int a_rows;              // set by the launcher: rows of the hidden states that a tile fetches
   int listed;              // columns per row in `cols` (kEpiDistillStats)
   const int* target;       // [M]: the column whose z goes to target_z (statistics)
   float* target_z;

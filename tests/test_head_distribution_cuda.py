@@ -145,6 +145,21 @@ def test_few_rows(M, V, C):
     _check_grads((g, None), (want, None), torch.maximum(dz.abs(), q * (4 * tol)), tol, h, w, _kept_error(zd, q / 0.7, 0.7))
 
 
+@pytest.mark.parametrize("M", [1, 7, 40, 100])
+def test_few_rows_after_rows_of_nan(M):
+    """What an earlier call left in shared memory stays out of the results: bit for bit the same after clean rows and NaN."""
+    h, w, ids = _operands(M, 9473, 1024, seed=M)
+    up = torch.ones(M, device="cuda")
+    out = []
+    for fill in (0.0, math.nan):
+        with torch.no_grad():
+            ops.head_token_logprobs(torch.full((128, 1024), fill, dtype=torch.bfloat16, device="cuda"), w, torch.zeros(128, dtype=torch.int32, device="cuda"))
+        lp, ent = ops.head_token_logprobs(h, w, ids)
+        out.append((lp, ent) + torch.autograd.grad((lp, ent), (h, w), (up, up)))
+    for a, b in zip(*out):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 def test_a_short_last_chunk():
     """More rows than one launch of the statistics takes."""
     h, w, ids = _operands(32768 + 3, 300, 64)
