@@ -783,14 +783,13 @@ void save_head(AutogradContext* ctx, const Tensor& hidden, const Tensor& w, cons
   ctx->saved_data["main"] = main;             // written in backward, so not a saved variable
   ctx->saved_data["grad_bytes"] = grad_bytes;
   ctx->saved_data["pair"] = pair;
-  ctx->saved_data["need_h"] = hidden.requires_grad();
-  ctx->saved_data["need_w"] = w.requires_grad();
 }
+// The hidden states and the weight are a node's first two inputs; a product whose gradient nobody asked for is left out.
 template <typename F>
 std::pair<Tensor, Tensor> head_backward(AutogradContext* ctx, const Tensor& h, const Tensor& wc, const Tensor& scale, F&& fill) {
   auto& d = ctx->saved_data;
   auto r = head_backward(h, wc, (at::ScalarType)d["w_type"].toInt(), d["main"].toOptional<Tensor>(), d["grad_bytes"].toInt(), d["pair"].toInt(),
-                         d["need_h"].toBool(), d["need_w"].toBool(), scale, fill);
+                         ctx->needs_input_grad(0), ctx->needs_input_grad(1), scale, fill);
   if (r.first.defined()) r.first = r.first.view(d["shape"].toIntVector());
   return r;
 }

@@ -298,6 +298,40 @@ def test_frozen_sides():
         assert not ops.head_token_logprobs(h, w, ids)[0].requires_grad
 
 
+def test_gradient_of_one_side_alone():
+    """Asking for the gradient of the hidden states leaves a bound main gradient of the head as it was."""
+    h, w, ids = _operands(70, 500, 128)
+    t_ids, t = _teacher(70, 500, 5, 3)
+    calls = (lambda head: ops.head_token_logprobs(h, head, ids)[0].sum(),
+             lambda head: ops.head_distill_loss(h, head, ids, None, t_ids, t)[4])
+    for call in calls:
+        both = torch.autograd.grad(call(w), (h, w))
+        assert torch.equal(both[0], torch.autograd.grad(call(w), (h,))[0])
+        assert torch.equal(both[1], torch.autograd.grad(call(w), (w,))[0])
+        held = w.detach().clone().requires_grad_()
+        held._main_grad = torch.full((500, 128), 0.5, device="cuda")
+        assert torch.equal(both[0], torch.autograd.grad(call(held), (h,))[0])
+        assert (held._main_grad == 0.5).all()
+
+
+def test_many_rows_of_a_small_vocabulary():
+    """More rows than a launch's second grid axis holds."""
+    M, V, C = 70001, 24, 16
+    h, w, ids = _operands(M, V, C)
+    lp, ent = ops.head_token_logprobs(h, w, ids)
+    got = torch.autograd.grad((lp[-40:].sum() + lp[:40].sum(),), (h, w))
+    hd, wd = _double(h, w)
+    zd = hd @ wd.T
+    ref = R.token_logprobs(zd, ids)
+    tol = _row_tol(h, w, zd, 1.0)
+    assert (lp - ref[0]).abs().max() <= tol
+    want = torch.autograd.grad((ref[0][-40:].sum() + ref[0][:40].sum(),), (hd, wd, zd))
+    q = torch.softmax(zd.detach(), -1)
+    terms = torch.zeros_like(q)
+    terms[-40:], terms[:40] = q[-40:], q[:40]
+    _check_grads(got, want, want[2], tol, h, w, kept=_kept_error(zd, terms, 1.0))
+
+
 def test_layouts_and_other_types():
     h, w, ids = _operands(48, 300, 64)
     want = ops.head_token_logprobs(h.detach(), w.detach(), ids)
