@@ -935,8 +935,8 @@ __global__ void __launch_bounds__(256) head_distill_fix_kernel(HeadFix a) {
 
 // Gradient from kept logits: fp16 distances in, bf16 out.  A thread takes 8 columns at a time (16 bytes in, 16 out), a CTA
 // `iters` blocks of 8192 columns, the next block's in flight while one is written.  Rows from the last to the first, as above.
-// Bound by memory and, with two temperatures, by two exponentials an element: 16384 x 65536 take 858 us, 5.0 TB/s; 4093 x
-// 65536 with one 164 us, 6.5 TB/s.
+// Bound by memory and, with two temperatures, by two exponentials an element: 16384 x 65536 take 811 us, 5.3 TB/s; 4093 x
+// 65536 with one 170 us, 6.3 TB/s.
 template <bool DISTILL>
 __global__ void __launch_bounds__(256, 4) head_grad_kept_kernel(HeadFix a, const __half* __restrict__ z, int64_t ldz,
                                                                 const float* __restrict__ z_top, int iters) {
@@ -1018,6 +1018,7 @@ int launch_grad_kept(const HeadFix& a, const void* z, int64_t ldz, const float* 
   if (a.rows > 65535 || (ldz & 7) || (a.ld & 7) || ldz < (a.V + 7) / 8 * 8 || a.ld < (a.V + 7) / 8 * 8) return 6;
   const int blocks = (a.V + 8191) / 8192;
   // as in row_grad; 16384 x 65536: 1331 us with one block per CTA, 1057 with two, 894 with four, 858 with eight
+  // (811 since it computes on pairs)
   int iters = 1;
   while (iters < 8 && iters < blocks && (int64_t)a.rows * blocks >= 2ll * iters * 4 * 148) iters *= 2;
   head_grad_kept_kernel<DISTILL><<<dim3((blocks + iters - 1) / iters, a.rows), 256, 0, st>>>(a, static_cast<const __half*>(z), ldz, z_top, iters);
