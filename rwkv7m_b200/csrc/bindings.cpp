@@ -312,7 +312,8 @@ Tensor logits_grad(const Tensor& logits, const Tensor& stats, const Tensor& ids,
   return d;
 }
 
-// ids int32 [R, K], logits bf16/fp32 [R, K] -> ids and probabilities sorted by id, {sum p ln p, any} per row
+// ids int32 [R, K], logits bf16/fp32 [R, K] -> ids and probabilities sorted by id, {sum p ln p, any} per row, and
+// where the ids enter each block of 256 columns
 std::vector<Tensor> teacher_prepare(const Tensor& ids, const Tensor& logits, int64_t V, double tau) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.is_contiguous() &&
                   (logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kFloat),
@@ -323,11 +324,13 @@ std::vector<Tensor> teacher_prepare(const Tensor& ids, const Tensor& logits, int
   check_rows(ids, logits, at::kInt, {R, K}, "teacher ids");
   auto f32 = logits.options().dtype(at::kFloat);
   Tensor oid = torch::empty({R, K}, f32.dtype(at::kInt)), p = torch::empty({R, K}, f32), row = torch::empty({R, 2}, f32);
+  Tensor first = torch::empty({R, (V + 255) / 256}, f32.dtype(at::kShort));
   TORCH_CHECK(rk::teacher_prepare(ids.data_ptr<int>(), logits.data_ptr(), logits.scalar_type() == at::kBFloat16, (int)R, (int)K,
                                   (int)V, (float)(1.0 / tau), oid.data_ptr<int>(), p.data_ptr<float>(),
-                                  reinterpret_cast<float2*>(row.data_ptr<float>()), stream()) == 0,
+                                  reinterpret_cast<float2*>(row.data_ptr<float>()),
+                                  reinterpret_cast<uint16_t*>(first.data_ptr<int16_t>()), stream()) == 0,
               "teacher_prepare launch failed");
-  return {oid, p, row};
+  return {oid, p, row, first};
 }
 
 // ids int32 [R, K], t_logits bf16/fp32 [R, K] -> stats [R, 2], the scalars sum of mask tau^2 KL and sum of mask, and the
@@ -470,8 +473,8 @@ void head_prob_grad(const Tensor& H, const Tensor& W, const Tensor& ids, const T
 // -> scalars ce_total, ce_count, l2_total, l2_count, kd_total, kd_count, then stat [M, 4], weight [M, 2], argmax, target z [M],
 // z of the teacher's alternatives [M, K], the kept logits
 std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const Tensor& targets, const c10::optional<Tensor>& mask,
-                                       const Tensor& t_ids, const Tensor& t_prob, const Tensor& t_row, double tau, int64_t pair,
-                                       bool keep) {
+                                       const Tensor& t_ids, const Tensor& t_prob, const Tensor& t_row, const Tensor& t_first,
+                                       double tau, int64_t pair, bool keep) {
   check_head(H, W, "head_distill_loss");
   c10::cuda::CUDAGuard guard(H.device());
   const int64_t M = H.size(0), V = W.size(0), K = t_ids.size(1), tiles = (V + 255) / 256;
@@ -479,6 +482,7 @@ std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const T
   check_rows(t_ids, H, at::kInt, {M, K}, "teacher ids");
   check_rows(t_prob, H, at::kFloat, {M, K}, "teacher probabilities");
   check_rows(t_row, H, at::kFloat, {M, 2}, "teacher rows");
+  check_rows(t_first, H, at::kShort, {M, tiles}, "teacher blocks");
   const float* msk = rows_ptr(mask, H, M, "mask");
   auto f32 = H.options().dtype(at::kFloat);
   Tensor stat = torch::empty({M, 4}, f32), weight = torch::empty({M, 2}, f32), am = torch::empty({M}, f32.dtype(at::kInt));
@@ -496,6 +500,7 @@ std::vector<Tensor> head_distill_stats(const Tensor& H, const Tensor& W, const T
     p.vocab.listed = (int)K;
     p.vocab.cols = t_ids.data_ptr<int>() + r * K;
     p.vocab.cols_z = cz.data_ptr<float>() + r * K;
+    p.vocab.first = reinterpret_cast<const uint16_t*>(t_first.data_ptr<int16_t>()) + r * tiles;
     const int rc = rk::gemm_bf16(p, stream());
     TORCH_CHECK(rc == 0, "head_distill_loss: product launch failed with code ", rc);
     rk::HeadDistillRows a{};
@@ -855,7 +860,7 @@ struct HeadDistillLoss : torch::autograd::Function<HeadDistillLoss> {
     Tensor h = aligned_rows(vocab_rows(hidden)), wc = aligned_rows(wc_in), tgt = id_rows(targets);
     const std::pair<Tensor, Tensor> raw = teacher_rows(t_ids, t_logits);
     const std::vector<Tensor> t = teacher_prepare(raw.first, raw.second, wc.size(0), tau);
-    std::vector<Tensor> out = head_distill_stats(h, wc, tgt, mask_rows(mask), t[0], t[1], t[2], tau, pair,
+    std::vector<Tensor> out = head_distill_stats(h, wc, tgt, mask_rows(mask), t[0], t[1], t[2], t[3], tau, pair,
                                                  ctx != nullptr && keeps(h, wc, keep_bytes));
     if (ctx != nullptr) {
       save_head(ctx, hidden, w, main, tau, grad_bytes, pair);

@@ -216,6 +216,11 @@ __device__ __forceinline__ void* plane_of(void* D, int split, int M, int ldd) {
 
 template <int EPI> constexpr bool kVocabEpilogue =
     EPI == kEpiProbStats || EPI == kEpiDistillStats || EPI == kEpiProbGrad || EPI == kEpiDistillGrad;
+// The statistics epilogues have two groups of four warps, one per accumulator: alone on its scheduler, a warp waits for its own
+// latencies most of the time.  512 rows x 65536 columns of 64 terms, logits kept: 37 us with one group, 28 with two (with a teacher
+// of 16 alternatives 54 and 40); of 768 terms 53 and 51 (70 and 60); from 1536 terms on the tensor cores decide.
+template <int EPI> constexpr int kEpiGroups = EPI == kEpiProbStats || EPI == kEpiDistillStats ? 2 : 1;
+template <int EPI> constexpr int kThreadsOf = 64 + 128 * kEpiGroups<EPI>;
 template <int EPI> constexpr bool kScales = EPI == kEpiStoreBf16 || EPI == kEpiStoreF32 || EPI == kEpiAccumF32;
 
 __device__ __forceinline__ void scale_chunk(uint32_t (&v)[32], float sc) {
@@ -265,8 +270,23 @@ __device__ __forceinline__ float pick32(const uint32_t (&v)[32], int off) {
 // temperature 1 next to s1 at tau (kEpiDistillStats).
 struct VocabRow {
   float m, s1, s2;
-  int am, k, next, tgt;
+  int am, k, next, after, tgt;      // next, after: the teacher's k-th and k + 1-st column
 };
+
+// What a row brings to a tile, asked for before the tile's product is there.
+template <int EPI>
+__device__ __forceinline__ VocabRow vocab_row(int row, int M, int n0, int N, const GemmVocab& g) {
+  VocabRow st{-INFINITY, 0.f, 0.f, 0, 0, 0x7fffffff, 0x7fffffff, -1};
+  if (row >= M) return st;
+  st.tgt = g.target[row];
+  if (EPI == kEpiDistillStats) {
+    const int* cols = g.cols + (size_t)row * g.listed;
+    st.k = g.first[(size_t)row * ((N + 255) >> 8) + (n0 >> 8)];
+    if (st.k < g.listed) st.next = cols[st.k];
+    if (st.k + 1 < g.listed) st.after = cols[st.k + 1];
+  }
+  return st;
+}
 
 // columns past the last one take no part
 __device__ __forceinline__ void vocab_mask_columns(uint32_t (&v)[32], int col0, int N) {
@@ -286,7 +306,8 @@ __device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, const uint32_t (
     while (st.next < col0 + 32) {          // the teacher's alternatives come in the order of the columns
       g.cols_z[row * g.listed + st.k] = pick32(v, st.next - col0);
       ++st.k;
-      st.next = st.k < g.listed ? g.cols[row * g.listed + st.k] : 0x7fffffff;
+      st.next = st.after;                   // on its way since the last one
+      st.after = st.k + 1 < g.listed ? g.cols[row * g.listed + st.k + 1] : 0x7fffffff;
     }
   }
   if (cm > st.m) {
@@ -298,10 +319,13 @@ __device__ __forceinline__ void vocab_stats_chunk(VocabRow& st, const uint32_t (
     }
     st.m = cm;
     if (EPI == kEpiDistillStats) {
-      int ci = 31;
+      int ci[4] = {31, 31, 31, 31};         // the lowest column among equal values, in four chains
 #pragma unroll
-      for (int j = 30; j >= 0; --j) ci = __uint_as_float(v[j]) == cm ? j : ci;   // the lowest column among equal values
-      st.am = col0 + ci;
+      for (int j = 7; j >= 0; --j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ci[q] = __uint_as_float(v[8 * q + j]) == cm ? 8 * q + j : ci[q];
+      }
+      st.am = col0 + min(min(ci[0], ci[1]), min(ci[2], ci[3]));
     }
   }
   const bool one = EPI == kEpiDistillStats && g.tau == 1.f;     // both temperatures are the same
@@ -391,7 +415,7 @@ __device__ __forceinline__ void vocab_grad_chunk(uint32_t (&v)[32], const VocabC
 // that precedes the next one, so a buffer is free again by the time the warps return to it.
 constexpr int kOutStageBytes = 128 * 128;   // 128 rows x 64 bf16
 
-__device__ __forceinline__ void epilogue_named_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void epilogue_named_barrier(int id = 1) { asm volatile("bar.sync %0, 128;" :: "r"(id) : "memory"); }
 
 // 64 logits of this thread's row as fp16 distances below their largest, into a 16 KB staging buffer (128 rows x 128 bytes,
 // 128-byte swizzle).  What matters in a row is close to its maximum: a distance d is off by at most 2^-11 |d|, and with it its
@@ -421,26 +445,13 @@ __device__ __forceinline__ float max32(const uint32_t (&v)[32]) {
 }
 
 // Statistics of this thread's row over the 256 columns of a tile, from the accumulator at taddr.  With `tm` not null the
-// logits are kept as well, 64 columns at a time: the largest in fp32, the distances below it through the staging buffers.
+// logits are kept as well, 64 columns at a time: the largest in fp32, the distances below it through the group's one staging
+// buffer (its last store had the time of 64 columns' statistics to be read).
 template <int EPI>
-__device__ __forceinline__ void vocab_stats_tile(uint32_t taddr, int m0, int tile_row, int n0, int N, int M, float4* __restrict__ out,
-                                                 const GemmVocab& g, const CUtensorMap* tm, uint8_t* out_stage, int& obuf, bool issuer) {
+__device__ __forceinline__ void vocab_stats_tile(VocabRow st, uint32_t taddr, int m0, int tile_row, int n0, int N, int M, float4* __restrict__ out,
+                                                 const GemmVocab& g, const CUtensorMap* tm, uint8_t* buf, int barrier, bool issuer) {
   const int row = m0 + tile_row;
   const bool live = row < M;
-  VocabRow st{-INFINITY, 0.f, 0.f, 0, 0, 0x7fffffff, -1};
-  if (live) {
-    st.tgt = g.target[row];
-    if (EPI == kEpiDistillStats) {
-      const int* cols = g.cols + (size_t)row * g.listed;
-      int lo = 0, hi = g.listed;             // first listed column at or right of this tile
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (cols[mid] < n0) lo = mid + 1; else hi = mid;
-      }
-      st.k = lo;
-      if (lo < g.listed) st.next = cols[lo];
-    }
-  }
 #pragma unroll 1
   for (int c = 0; c < 8; c += 2) {
     uint32_t v0[32], v1[32];
@@ -452,14 +463,13 @@ __device__ __forceinline__ void vocab_stats_tile(uint32_t taddr, int m0, int til
     vocab_mask_columns(v1, c0 + 32, N);
     const float m0c = max32(v0), m1c = max32(v1);
     if (tm != nullptr && m0 < M && c0 < N) {           // the same for all 128 threads
-      uint8_t* buf = out_stage + obuf * kOutStageBytes;
       const float top = fmaxf(m0c, m1c);
+      if (issuer) tma_store_wait_read<0>();
+      epilogue_named_barrier(barrier);
       stage_distances(v0, v1, top, buf, tile_row);
       if (live) g.z_top[(size_t)row * ((N + 63) / 64) + c0 / 64] = top;
-      if (issuer) tma_store_wait_read<0>();           // the other buffer, before the next round writes it
-      epilogue_named_barrier();
+      epilogue_named_barrier(barrier);
       if (issuer) { tma_store_2d(tm, buf, c0, m0); tma_store_commit(); }
-      obuf ^= 1;                                      // over the tiles too: a ragged tile may end on either buffer
     }
     vocab_stats_chunk<EPI>(st, v0, m0c, c0, N, (size_t)row, g);
     vocab_stats_chunk<EPI>(st, v1, m1c, c0 + 32, N, (size_t)row, g);
@@ -532,7 +542,7 @@ struct Tile {
 };
 
 template <int BN, int A_MN, int B_MN, int EPI>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreadsOf<EPI>, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmD, int tma_out,
                  void* __restrict__ Dptr, int M, int N, int K, int ldd, int raster_m, int splits,
@@ -646,22 +656,26 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   } else {
     // ---------------- epilogue ----------------
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    int acc = 0; uint32_t acc_phase = 0;
+    constexpr int kGroups = kEpiGroups<EPI>;
+    const int group = kGroups == 2 ? (warp - 2) >> 2 : 0;     // with two, a group takes every second tile and its accumulator
+    int acc = group; uint32_t acc_phase = 0;
     bool ok = true;
     const bool atomic = splits > 1;
     constexpr bool kTwoInput = EPI == kEpiMulSqrt2Bf16 || EPI == kEpiAddBf16;
     constexpr bool kVocabGrad = EPI == kEpiProbGrad || EPI == kEpiDistillGrad;     // always staged: the host insists on it
     constexpr bool kCanStage = (EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput || kVocabGrad) && BN >= 64;
     const bool staged = kCanStage && tma_out != 0;
-    const bool issuer = warp == 2 && lane == 0;   // the one thread whose bulk groups track the output stores
+    const bool issuer = warp == 2 + 4 * group && lane == 0;   // the one thread whose bulk groups track the group's output stores
     int obuf = 0;
-    for (int work = blockIdx.x; work < num_work && ok; work += gridDim.x) {
+    for (int work = blockIdx.x + group * gridDim.x; work < num_work && ok; work += kGroups * gridDim.x) {
       int tm, tn;
       tile_coords(work % num_tiles, tiles_m, tiles_n, raster_m, tm, tn);
       const int m0 = tm * BM, n0 = tn * BN;
+      const int row = m0 + q * 32 + lane;
+      VocabRow vrow;
+      if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) vrow = vocab_row<EPI>(row, M, n0, N, vocab);
       if (!wait_bar(&tfull_bar[acc], acc_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      const int row = m0 + q * 32 + lane;
       const uint32_t t0 = tmem_base + (uint32_t(q * 32) << 16) + acc * BN;
       const float sc = kScales<EPI> && vocab.scale != nullptr ? *vocab.scale : 1.f;
       if constexpr (EPI == kEpiCeStats) {
@@ -679,8 +693,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (row < M)
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
       } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
-        vocab_stats_tile<EPI>(t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
-                              tma_out != 0 ? &tmD : nullptr, out_stage, obuf, issuer);
+        vocab_stats_tile<EPI>(vrow, t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
+                              tma_out != 0 ? &tmD : nullptr, out_stage + group * kOutStageBytes, 1 + group, issuer);
       } else if constexpr (BN >= 64) {
         VocabCoef coef;
         if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
@@ -728,7 +742,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty_bar[acc]);
-      acc ^= 1; if (acc == 0) acc_phase ^= 1u;
+      if (kGroups == 1) acc ^= 1;
+      if (acc == group) acc_phase ^= 1u;
     }
     if ((staged || ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && tma_out != 0)) && issuer)
       tma_store_wait<0>();   // the staging buffers are read until the last store has drained
@@ -948,7 +963,7 @@ struct PairTile {
 };
 
 template <int A_MN, int B_MN, int EPI>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsOf<EPI>, 1)
 gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                       const __grid_constant__ CUtensorMap tmD, int tma_out,
                       void* __restrict__ Dptr, int M, int N, int K, int ldd, int raster_m, int splits,
@@ -1072,22 +1087,26 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   } else {
     // ---------------- epilogue (both CTAs, own 128 rows x 256 columns) ----------------
     const int q = warp & 3;
-    int acc = 0; uint32_t acc_phase = 0;
+    constexpr int kGroups = kEpiGroups<EPI>;
+    const int group = kGroups == 2 ? (warp - 2) >> 2 : 0;
+    int acc = group; uint32_t acc_phase = 0;
     bool ok = true;
     constexpr bool kTwoInput = EPI == kEpiMulSqrt2Bf16 || EPI == kEpiAddBf16;
     constexpr bool kVocabGrad = EPI == kEpiProbGrad || EPI == kEpiDistillGrad;
     constexpr bool kCanStage = EPI == kEpiStoreBf16 || EPI == kEpiReluSqBf16 || kTwoInput || kVocabGrad;
     const bool staged = kCanStage && tma_out != 0;
-    const bool issuer = warp == 2 && lane == 0;
+    const bool issuer = warp == 2 + 4 * group && lane == 0;
     int obuf = 0;
     const bool atomic = splits > 1;
-    for (int work = pair_id; work < num_work && ok; work += num_pairs) {
+    for (int work = pair_id + group * num_pairs; work < num_work && ok; work += kGroups * num_pairs) {
       int tm, tn;
       tile_coords(work % num_tiles, tiles_m, tiles_n, raster_m, tm, tn);
       const int m0 = tm * 2 * BM + (int)cta * BM, n0 = tn * BN2;
+      const int row = m0 + q * 32 + lane;
+      VocabRow vrow;
+      if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) vrow = vocab_row<EPI>(row, M, n0, N, vocab);
       if (!wait_bar(&tfull_bar[acc], acc_phase, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      const int row = m0 + q * 32 + lane;
       const uint32_t t0 = tmem_base + (uint32_t(q * 32) << 16) + acc * BN2;
       const float sc = kScales<EPI> && vocab.scale != nullptr ? *vocab.scale : 1.f;
       if constexpr (EPI == kEpiCeStats) {
@@ -1105,8 +1124,8 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
         if (row < M)
           reinterpret_cast<float4*>(Dptr)[(size_t)row * (ldd / 4) + tn] = make_float4(st.m, st.s, __int_as_float(st.am), st.tl);
       } else if constexpr (EPI == kEpiProbStats || EPI == kEpiDistillStats) {
-        vocab_stats_tile<EPI>(t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
-                              tma_out != 0 ? &tmD : nullptr, out_stage, obuf, issuer);
+        vocab_stats_tile<EPI>(vrow, t0, m0, q * 32 + lane, n0, N, M, reinterpret_cast<float4*>(Dptr) + (size_t)row * (ldd / 4) + tn, vocab,
+                              tma_out != 0 ? &tmD : nullptr, out_stage + group * kOutStageBytes, 1 + group, issuer);
       } else {
       VocabCoef coef;
       if constexpr (kVocabGrad) coef = vocab_coef<EPI>(row, M, N, vocab);
@@ -1144,7 +1163,8 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[acc]), 0));
-      acc ^= 1; if (acc == 0) acc_phase ^= 1u;
+      if (kGroups == 1) acc ^= 1;
+      if (acc == group) acc_phase ^= 1u;
     }
     if ((staged || ((EPI == kEpiProbStats || EPI == kEpiDistillStats) && tma_out != 0)) && issuer) tma_store_wait<0>();
     if (!ok && lane == 0) { *abort_flag = 1; atomicExch(err, 0x30000 | 3); }
@@ -1341,7 +1361,7 @@ int launch(const GemmArgs& p, cudaStream_t st) {
   const int work = tiles * splits;
   const int grid = work < sm_count() ? work : sm_count();
   RK_TRACE("attr ok grid=%d smem=%d splits=%d\n", grid, TL::kSmemBytes, splits);
-  kern<<<grid, kThreads, TL::kSmemBytes, st>>>(ta, tb, td, tma_out, p.D, p.M, p.N, p.K, p.ldd, raster_rows(p), splits, p.aux,
+  kern<<<grid, kThreadsOf<EPI>, TL::kSmemBytes, st>>>(ta, tb, td, tma_out, p.D, p.M, p.N, p.K, p.ldd, raster_rows(p), splits, p.aux,
                                                p.ldaux, p.act, vocab, p.error_flag);
   RK_TRACE("launched\n");
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
@@ -1449,7 +1469,7 @@ int launch_pair(const GemmArgs& p, cudaStream_t st) {
   if (EPI == kEpiStoreF32 && p.planes > 1) splits = p.planes;
   const int work = tiles * splits;
   const int pairs = work < max_pairs ? work : max_pairs;
-  kern<<<2 * pairs, kThreads, TL::kSmemBytes, st>>>(ta, tb, td, tma_out, p.D, p.M, p.N, p.K, p.ldd, raster_rows(p), splits,
+  kern<<<2 * pairs, kThreadsOf<EPI>, TL::kSmemBytes, st>>>(ta, tb, td, tma_out, p.D, p.M, p.N, p.K, p.ldd, raster_rows(p), splits,
                                                     p.aux, p.ldaux, p.act, p.vocab, p.error_flag);
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }

@@ -138,9 +138,10 @@ struct RowGradArgs {
   int K; const int* ids; const float* w; // [rows, K] sparse part; ids outside [0, V) are skipped
 };
 int row_grad(const RowGradArgs& a, cudaStream_t st);
-// Teacher's alternatives -> probabilities sorted by id (absent ones last, id INT_MAX), {sum p ln p, any} per row.
+// Teacher's alternatives -> probabilities sorted by id (absent ones last, id INT_MAX), {sum p ln p, any} per row, and first
+// [rows, ceil(V / 256)]: how many ids lie left of each block of 256 columns.
 int teacher_prepare(const int* ids, const void* logits, bool logits_bf16, int rows, int K, int V, float inv_tau, int* out_ids,
-                    float* out_p, float2* out_row, cudaStream_t st);
+                    float* out_p, float2* out_row, uint16_t* first, cudaStream_t st);
 // *out[i] = sum of in[i] over the rows (the row count where in[i] is null)
 constexpr int kMaxTotals = 6;
 struct RowTotalsArgs {
@@ -310,6 +311,7 @@ struct GemmVocab {
   float* target_z;
   const int* cols;         // [M, listed] in rising order, INT_MAX where there is none: their z goes to cols_z
   float* cols_z;
+  const uint16_t* first;   // [M, ceil(N / 256)]: how many of them lie left of each tile
   const float4* stat;      // [M] gradients: {max, log2 S at temperature 1, log2 S at tau, entropy}
   const float2* weight;    // [M] kEpiDistillGrad: weights of the cross-entropy and of the distillation term
   const float* g0;         // upstream gradients: [M] of the log-probability, or the scalar of the cross-entropy; null = 0
